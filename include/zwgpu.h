@@ -566,6 +566,154 @@ ZWG_API int zwg_gemm_f16(const uint16_t* a, size_t lda, size_t a_bs, const uint1
                          size_t K, size_t n_batch, const float* bias, int gelu, const float* addend, size_t ld_add,
                          int accumulate, void* out, int out_type, size_t ld_out, size_t out_bs, void* stream);
 
+/* ---- a decode step over a cache in 8 bits ------------------------------------------------
+ * No reference counterpart (the reference's caches are f32): rotary positions of any layout,
+ * a key/value cache of int8 values with one f32 scale for each block of 32 tokens and kv
+ * head, the attention that reads it, and the rules on a step's logits. It holds a sequence in
+ * a quarter of the f32 caches' memory, and a decode step reads a quarter of their bytes. All
+ * buffers are device pointers; the calls allocate nothing, launch on `stream` and may be
+ * captured into a graph. They run on the calling thread's device (zwg_init), whatever the
+ * current device is. */
+#define ZWG_TYPE_F32 0
+#define ZWG_TYPE_BF16 2
+
+/* The tokens of one call: token i of sequence b is at position p = n_past + i, or past[b] + i
+ * where `past` (device int32 [n_batch]) is given; n_past is then the most that past[b] may
+ * be. count (device int32 [n_batch], or NULL): sequence b has count[b] <= n tokens in this
+ * call, and rows i >= count[b] of every buffer are neither read nor written. first (device
+ * int32 [n_batch], or NULL; zwg_kv8_attn only): keys before first[b] are not seen (a batch
+ * padded on the left). A sequence whose past[b], count[b] or first[b] is out of range (below 0,
+ * past[b] > n_past, count[b] > n, beyond the cache or the tables) is skipped: its rows stay as
+ * they were, and the device error word is set (reported by zwg_sync). */
+typedef struct zwg_seqs {
+    size_t n_batch;
+    size_t n;
+    size_t n_past;
+    const int32_t* past;
+    const int32_t* count;
+    const int32_t* first;
+} zwg_seqs;
+
+/* Rows of a call: the head h of token i of sequence b is the d consecutive elements at
+ * data + b * batch_stride + i * token_stride + h * d (strides in elements), so the three
+ * parts of a packed q|k|v row need no copy. */
+typedef struct zwg_rows {
+    void* data;
+    size_t batch_stride;
+    size_t token_stride;
+} zwg_rows;
+
+/* Rotary tables: cos and sin [n_ctx][rot / 2] f32. The first `rot` elements of a head are
+ * rotated (even, at most d), the rest stay. Pair i is (i, i + rot/2), or (2i, 2i + 1) with
+ * `interleaved`. Scaling for long contexts is a matter of the tables. */
+typedef struct zwg_rope_tables {
+    const float* cos;
+    const float* sin;
+    size_t n_ctx;
+    size_t rot;
+    int32_t interleaved;
+} zwg_rope_tables;
+
+/* Rotate q [n_head heads] and, where k is given, k [n_head_kv heads] of every token of `s`
+ * to its position: a' = a cos - b sin, b' = a sin + b cos in f32 with separately rounded
+ * products and sums (as zwg_rope_kt_append), one rounding to `type` at the end. q_out and
+ * k_out take the result; NULL rotates in place. An output may be its input, but may not
+ * overlap it in another way. */
+ZWG_API int zwg_rope(const zwg_seqs* s, const zwg_rope_tables* t, int type, size_t d, size_t n_head, const zwg_rows* q,
+                     const zwg_rows* q_out, size_t n_head_kv, const zwg_rows* k, const zwg_rows* k_out, void* stream);
+
+/* A cache of n_batch sequences of up to n_ctx tokens (a multiple of 32), d 64 or 128:
+ *   k        int8 [n_batch][n_head_kv][n_ctx/32][32][d]      (16-byte aligned)
+ *   v        int8 [n_batch][n_head_kv][n_ctx/32][d][32]      (16-byte aligned)
+ *   k_scale, v_scale  f32 [n_batch][n_head_kv][n_ctx/32]
+ *   k_open, v_open    f32 [n_batch][n_head_kv][32][d]        (16-byte aligned)
+ *   open_block        int32 [n_batch][n_head_kv], -1 in an empty cache
+ * A block's scale is the largest magnitude of its tokens' 32 x d values / 127, and its int8
+ * values are round-to-nearest-even(127 x / largest). While a block fills, its rows are kept
+ * in f32 as well (k_open, v_open of block open_block), and its int8 values come from those
+ * rows at every append: the cache does not depend on how its tokens were split into calls.
+ * Appending inside a block that is no longer open (a sequence cut back to an earlier length)
+ * goes on from the values the cache holds. A block that takes in an infinity or a NaN reads
+ * as NaN, and so does every query that sees it, until it is filled anew. */
+typedef struct zwg_kv8 {
+    int8_t* k;
+    float* k_scale;
+    int8_t* v;
+    float* v_scale;
+    float* k_open;
+    float* v_open;
+    int32_t* open_block;
+    size_t n_batch, n_head_kv, d, n_ctx;
+} zwg_kv8;
+
+/* Append k and v of the call's tokens (heads n_head_kv, `type`), which end the sequences: what
+ * a sequence held from its position on is replaced. With rope, k is rotated on the way in
+ * (as zwg_rope, kept in f32). One call at a time on a cache. */
+ZWG_API int zwg_kv8_append(const zwg_kv8* c, const zwg_seqs* s, int type, const zwg_rows* k, const zwg_rows* v,
+                           const zwg_rope_tables* rope, void* stream);
+
+/* The values the cache stands for (int8 * scale) at the call's positions: k, v
+ * [n_batch][n][n_head_kv][d] f32, either may be NULL. */
+ZWG_API int zwg_kv8_read(const zwg_kv8* c, const zwg_seqs* s, float* k, float* v, void* stream);
+
+/* Bytes of workspace zwg_kv8_attn needs (0: none). */
+ZWG_API size_t zwg_kv8_attn_workspace(const zwg_kv8* c, const zwg_seqs* s, size_t n_head);
+
+/* Attention of the call's queries (n_head a multiple of n_head_kv; query head h reads kv head
+ * h / (n_head / n_head_kv)) over the cache: query i of sequence b sees keys first[b] .. p, its
+ * own token included, so the call's tokens are appended before it. Softmax of q . k / sqrt(d)
+ * in f32, sums in f32. A query that sees no key gives zeros. The context's math mode applies to
+ * f32 queries: ZWG_MATH_F32 holds each query and probability in two f16 pieces (22 bits)
+ * against the exact int8 values, ZWG_MATH_TF32 in one (11 bits, as that mode's operands);
+ * bf16 queries are exact in one piece. The workspace belongs to one call at a time: calls that
+ * may overlap (other streams, graphs replayed side by side) need their own. */
+ZWG_API int zwg_kv8_attn(const zwg_kv8* c, const zwg_seqs* s, int type, size_t n_head, const zwg_rows* q,
+                         const zwg_rows* out, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The rules on a step's logits. For each row, in this order and in f32:
+ *   1. a token that is c > 0 times among the row's last `window` recent tokens: x / repeat
+ *      (x > 0) or x * repeat (otherwise), once however often it is there (zwg_llm_greedy
+ *      repeats it); then x - (c * frequency + presence);
+ *   2. x + bias[j] for each j with bias_ids[j] = the token, their sum taken in the order of j;
+ *   3. -inf where the token's bit in `allow` is 0 (token t: bit t % 32 of word t / 32).
+ * recent: device int32, row r at recent + r * recent_stride, its tokens 0 .. n_recent, or
+ * 0 .. n_recents[r] where that (device int32 [m]) is given; negative entries are padding.
+ * bias_ids, bias: n_bias entries (at most 4096), row r's at r * bias_stride (0: one list for
+ * all rows). allow: row r's words at allow + r * allow_stride (0: one mask for all rows), NULL:
+ * all are allowed. An id of n_vocab or more, in either list, or a negative bias id is left out
+ * and sets the device error word; n_recents[r] is clamped to 0 .. n_recent in the same way. */
+typedef struct zwg_logit_rules {
+    const int32_t* recent;
+    size_t recent_stride;
+    size_t n_recent;
+    const int32_t* n_recents;
+    size_t window;
+    float repeat, presence, frequency;
+    const int32_t* bias_ids;
+    const float* bias;
+    size_t n_bias, bias_stride;
+    const uint32_t* allow;
+    size_t allow_stride;
+} zwg_logit_rules;
+#define ZWG_MAX_BIAS 4096
+
+/* Apply the rules to m rows of logits (device f32, row r at logits + r * stride, in place);
+ * where out is given, out[r * out_stride] = the first index of the row's largest logit, or -1
+ * where none is above -inf (a mask that leaves nothing; NaN is never the largest). */
+ZWG_API int zwg_llm_logits(float* logits, size_t m, size_t n_vocab, size_t stride, const zwg_logit_rules* rules,
+                           int32_t* out, size_t out_stride, void* stream);
+
+/* An LLM state whose layers keep their keys and values in 8 bits (zwg_kv8), for calls of up to
+ * n_chunk tokens. Every zwg_llm_* call on a state takes it (d 64 or 128, n_ctx a multiple of 32);
+ * zwg_llm_state_cache does not, zwg_llm_state_kv8 gives a layer's cache instead. */
+ZWG_API int zwg_llm_state_create_kv8(size_t n_layer, size_t n_batch, size_t n_head, size_t n_head_kv, size_t d,
+                                     size_t n_ctx, size_t n_chunk, double rope_base, zwg_llm_state** out);
+ZWG_API int zwg_llm_state_kv8(const zwg_llm_state* st, size_t layer, zwg_kv8* out);
+
+/* Replace the rotary tables of a state (either kind) by the caller's: cos and sin [n_ctx][d/2]
+ * f32, host or device, copied on `stream`. For contexts scaled beyond the training length. */
+ZWG_API int zwg_llm_state_set_rope(zwg_llm_state* st, const float* cos, const float* sin, void* stream);
+
 /* Self-test of the timeout path every kernel relies on: launches one bounded device-side
  * wait on a barrier nothing ever completes (a few seconds), then synchronizes. Returns
  * ZWG_TIMEOUT when the wait ran out, was reported through the error word and left the

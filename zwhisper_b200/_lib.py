@@ -18,6 +18,8 @@ ZWG_TIMEOUT = 4
 ZWG_MATH_F32 = 0
 ZWG_MATH_BF16 = 1
 ZWG_MATH_TF32 = 2
+ZWG_TYPE_F32 = 0
+ZWG_TYPE_BF16 = 2
 
 c_size = ctypes.c_size_t
 c_ptr = ctypes.c_void_p
@@ -129,6 +131,42 @@ class EncWeightsC(ctypes.Structure):
     ]
 
 
+class SeqsC(ctypes.Structure):
+    """zwg_seqs: the tokens of a call; past, count and first are device pointers or None."""
+
+    _fields_ = [("n_batch", c_size), ("n", c_size), ("n_past", c_size), ("past", c_ptr), ("count", c_ptr),
+                ("first", c_ptr)]
+
+
+class RowsC(ctypes.Structure):
+    """zwg_rows: rows of heads, strides in elements."""
+
+    _fields_ = [("data", c_ptr), ("batch_stride", c_size), ("token_stride", c_size)]
+
+
+class RopeTablesC(ctypes.Structure):
+    """zwg_rope_tables: cos and sin [n_ctx][rot / 2] f32 on the device."""
+
+    _fields_ = [("cos", c_ptr), ("sin", c_ptr), ("n_ctx", c_size), ("rot", c_size), ("interleaved", ctypes.c_int32)]
+
+
+class Kv8C(ctypes.Structure):
+    """zwg_kv8: a cache in 8 bits."""
+
+    _fields_ = [("k", c_ptr), ("k_scale", c_ptr), ("v", c_ptr), ("v_scale", c_ptr), ("k_open", c_ptr),
+                ("v_open", c_ptr), ("open_block", c_ptr), ("n_batch", c_size), ("n_head_kv", c_size), ("d", c_size),
+                ("n_ctx", c_size)]
+
+
+class LogitRulesC(ctypes.Structure):
+    """zwg_logit_rules: penalties, biases and mask of a step's logits."""
+
+    _fields_ = [("recent", c_ptr), ("recent_stride", c_size), ("n_recent", c_size), ("n_recents", c_ptr),
+                ("window", c_size), ("repeat", ctypes.c_float), ("presence", ctypes.c_float),
+                ("frequency", ctypes.c_float), ("bias_ids", c_ptr), ("bias", c_ptr), ("n_bias", c_size),
+                ("bias_stride", c_size), ("allow", c_ptr), ("allow_stride", c_size)]
+
+
 # name -> (restype, argtypes); every symbol include/zwgpu.h declares
 SIGNATURES = {
     "zwg_version": (ctypes.c_int, []),
@@ -206,6 +244,20 @@ SIGNATURES = {
     "zwg_gemm_f16": (ctypes.c_int, [c_ptr, c_size, c_size, c_ptr, c_size, c_size, c_size, c_size, c_size, c_ptr,
                                     ctypes.c_int, c_ptr, c_size, ctypes.c_int, c_ptr, ctypes.c_int, c_size, c_size,
                                     c_ptr]),
+    "zwg_rope": (ctypes.c_int, [ctypes.POINTER(SeqsC), ctypes.POINTER(RopeTablesC), ctypes.c_int, c_size, c_size,
+                                ctypes.POINTER(RowsC), ctypes.POINTER(RowsC), c_size, ctypes.POINTER(RowsC),
+                                ctypes.POINTER(RowsC), c_ptr]),
+    "zwg_kv8_append": (ctypes.c_int, [ctypes.POINTER(Kv8C), ctypes.POINTER(SeqsC), ctypes.c_int, ctypes.POINTER(RowsC),
+                                      ctypes.POINTER(RowsC), ctypes.POINTER(RopeTablesC), c_ptr]),
+    "zwg_kv8_read": (ctypes.c_int, [ctypes.POINTER(Kv8C), ctypes.POINTER(SeqsC), c_ptr, c_ptr, c_ptr]),
+    "zwg_kv8_attn_workspace": (c_size, [ctypes.POINTER(Kv8C), ctypes.POINTER(SeqsC), c_size]),
+    "zwg_kv8_attn": (ctypes.c_int, [ctypes.POINTER(Kv8C), ctypes.POINTER(SeqsC), ctypes.c_int, c_size,
+                                    ctypes.POINTER(RowsC), ctypes.POINTER(RowsC), c_ptr, c_size, c_ptr]),
+    "zwg_llm_logits": (ctypes.c_int, [c_ptr, c_size, c_size, c_size, ctypes.POINTER(LogitRulesC), c_ptr, c_size,
+                                      c_ptr]),
+    "zwg_llm_state_create_kv8": (ctypes.c_int, [c_size] * 7 + [ctypes.c_double, ctypes.POINTER(c_ptr)]),
+    "zwg_llm_state_kv8": (ctypes.c_int, [c_ptr, c_size, ctypes.POINTER(Kv8C)]),
+    "zwg_llm_state_set_rope": (ctypes.c_int, [c_ptr, c_ptr, c_ptr, c_ptr]),
     "zwg_dec_forward_q8": (ctypes.c_int, [c_ptr, ctypes.POINTER(DecWeightsC), c_ptr, c_size, c_size, c_ptr, c_ptr,
                                           c_ptr, c_size, c_ptr]),
 }

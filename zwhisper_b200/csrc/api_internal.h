@@ -127,6 +127,14 @@ struct zwg_llm_state {
     size_t n_layer = 0, n_batch = 0, n_head = 0, n_head_kv = 0, d = 0, n_ctx = 0;
     // per layer: cache_kt [n_batch][n_head_kv][d][n_ctx] (zeroed), cache_v [n_batch][n_ctx][n_head_kv*d]
     std::vector<float*> cache_kt, cache_v;
+    // or, with caches in 8 bits (kv8_api.cu): a cache per layer, all in one allocation, and the
+    // staging of a chunk's rotated keys [n_batch][n_head_kv][d][pitch] and values
+    // [n_batch][pitch][n_head_kv*d], which the q/k/v product writes as it writes the f32 caches
+    std::vector<zwg_kv8> kv8;
+    void* kv8_mem = nullptr;
+    size_t n_chunk = 0;
+    float *stage_kt = nullptr, *stage_v = nullptr;
+    static size_t stage_pitch(size_t n) { return (n + 3) & ~(size_t)3; }
     float* cos_tab = nullptr;  // [n_ctx][d/2]
     float* sin_tab = nullptr;
     zwg::capi::DevBuf ws;
@@ -138,5 +146,11 @@ namespace capi {
 // Causal GQA attention of q [n_batch][n][n_head*d] over one layer's caches, n_kv = n_past + n
 // (the body of zwg_llm_attn_prefill / _decode).
 int llm_attn(zwg_llm_state* st, size_t layer, const float* q, size_t n_past, size_t n, float* out, void* stream);
+// The same calls on a state whose caches are in 8 bits (kv8_api.cu): RoPE on q and k and the
+// append; the append of what the q/k/v product left in the staging; the attention.
+int kv8_llm_append(zwg_llm_state* st, size_t layer, float* q, const float* k, const float* v, size_t n_past, size_t n,
+                   cudaStream_t s);
+int kv8_llm_append_staged(zwg_llm_state* st, size_t layer, size_t n_past, size_t n, cudaStream_t s);
+int kv8_llm_attn(zwg_llm_state* st, size_t layer, const float* q, size_t n_past, size_t n, float* out, cudaStream_t s);
 }  // namespace capi
 }  // namespace zwg

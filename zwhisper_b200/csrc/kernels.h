@@ -202,6 +202,95 @@ int greedy_launch(float* logits, size_t m, size_t n_vocab, const int32_t* recent
 // One bounded wait that nothing completes (selftest.cu); gave_up is set to 1 when it ran out.
 int wait_timeout_selftest_launch(int* err, int* gave_up, cudaStream_t st);
 
+// ---- the decode step over a cache in 8 bits -----------------------------------------------
+// Tokens of a call (zwg_seqs, include/zwgpu.h); n_past is the most past[b] may be.
+struct Seqs {
+    int n_batch, n, n_past;
+    const int32_t* past;
+    const int32_t* count;
+    const int32_t* first;
+};
+// Element types of rows (the ZWG_TYPE_* codes of include/zwgpu.h).
+enum { TYPE_F32 = 0, TYPE_BF16 = 2 };
+// Rows of heads: head h of token i of sequence b at data + b * bs + i * ts + h * d (elements).
+struct Rows {
+    const void* data;
+    size_t bs, ts;
+};
+// Rotary tables [n_ctx][rot / 2]; cos null: no rotation.
+struct RopeTables {
+    const float* cos;
+    const float* sin;
+    int n_ctx, rot, interleaved;
+};
+
+// Rotary positions of any layout (rope.cu); k.data null: q alone.
+struct RopeCall {
+    Seqs s;
+    RopeTables t;
+    int d, n_head, n_head_kv;
+    Rows q, q_out, k, k_out;
+    int* err;
+};
+int rope_launch(const RopeCall& p, int type, cudaStream_t st);
+
+// A cache in 8 bits (zwg_kv8, include/zwgpu.h): blocks of KV8_BLOCK tokens.
+constexpr int KV8_BLOCK = 32;
+struct Kv8 {
+    int8_t* k;        // [n_batch][n_head_kv][blocks][32][d]
+    float* k_scale;   // [n_batch][n_head_kv][blocks]
+    int8_t* v;        // [n_batch][n_head_kv][blocks][d][32]
+    float* v_scale;
+    float* k_open;    // [n_batch][n_head_kv][32][d]
+    float* v_open;
+    int32_t* open_block;
+    int n_head_kv, d, blocks;
+};
+// New rows for the cache (kv8.cu). k and v elements are `es` apart: 1 for rows of heads; the
+// staging of the q/k/v product keeps keys transposed (element stride n, token stride 1).
+struct Kv8Append {
+    Kv8 c;
+    Seqs s;
+    Rows k, v;
+    size_t k_hs, v_hs, k_es;  // head strides, and k's element stride
+    RopeTables rope;
+    int* err;
+};
+int kv8_append_launch(const Kv8Append& p, int type, cudaStream_t st);
+// The cache's values at the call's positions, [n_batch][n][n_head_kv][d] f32 (null: left out).
+int kv8_read_launch(const Kv8& c, const Seqs& s, float* k, float* v, int* err, cudaStream_t st);
+
+// Attention over the cache (kv8_attn.cu).
+struct Kv8Attn {
+    Kv8 c;
+    Seqs s;
+    int n_head;
+    Rows q, out;
+    float* ws;
+    int* err;
+};
+size_t kv8_attn_workspace_bytes(const Kv8& c, const Seqs& s, int n_head, int sm_count);
+// pieces: f16 pieces of a query and a probability, 1 or 2.
+int kv8_attn_launch(const Kv8Attn& p, int type, int pieces, int sm_count, cudaStream_t st);
+
+// Penalties, biases, mask and argmax on rows of logits (logits.cu).
+struct LogitRules {
+    const int32_t* recent;
+    size_t recent_stride;
+    int n_recent;
+    const int32_t* n_recents;
+    int window;
+    float repeat, presence, frequency;
+    const int32_t* bias_ids;
+    const float* bias;
+    int n_bias;
+    size_t bias_stride;
+    const uint32_t* allow;
+    size_t allow_stride;
+};
+int logit_rules_launch(float* logits, size_t m, int n_vocab, size_t stride, const LogitRules& r, int32_t* out,
+                       size_t out_stride, int* err, cudaStream_t st);
+
 // Elementwise helpers (misc.cu).
 int f32_to_bf16_launch(const float* x, uint16_t* y, size_t n, cudaStream_t st);
 

@@ -101,11 +101,23 @@ int qkv(zwg_llm_state* st, size_t layer, const float* x, const zwg_llm_layer_wei
     p.cos_tab = st->cos_tab;
     p.sin_tab = st->sin_tab;
     p.q_out = q_out;
-    p.cache_kt = st->cache_kt[layer];
-    p.cache_v = st->cache_v[layer];
+    p.cache_kt = st->kv8.empty() ? st->cache_kt[layer] : nullptr;
+    p.cache_v = st->kv8.empty() ? st->cache_v[layer] : nullptr;
     p.cache_bs = st->n_head_kv * st->d * st->n_ctx;
+    const bool kv8 = !st->kv8.empty();
+    if (kv8) {  // into the staging, as a cache of just this chunk; the tables start at n_past
+        if (n > st->n_chunk) return fail("llm_qkv_q8: %zu tokens, the state was made for chunks of %zu", n, st->n_chunk);
+        const size_t pitch = st->stage_pitch(n);
+        p.n_past = 0;
+        p.n_ctx = (int)pitch;
+        p.cos_tab += n_past * (st->d / 2);
+        p.sin_tab += n_past * (st->d / 2);
+        p.cache_kt = st->stage_kt;
+        p.cache_v = st->stage_v;
+        p.cache_bs = st->n_head_kv * st->d * pitch;
+    }
     if (zwg::q8_pair_launch(p, zwg::PAIR_ROPE, s)) return cuda_fail("qkv launch", cudaGetLastError());
-    return ZWG_OK;
+    return kv8 ? kv8_llm_append_staged(st, layer, n_past, n, s) : ZWG_OK;
 }
 
 int layer_body(zwg_llm_state* st, size_t layer, const zwg_llm_weights* w, float* x, size_t n_past, size_t n,

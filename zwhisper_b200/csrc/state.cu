@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 
 #include <cmath>
+#include <new>
 #include <vector>
 
 #include "../../include/zwgpu.h"
@@ -46,6 +47,24 @@ int ensure_ws(DevBuf& ws, const zwg_attn_shape* sh, size_t n_batch, int sm_count
     return ZWG_OK;
 }
 
+// The state's rotary tables in f64, cast to f32 (src/llm.zig:128-137).
+int make_tables(zwg_llm_state* st, double rope_base) {
+    const size_t half = st->d / 2;
+    std::vector<float> cs(st->n_ctx * half), sn(st->n_ctx * half);
+    for (size_t p = 0; p < st->n_ctx; p++)
+        for (size_t i = 0; i < half; i++) {
+            const double inv = 1.0 / std::pow(rope_base, (double)(2 * i) / (double)st->d);
+            const double ang = (double)p * inv;
+            cs[p * half + i] = (float)std::cos(ang);
+            sn[p * half + i] = (float)std::sin(ang);
+        }
+    cudaError_t e = cudaMalloc(&st->cos_tab, cs.size() * sizeof(float));
+    if (e == cudaSuccess) e = cudaMalloc(&st->sin_tab, sn.size() * sizeof(float));
+    if (e == cudaSuccess) e = cudaMemcpy(st->cos_tab, cs.data(), cs.size() * sizeof(float), cudaMemcpyHostToDevice);
+    if (e == cudaSuccess) e = cudaMemcpy(st->sin_tab, sn.data(), sn.size() * sizeof(float), cudaMemcpyHostToDevice);
+    return e == cudaSuccess ? ZWG_OK : cuda_fail("rope tables", e);
+}
+
 }  // namespace
 
 Ctx* zwg::capi::ctx_for(int device) {
@@ -65,6 +84,7 @@ int zwg::capi::llm_attn(zwg_llm_state* st, size_t layer, const float* q, size_t 
     if (n_past + n > st->n_ctx) return fail("llm attention: context full (%zu + %zu > %zu)", n_past, n, st->n_ctx);
     Ctx* c = ctx_for(st->device);
     if (!c) return ZWG_ERROR;
+    if (!st->kv8.empty()) return kv8_llm_attn(st, layer, q, n_past, n, out, (cudaStream_t)stream);
     const size_t H = st->n_head, Hkv = st->n_head_kv, d = st->d, n_ctx = st->n_ctx;
     // the reference's call (src/llm.zig:191-202), over every sequence of the batch
     zwg_attn_shape sh{n, n_past + n, H, Hkv, d, H * d, Hkv * d, H * d, 1, n_ctx};
@@ -227,29 +247,79 @@ int zwg_llm_state_create(size_t n_layer, size_t n_batch, size_t n_head, size_t n
     // cache_kt is zeroed so columns beyond n_kv are finite, as the reference does (src/llm.zig:125)
     int rc = alloc_layers(st->cache_kt, n_layer, per, true);
     if (!rc) rc = alloc_layers(st->cache_v, n_layer, per, false);
-    if (!rc) {
-        // rotary tables in f64, cast to f32 (src/llm.zig:128-137)
-        const size_t half = d / 2;
-        std::vector<float> cs(n_ctx * half), sn(n_ctx * half);
-        for (size_t p = 0; p < n_ctx; p++)
-            for (size_t i = 0; i < half; i++) {
-                const double inv = 1.0 / std::pow(rope_base, (double)(2 * i) / (double)d);
-                const double ang = (double)p * inv;
-                cs[p * half + i] = (float)std::cos(ang);
-                sn[p * half + i] = (float)std::sin(ang);
-            }
-        cudaError_t e = cudaMalloc(&st->cos_tab, cs.size() * sizeof(float));
-        if (e == cudaSuccess) e = cudaMalloc(&st->sin_tab, sn.size() * sizeof(float));
-        if (e == cudaSuccess) e = cudaMemcpy(st->cos_tab, cs.data(), cs.size() * sizeof(float), cudaMemcpyHostToDevice);
-        if (e == cudaSuccess) e = cudaMemcpy(st->sin_tab, sn.data(), sn.size() * sizeof(float), cudaMemcpyHostToDevice);
-        if (e != cudaSuccess) rc = cuda_fail("rope tables", e);
-    }
+    if (!rc) rc = make_tables(st, rope_base);
     if (!rc) {
         // worst case of a decode step: one query over the whole context
         zwg_attn_shape s1{1, n_ctx, n_head, n_head_kv, d, n_head * d, n_head_kv * d, n_head * d, 1, n_ctx};
         rc = ensure_ws(st->ws, &s1, n_batch, c->sm_count);
         if (!rc && !st->tickets.init(c, n_batch * n_head_kv)) rc = fail("llm state: ticket buffer");
     }
+    if (rc) {
+        zwg_llm_state_destroy(st);
+        return rc;
+    }
+    *out = st;
+    return ZWG_OK;
+}
+
+int zwg_llm_state_create_kv8(size_t n_layer, size_t n_batch, size_t n_head, size_t n_head_kv, size_t d, size_t n_ctx,
+                             size_t n_chunk, double rope_base, zwg_llm_state** out) {
+    if (!out) return fail("null output pointer");
+    *out = nullptr;
+    Ctx* c = cur();
+    if (!c) return ZWG_ERROR;
+    if (!n_layer || !n_batch || !n_head || !n_head_kv || n_head % n_head_kv || (d != 64 && d != 128) || !n_ctx ||
+        n_ctx % 32 || n_ctx >= (1u << 30) || !n_chunk || n_chunk > n_ctx || n_batch * n_head_kv > 65535 || !(rope_base > 0))
+        return fail("llm state in 8 bits: bad sizes (n_head %zu, n_head_kv %zu, d %zu, n_ctx %zu, n_chunk %zu)", n_head,
+                    n_head_kv, d, n_ctx, n_chunk);
+    zwg_llm_state* st = new (std::nothrow) zwg_llm_state();
+    if (!st) return fail("llm state: out of memory");
+    st->device = c->device;
+    st->n_layer = n_layer;
+    st->n_batch = n_batch;
+    st->n_head = n_head;
+    st->n_head_kv = n_head_kv;
+    st->d = d;
+    st->n_ctx = n_ctx;
+    st->n_chunk = n_chunk;
+    // a layer's buffers one after another, each from a 256-byte boundary
+    const size_t segs = n_batch * n_head_kv, blocks = n_ctx / 32;
+    const auto round = [](size_t b) { return (b + 255) & ~(size_t)255; };
+    const size_t ints = round(segs * n_ctx * d), scales = round(segs * blocks * sizeof(float)),
+                 open = round(segs * 32 * d * sizeof(float)), tags = round(segs * sizeof(int32_t));
+    const size_t per = 2 * (ints + scales + open) + tags;
+    const size_t stage = segs * d * zwg_llm_state::stage_pitch(n_chunk) * sizeof(float);
+    int rc = ZWG_OK;
+    cudaError_t e = cudaMalloc(&st->kv8_mem, per * n_layer);
+    if (e == cudaSuccess) e = cudaMemset(st->kv8_mem, 0, per * n_layer);
+    if (e == cudaSuccess) e = cudaMalloc(&st->stage_kt, stage);
+    if (e == cudaSuccess) e = cudaMalloc(&st->stage_v, stage);
+    for (size_t l = 0; l < n_layer && e == cudaSuccess; l++) {
+        char* p = (char*)st->kv8_mem + l * per;
+        zwg_kv8 k{};
+        k.k = (int8_t*)p;
+        k.v = (int8_t*)(p + ints);
+        k.k_scale = (float*)(p + 2 * ints);
+        k.v_scale = (float*)(p + 2 * ints + scales);
+        k.k_open = (float*)(p + 2 * (ints + scales));
+        k.v_open = (float*)(p + 2 * (ints + scales) + open);
+        k.open_block = (int32_t*)(p + 2 * (ints + scales + open));
+        k.n_batch = n_batch;
+        k.n_head_kv = n_head_kv;
+        k.d = d;
+        k.n_ctx = n_ctx;
+        e = cudaMemset(k.open_block, 0xff, segs * sizeof(int32_t));
+        st->kv8.push_back(k);
+    }
+    if (e != cudaSuccess) rc = cuda_fail("llm state in 8 bits", e);
+    if (!rc) rc = make_tables(st, rope_base);
+    // the most a call of up to n_chunk tokens needs, at the end of the context
+    size_t ws = 0;
+    for (size_t n = 1; n <= n_chunk && !rc; n++) {
+        const zwg_seqs s{n_batch, n, n_ctx - n, nullptr, nullptr, nullptr};
+        ws = std::max(ws, zwg_kv8_attn_workspace(&st->kv8[0], &s, n_head));
+    }
+    if (!rc && ws && !st->ws.ensure(ws)) rc = fail("llm state: workspace of %zu bytes", ws);
     if (rc) {
         zwg_llm_state_destroy(st);
         return rc;
@@ -266,6 +336,9 @@ int zwg_llm_state_destroy(zwg_llm_state* st) {
     cudaDeviceSynchronize();
     free_all(st->cache_kt);
     free_all(st->cache_v);
+    if (st->kv8_mem) cudaFree(st->kv8_mem);
+    if (st->stage_kt) cudaFree(st->stage_kt);
+    if (st->stage_v) cudaFree(st->stage_v);
     if (st->cos_tab) cudaFree(st->cos_tab);
     if (st->sin_tab) cudaFree(st->sin_tab);
     st->ws.release();
@@ -277,6 +350,7 @@ int zwg_llm_state_destroy(zwg_llm_state* st) {
 
 int zwg_llm_state_cache(const zwg_llm_state* st, size_t layer, float** cache_kt, float** cache_v) {
     if (!st || layer >= st->n_layer) return fail("bad state or layer");
+    if (!st->kv8.empty()) return fail("llm_state_cache: the state's caches are in 8 bits (zwg_llm_state_kv8)");
     if (cache_kt) *cache_kt = st->cache_kt[layer];
     if (cache_v) *cache_v = st->cache_v[layer];
     return ZWG_OK;
@@ -290,6 +364,7 @@ int zwg_llm_append_rope(zwg_llm_state* st, size_t layer, float* q, const float* 
     if (n_past + n > st->n_ctx) return fail("llm_append_rope: context full (%zu + %zu > %zu)", n_past, n, st->n_ctx);
     Ctx* c = ctx_for(st->device);
     if (!c) return ZWG_ERROR;
+    if (!st->kv8.empty()) return kv8_llm_append(st, layer, q, k, v, n_past, n, (cudaStream_t)stream);
     const size_t kvw = st->n_head_kv * st->d;
     zwg::RopeParams p{q, k, v, st->cache_kt[layer], st->cache_v[layer], st->cos_tab, st->sin_tab, n, n_past,
                       st->n_head, st->n_head_kv, st->d, st->n_ctx, n * st->n_head * st->d, n * kvw, kvw * st->n_ctx};

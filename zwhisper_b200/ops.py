@@ -17,7 +17,8 @@ states `DecoderState` and `LlmState`; the Q8 projections `quantize_q8`, `linear_
 168-216, 268-321): `rms_norm`, `embed_q8`, `llm_greedy`, `LlmWeightsQ8` with
 `LlmState.qkv_q8 / layer_q8 / forward_q8`; and the Whisper decoder step (src/decoder.zig:
 151-206): `layer_norm`, `linear_q8_gelu`, `DecoderWeightsQ8` with
-`DecoderState.set_audio_q8 / forward_q8`.
+`DecoderState.set_audio_q8 / forward_q8`. A decode step over a cache in 8 bits: `rope`,
+`scaled_rope_tables`, `Kv8Cache`, `LlmState(kv8=True)` and `llm_logits`.
 """
 from __future__ import annotations
 
@@ -407,26 +408,33 @@ class DecoderState:
         return x, logits
 
 class _DeviceArray:
-    """A float32 device buffer described by __cuda_array_interface__ (for zero-copy views)."""
+    """A device buffer (float32 unless typestr says otherwise) described by
+    __cuda_array_interface__ (for zero-copy views)."""
 
-    def __init__(self, ptr: int, shape):
-        self.__cuda_array_interface__ = {"shape": tuple(shape), "typestr": "<f4", "data": (ptr, False),
+    def __init__(self, ptr: int, shape, typestr: str = "<f4"):
+        self.__cuda_array_interface__ = {"shape": tuple(shape), "typestr": typestr, "data": (ptr, False),
                                          "version": 3, "strides": None}
 
 
 class LlmState:
     """Qwen2 attention state on one device (zwg_llm_state): per layer cache_kt
     [n_batch][n_head_kv][d][n_ctx] and cache_v [n_batch][n_ctx][n_head_kv*d], RoPE tables in
-    f64 (src/llm.zig:27-28, 124-137)."""
+    f64 (src/llm.zig:27-28, 124-137). With kv8 the caches are in 8 bits (Kv8Cache, d 64 or 128,
+    n_ctx a multiple of 32) and a call takes up to n_chunk tokens."""
 
     def __init__(self, n_layer: int, n_batch: int, n_head: int, n_head_kv: int, d: int, n_ctx: int,
-                 rope_base: float = 1e6, device: int = 0):
+                 rope_base: float = 1e6, device: int = 0, kv8: bool = False, n_chunk: int = 256):
+        self._h = ctypes.c_void_p()
         _lib.ensure_init(device)
         self.device, self.n_layer, self.n_batch = device, n_layer, n_batch
-        self.n_head, self.n_head_kv, self.d, self.n_ctx = n_head, n_head_kv, d, n_ctx
+        self.n_head, self.n_head_kv, self.d, self.n_ctx, self.kv8 = n_head, n_head_kv, d, n_ctx, kv8
         h = ctypes.c_void_p()
-        _lib.check(_lib.load().zwg_llm_state_create(n_layer, n_batch, n_head, n_head_kv, d, n_ctx, float(rope_base),
-                                                    ctypes.byref(h)))
+        if kv8:
+            _lib.check(_lib.load().zwg_llm_state_create_kv8(n_layer, n_batch, n_head, n_head_kv, d, n_ctx,
+                                                            min(n_chunk, n_ctx), float(rope_base), ctypes.byref(h)))
+        else:
+            _lib.check(_lib.load().zwg_llm_state_create(n_layer, n_batch, n_head, n_head_kv, d, n_ctx,
+                                                        float(rope_base), ctypes.byref(h)))
         self._h = h
 
     def close(self) -> None:
@@ -455,6 +463,32 @@ class LlmState:
         shapes = ((self.n_batch, self.n_head_kv, self.d, self.n_ctx),
                   (self.n_batch, self.n_ctx, self.n_head_kv * self.d))
         return tuple(torch.as_tensor(_DeviceArray(p, shp), device=dev) for p, shp in zip((kt, v), shapes))
+
+    def kv8_cache(self, layer: int) -> "Kv8Cache":
+        """One layer's cache in 8 bits (no copy). Valid until close()."""
+        torch = _torch()
+        c = _lib.Kv8C()
+        _lib.check(_lib.load().zwg_llm_state_kv8(self._h, layer, ctypes.byref(c)))
+        B, H, d, nb = self.n_batch, self.n_head_kv, self.d, self.n_ctx // 32
+        dev = torch.device("cuda", self.device)
+
+        def view(ptr, typestr, *shape):
+            return torch.as_tensor(_DeviceArray(ptr, shape, typestr), device=dev)
+
+        return Kv8Cache(view(c.k, "|i1", B, H, nb, 32, d), view(c.k_scale, "<f4", B, H, nb),
+                        view(c.v, "|i1", B, H, nb, d, 32), view(c.v_scale, "<f4", B, H, nb),
+                        view(c.k_open, "<f4", B, H, 32, d), view(c.v_open, "<f4", B, H, 32, d),
+                        view(c.open_block, "<i4", B, H))
+
+    def set_rope(self, cos, sin) -> None:
+        """Replace the rotary tables by cos, sin [n_ctx][d/2] f32 (CUDA tensors), for example
+        scaled_rope_tables'."""
+        torch = _torch()
+        for t, name in ((cos, "cos"), (sin, "sin")):
+            if t.numel() != self.n_ctx * (self.d // 2):
+                raise ValueError(f"{name} must hold n_ctx * d / 2 floats, got {t.numel()}")
+        _lib.check(_lib.load().zwg_llm_state_set_rope(self._h, _dev_ptr(cos, torch.float32, "cos"),
+                                                      _dev_ptr(sin, torch.float32, "sin"), _stream_of(cos)))
 
     def append_rope(self, layer: int, q, k, v, n_past: int) -> None:
         """RoPE on q (in place) and k, cache append at n_past.. (src/llm.zig:180-190)."""
@@ -750,6 +784,307 @@ def linear_q8_gelu(x, q, scales, bias=None, out=None):
     _lib.check(_lib.load().zwg_linear_q8_gelu(_dev_ptr(x, torch.float32, "x"), m, k, q.data_ptr(), sp,
                                               _dev_ptr(bias, torch.float32, "bias") if bias is not None else None,
                                               n, _dev_ptr(out, torch.float32, "out"), _stream_of(x)))
+    return out
+
+
+# ---- a decode step over a cache in 8 bits (zwg_rope, zwg_kv8_*, zwg_llm_logits) -----------
+
+def scaled_rope_tables(n_ctx: int, rot: int, base: float, scaling: str = "none", factor: float = 1.0,
+                       n_train: int = 0, low: float = 1.0, high: float = 4.0, attn_factor: Optional[float] = None):
+    """Rotary tables cos, sin [n_ctx][rot/2] f32 for a context longer than the n_train positions
+    a model was trained on, angles in f64. Pair i turns base^(-2i/rot) per position; `scaling`:
+      "none"     as it is;
+      "linear"   all turns slower by `factor`;
+      "ntk"      base * factor^(rot / (rot - 2)): the fastest pair stays, the slowest slows by factor;
+      "bands"    pairs with more than `high` turns within n_train stay, those with fewer than `low`
+                 slow by factor, those between blend the two by their number of turns;
+      "yarn"     pairs are blended linearly in their index, between the index that makes `high`
+                 turns within n_train (usually 32) and the one that makes `low` (usually 1), and cos
+                 and sin are multiplied by attn_factor (default 0.1 ln(factor) + 1)."""
+    if rot <= 0 or rot % 2 or n_ctx <= 0 or not base > 0 or not factor > 0:
+        raise ValueError(f"bad rotary sizes: n_ctx {n_ctx}, rot {rot}, base {base}, factor {factor}")
+    if scaling in ("bands", "yarn") and not (n_train > 0 and high > low > 0):
+        raise ValueError("this scaling needs n_train > 0 and high > low > 0")
+    if scaling == "ntk":
+        if rot < 4:
+            raise ValueError("ntk scaling needs rot >= 4")
+        base = base * factor ** (rot / (rot - 2))
+    i = np.arange(rot // 2, dtype=np.float64)
+    inv = np.power(np.float64(base), -2.0 * i / rot)
+    scale = 1.0
+    if scaling == "linear":
+        inv = inv / factor
+    elif scaling == "bands":
+        turns = n_train * inv / (2 * np.pi)
+        keep = np.clip((turns - low) / (high - low), 0.0, 1.0)
+        inv = keep * inv + (1 - keep) * inv / factor
+    elif scaling == "yarn":
+        at = [rot * np.log(n_train / (t * 2 * np.pi)) / (2 * np.log(base)) for t in (high, low)]
+        lo, hi = max(np.floor(at[0]), 0.0), min(np.ceil(at[1]), rot - 1.0)
+        slow = np.clip((i - lo) / max(hi - lo, 1e-3), 0.0, 1.0)
+        inv = (1 - slow) * inv + slow * inv / factor
+        scale = (0.1 * np.log(factor) + 1.0 if factor > 1 else 1.0) if attn_factor is None else attn_factor
+    elif scaling not in ("none", "ntk"):
+        raise ValueError(f"unknown scaling {scaling!r}")
+    ang = np.arange(n_ctx, dtype=np.float64)[:, None] * inv[None, :]
+    return (np.cos(ang) * scale).astype(np.float32), (np.sin(ang) * scale).astype(np.float32)
+
+
+def _row_type(t, name):
+    torch = _torch()
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    if t.dtype == torch.float32:
+        return _lib.ZWG_TYPE_F32
+    if t.dtype == torch.bfloat16:
+        return _lib.ZWG_TYPE_BF16
+    raise ValueError(f"{name} must be float32 or bfloat16, got {t.dtype}")
+
+
+def _rows(t, like, heads: Optional[int], name: str) -> _lib.RowsC:
+    """Rows of heads [n_batch][n][heads][d] (any batch and token strides) of `like`'s batch, tokens,
+    d, type and device."""
+    if t.dim() != 4 or t.dtype != like.dtype or t.device != like.device:
+        raise ValueError(f"{name} must be a [n_batch][n][heads][d] tensor of {like.dtype} on {like.device}")
+    if t.shape[0] != like.shape[0] or t.shape[1] != like.shape[1] or t.shape[3] != like.shape[3]:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, which does not go with {tuple(like.shape)}")
+    if heads is not None and t.shape[2] != heads:
+        raise ValueError(f"{name} must have {heads} heads, got {t.shape[2]}")
+    sb, st, sh, sd = t.stride()
+    if (t.shape[3] > 1 and sd != 1) or (t.shape[2] > 1 and sh != t.shape[3]):
+        raise ValueError(f"{name}: a token's heads must lie one after another")
+    return _lib.RowsC(t.data_ptr(), sb, st)
+
+
+def _int32_of(t, device, shape, name):
+    torch = _torch()
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != device or tuple(t.shape) != shape:
+        raise ValueError(f"{name} must be an int32 tensor of shape {shape} on {device}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    return t.data_ptr()
+
+
+def _seqs(n_batch: int, n: int, n_past, count, first, max_past, device) -> _lib.SeqsC:
+    """zwg_seqs of a call: n_past a number, or an int32 tensor [n_batch] whose entries are at
+    most max_past."""
+    torch = _torch()
+    past = None
+    if isinstance(n_past, torch.Tensor):
+        past = _int32_of(n_past, device, (n_batch,), "n_past")
+        n_past = max_past
+    if n_past < 0:
+        raise ValueError(f"n_past must not be negative, got {n_past}")
+    return _lib.SeqsC(n_batch, n, n_past, past,
+                      None if count is None else _int32_of(count, device, (n_batch,), "count"),
+                      None if first is None else _int32_of(first, device, (n_batch,), "first"))
+
+
+def _tables(cos, sin, device, interleaved: bool) -> _lib.RopeTablesC:
+    torch = _torch()
+    for t, name in ((cos, "cos"), (sin, "sin")):
+        if t.dim() != 2 or t.shape != cos.shape or t.device != device:
+            raise ValueError(f"{name} must be [n_ctx][rot / 2] on {device}, cos and sin alike")
+    return _lib.RopeTablesC(_dev_ptr(cos, torch.float32, "cos"), _dev_ptr(sin, torch.float32, "sin"), cos.shape[0],
+                            2 * cos.shape[1], 1 if interleaved else 0)
+
+
+def rope(q, cos, sin, n_past=0, k=None, interleaved: bool = False, count=None, inplace: bool = True, q_out=None,
+         k_out=None):
+    """Rotary positions (zwg_rope) on q [n_batch][n][n_head][d] and, where given, k
+    [n_batch][n][n_head_kv][d] (CUDA f32 or bf16, any batch and token strides), token i of
+    sequence b at position n_past + i (n_past an int, or a CUDA int32 tensor [n_batch]). cos,
+    sin [n_ctx][rot/2] f32 (rope_tables, scaled_rope_tables): the first rot elements of a head
+    are rotated, in pairs (i, i + rot/2) or, interleaved, (2i, 2i + 1). count (CUDA int32
+    [n_batch]): tokens of each sequence, the rows behind them stay. In place, or into q_out and
+    k_out (new tensors with inplace=False). Returns q, or (q, k)."""
+    torch = _torch()
+    kind = _row_type(q, "q")
+    if q.dim() != 4:
+        raise ValueError("q must be [n_batch][n][n_head][d]")
+    B, n, H, d = q.shape
+    heads_kv = 0 if k is None else k.shape[2] if k.dim() == 4 else -1
+    if not inplace:
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else q_out
+        if k is not None and k_out is None:
+            k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    q_out = q if q_out is None else q_out
+    k_out = k if k_out is None else k_out
+    if k is None and k_out is not None:
+        raise ValueError("k_out without k")
+    qr, qo = _rows(q, q, H, "q"), _rows(q_out, q, H, "q_out")
+    kr = ko = None
+    if k is not None:
+        kr, ko = ctypes.byref(_rows(k, q, None, "k")), ctypes.byref(_rows(k_out, q, heads_kv, "k_out"))
+    _lib.ensure_init(q.device.index or 0)
+    tables = _tables(cos, sin, q.device, interleaved)
+    sq = _seqs(B, n, n_past, count, None, cos.shape[0], q.device)
+    _lib.check(_lib.load().zwg_rope(ctypes.byref(sq), ctypes.byref(tables), kind, d, H, ctypes.byref(qr),
+                                    ctypes.byref(qo), heads_kv, kr, ko, _stream_of(q)))
+    return q_out if k is None else (q_out, k_out)
+
+
+class Kv8Cache:
+    """A key/value cache in 8 bits (zwg_kv8): int8 K [n_batch][n_head_kv][n_ctx/32][32][d] and V
+    [n_batch][n_head_kv][n_ctx/32][d][32], f32 scales [n_batch][n_head_kv][n_ctx/32], the block
+    that is filling also in f32 (k_open, v_open [n_batch][n_head_kv][32][d], of block open_block
+    [n_batch][n_head_kv] int32, -1: none). d 64 or 128, n_ctx a multiple of 32; contiguous CUDA
+    tensors on one device, which the cache keeps. `Kv8Cache.empty` makes them."""
+
+    def __init__(self, k, k_scale, v, v_scale, k_open, v_open, open_block):
+        torch = _torch()
+        if k.dim() != 5 or k.shape[3] != 32:
+            raise ValueError("k must be [n_batch][n_head_kv][n_ctx/32][32][d]")
+        B, H, nb, _, d = k.shape
+        self.n_batch, self.n_head_kv, self.d, self.n_ctx, self.device = B, H, d, 32 * nb, k.device
+        want = (("k", k, torch.int8, (B, H, nb, 32, d)), ("k_scale", k_scale, torch.float32, (B, H, nb)),
+                ("v", v, torch.int8, (B, H, nb, d, 32)), ("v_scale", v_scale, torch.float32, (B, H, nb)),
+                ("k_open", k_open, torch.float32, (B, H, 32, d)), ("v_open", v_open, torch.float32, (B, H, 32, d)),
+                ("open_block", open_block, torch.int32, (B, H)))
+        for name, t, dtype, shape in want:
+            if tuple(t.shape) != shape or t.device != k.device:
+                raise ValueError(f"{name} must have shape {shape} on {k.device}, got {tuple(t.shape)} on {t.device}")
+        self._keep = tuple(t for _, t, _, _ in want)
+        self.k, self.k_scale, self.v, self.v_scale, self.k_open, self.v_open, self.open_block = self._keep
+        self._c = _lib.Kv8C(*(_dev_ptr(t, dtype, name) for name, t, dtype, _ in want), B, H, d, 32 * nb)
+
+    @classmethod
+    def empty(cls, n_batch: int, n_head_kv: int, d: int, n_ctx: int, device: int = 0) -> "Kv8Cache":
+        """An empty cache for up to n_ctx tokens a sequence."""
+        torch = _torch()
+        if n_ctx <= 0 or n_ctx % 32 or d not in (64, 128):
+            raise ValueError(f"n_ctx must be a positive multiple of 32 and d 64 or 128, got {n_ctx}, {d}")
+        dev, nb, z = torch.device("cuda", device), n_ctx // 32, torch.zeros
+        return cls(z(n_batch, n_head_kv, nb, 32, d, dtype=torch.int8, device=dev), z(n_batch, n_head_kv, nb, device=dev),
+                   z(n_batch, n_head_kv, nb, d, 32, dtype=torch.int8, device=dev), z(n_batch, n_head_kv, nb, device=dev),
+                   z(n_batch, n_head_kv, 32, d, device=dev), z(n_batch, n_head_kv, 32, d, device=dev),
+                   torch.full((n_batch, n_head_kv), -1, dtype=torch.int32, device=dev))
+
+    def _call(self, n: int, n_past, count, first, max_past) -> _lib.SeqsC:
+        _lib.ensure_init(self.device.index or 0)
+        return _seqs(self.n_batch, n, n_past, count, first, self.n_ctx if max_past is None else max_past, self.device)
+
+    def append(self, k, v, n_past, count=None, rope=None) -> None:
+        """Append k, v [n_batch][n][n_head_kv][d] (f32 or bf16) at n_past (an int, or a CUDA int32
+        tensor [n_batch]); count (CUDA int32 [n_batch]): tokens of each sequence. rope: (cos,
+        sin) or (cos, sin, interleaved), the rotation of k on its way in."""
+        kind = _row_type(k, "k")
+        if k.dim() != 4 or k.shape[0] != self.n_batch or k.shape[2:] != (self.n_head_kv, self.d) or k.device != self.device:
+            raise ValueError(f"k must be [{self.n_batch}][n][{self.n_head_kv}][{self.d}] on {self.device}")
+        kr, vr = _rows(k, k, None, "k"), _rows(v, k, self.n_head_kv, "v")
+        s = self._call(k.shape[1], n_past, count, None, None)
+        t = None
+        if rope is not None:
+            t = ctypes.byref(_tables(rope[0], rope[1], self.device, len(rope) > 2 and rope[2]))
+        _lib.check(_lib.load().zwg_kv8_append(ctypes.byref(self._c), ctypes.byref(s), kind, ctypes.byref(kr),
+                                              ctypes.byref(vr), t, _stream_of(k)))
+
+    def read(self, n: int, n_past, count=None, k=None, v=None):
+        """The values of n tokens from position n_past: (k, v) [n_batch][n][n_head_kv][d] f32."""
+        torch = _torch()
+        shape = (self.n_batch, n, self.n_head_kv, self.d)
+        out = []
+        for t, name in ((k, "k"), (v, "v")):
+            t = torch.empty(shape, dtype=torch.float32, device=self.device) if t is None else t
+            if tuple(t.shape) != shape or t.device != self.device:
+                raise ValueError(f"{name} must have shape {shape} on {self.device}")
+            out.append(t)
+        s = self._call(n, n_past, count, None, None)
+        _lib.check(_lib.load().zwg_kv8_read(ctypes.byref(self._c), ctypes.byref(s),
+                                            _dev_ptr(out[0], torch.float32, "k"), _dev_ptr(out[1], torch.float32, "v"),
+                                            _stream_of(out[0])))
+        return tuple(out)
+
+    def attn_workspace_bytes(self, n: int, n_head: int, n_past=None) -> int:
+        """Workspace of attn for n tokens after n_past (None: the most there can be)."""
+        s = self._call(n, max(self.n_ctx - n, 0) if n_past is None else n_past, None, None, None)
+        return int(_lib.load().zwg_kv8_attn_workspace(ctypes.byref(self._c), ctypes.byref(s), n_head))
+
+    def attn(self, q, n_past, count=None, first=None, max_past=None, out=None, workspace=None):
+        """Attention (zwg_kv8_attn) of q [n_batch][n][n_head][d] (f32 or bf16) at positions n_past..
+        (an int, or a CUDA int32 tensor [n_batch] whose entries are at most max_past) over the
+        cache, which holds the call's own tokens already: query i of sequence b sees keys
+        first[b] .. n_past + i. count, first: CUDA int32 [n_batch]; rows of out behind count[b]
+        stay as they are. Returns out, of q's shape and type."""
+        torch = _torch()
+        kind = _row_type(q, "q")
+        if q.dim() != 4 or q.shape[0] != self.n_batch or q.shape[3] != self.d or q.device != self.device:
+            raise ValueError(f"q must be [{self.n_batch}][n][n_head][{self.d}] on {self.device}")
+        n, H = q.shape[1], q.shape[2]
+        if out is None:
+            out = (torch.empty if count is None else torch.zeros)(q.shape, dtype=q.dtype, device=q.device)
+        qr, orow = _rows(q, q, H, "q"), _rows(out, q, H, "out")
+        s = self._call(n, n_past, count, first, max_past)
+        lib, c = _lib.load(), ctypes.byref(self._c)
+        if workspace is None:
+            need = lib.zwg_kv8_attn_workspace(c, ctypes.byref(s), H)
+            if need:
+                workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        ws, size = (workspace.data_ptr(), workspace.numel() * workspace.element_size()) if workspace is not None else (0, 0)
+        _lib.check(lib.zwg_kv8_attn(c, ctypes.byref(s), kind, H, ctypes.byref(qr), ctypes.byref(orow), ws, size,
+                                    _stream_of(q)))
+        return out
+
+
+def llm_logits(logits, recent=None, n_recent=None, window: Optional[int] = None, repeat: float = 1.0,
+               presence: float = 0.0, frequency: float = 0.0, bias_ids=None, bias=None, allow=None, out=None):
+    """The rules on a step's logits (zwg_llm_logits), in place on CUDA f32 logits [m][n_vocab]:
+    a token that is c > 0 times among a row's last `window` (None: all) recent tokens is divided
+    by `repeat` (positive logits) or multiplied by it (others), then reduced by c * frequency +
+    presence; biases are added; tokens whose bit in `allow` is 0 become -inf. recent: CUDA int32
+    [m][n] (negative entries are padding), n_recent: how many of a row's count, an int or a CUDA
+    int32 tensor [m]; bias_ids, bias: CUDA int32 and f32, [n] for all rows or [m][n]; allow: CUDA
+    int32 words [n_vocab/32 rounded up], for all rows or [m][...]. Returns each row's first index
+    of its largest logit, -1 where none is above -inf (CUDA int32 [m], or in `out`)."""
+    torch = _torch()
+    if not isinstance(logits, torch.Tensor) or not logits.is_cuda or logits.dtype != torch.float32 or logits.dim() != 2:
+        raise ValueError("logits must be a CUDA float32 [m][n_vocab] tensor")
+    m, V = logits.shape
+    if V > 1 and logits.stride(1) != 1:
+        raise ValueError("a row's logits must lie one after another")
+    dev = logits.device
+
+    def lists(t, dtype, name, width=None):
+        """(pointer, row stride, entries) of a list for all rows, or one for each."""
+        if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != dev or t.dim() not in (1, 2):
+            raise ValueError(f"{name} must be a {dtype} tensor [n] or [m][n] on {dev}")
+        if t.dim() == 2 and t.shape[0] != m:
+            raise ValueError(f"{name} must have {m} rows, got {t.shape[0]}")
+        if t.shape[-1] > 1 and t.stride(-1) != 1:
+            raise ValueError(f"{name} must have unit stride along its entries")
+        if width is not None and t.shape[-1] < width:
+            raise ValueError(f"{name} must have {width} entries, got {t.shape[-1]}")
+        return t.data_ptr(), t.stride(0) if t.dim() == 2 else 0, t.shape[-1]
+
+    r = _lib.LogitRulesC()
+    r.repeat, r.presence, r.frequency = repeat, presence, frequency
+    if recent is not None:
+        r.recent, r.recent_stride, r.n_recent = lists(recent, torch.int32, "recent")
+        if isinstance(n_recent, torch.Tensor):
+            r.n_recents = _int32_of(n_recent, dev, (m,), "n_recent")
+        elif n_recent is not None:
+            if not 0 <= n_recent <= recent.shape[-1]:
+                raise ValueError(f"n_recent must be 0 .. {recent.shape[-1]}, got {n_recent}")
+            r.n_recent = n_recent
+        r.window = recent.shape[-1] if window is None else max(window, 0)
+    if (bias_ids is None) != (bias is None):
+        raise ValueError("bias_ids and bias go together")
+    if bias is not None:
+        if bias.shape != bias_ids.shape:
+            raise ValueError("bias_ids and bias must have the same shape")
+        r.bias_ids, stride, r.n_bias = lists(bias_ids, torch.int32, "bias_ids")
+        r.bias, r.bias_stride, _ = lists(bias, torch.float32, "bias")
+        if stride != r.bias_stride:
+            raise ValueError("bias_ids and bias must have the same strides")
+    if allow is not None:
+        r.allow, r.allow_stride, _ = lists(allow, torch.int32, "allow", (V + 31) // 32)
+    if out is None:
+        out = torch.empty(m, dtype=torch.int32, device=dev)
+    if out.dtype != torch.int32 or tuple(out.shape) != (m,) or out.device != dev or (m > 1 and out.stride(0) < 1):
+        raise ValueError(f"out must be an int32 tensor [{m}] on {dev}")
+    _lib.ensure_init(dev.index or 0)
+    _lib.check(_lib.load().zwg_llm_logits(logits.data_ptr(), m, V, logits.stride(0), ctypes.byref(r), out.data_ptr(),
+                                          out.stride(0) if m else 1, _stream_of(logits)))
     return out
 
 
