@@ -400,7 +400,8 @@ def test_attention_strides_streams_and_graphs(env):
     assert past.tolist() == [1004] * B
     cache.append(k, v, 1000)
     cache.append(k, v, 1002)
-    assert torch.equal(cache.attn(q0, 1002), out)
+    # the same call outside the graph (with n_past a number the keys may be cut at other places)
+    assert torch.equal(cache.attn(q0, i32(torch, [1002] * B)), out)
     ops.sync()
 
 

@@ -14,28 +14,31 @@
 // order of the d elements inside a dot product and of the tokens inside a sum is free, so lane
 // (g, t) takes 16 consecutive bytes of a key's row and 8 consecutive tokens of a value's column,
 // and no shared memory or shuffle stands between memory and the tensor cores.
-// A warp takes whole blocks; its softmax state is merged with the other warps' in shared memory and
-// the splits' partials (m, l, O) by kv8_combine_kernel.
+// A warp takes whole blocks of the split's range, each one bulk copy of its keys and one of its
+// values into the warp's own ring in shared memory, so a warp never waits for another one before the
+// merge and loads run ahead of the arithmetic (24 KB an SM cover the latency of HBM; 3 CTAs hold 96).
+// The splits of a (sequence, kv head, tile of query rows) that fit a cluster (8 CTAs) meet in each
+// other's shared memory; more of them write partials (m, l, O) for kv8_combine_kernel.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include <algorithm>
 
+#include <cooperative_groups.h>
+
 #include "chain.cuh"
 #include "common.cuh"
 #include "kernels.h"
 #include "seqs.cuh"
+#include "sm100.cuh"
 
 namespace zwg {
 namespace {
 
+namespace cg = cooperative_groups;
+
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kUnit = 32768.f;  // P's f16 pieces hold 2^15 p: small probabilities stay normal
-
-ZWG_DEV float up(float x) { return x; }
-ZWG_DEV float up(__nv_bfloat16 x) { return __bfloat162float(x); }
-ZWG_DEV void down(float x, float& y) { y = x; }
-ZWG_DEV void down(float x, __nv_bfloat16& y) { y = __float2bfloat16_rn(x); }
 
 ZWG_DEV uint32_t h2u(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 
@@ -86,6 +89,9 @@ struct Plan {
 };
 
 constexpr int WARPS = 4;
+constexpr int MAX_CLUSTER = 8;
+constexpr int CTAS_PER_SM = 3;
+constexpr size_t RING = 64 * 1024;  // bytes a CTA's warps have for blocks on their way
 
 // Rows of a tile: one or two 8-wide N tiles.
 int tile_rows(int rows) { return rows <= 8 ? 8 : 16; }
@@ -96,38 +102,188 @@ Plan plan_for(const Kv8& c, const Seqs& s, int n_head, int sm_count) {
     p.tiles = (rows + tile_rows(rows) - 1) / tile_rows(rows);
     const long long ctas = (long long)s.n_batch * c.n_head_kv * p.tiles;
     const int blocks = (s.n_past + s.n + KV8_BLOCK - 1) / KV8_BLOCK;
-    // four CTAs an SM, each with at least a block for every warp
-    const long long want = std::max<long long>(1, 4ll * sm_count / ctas);
-    p.splits = (int)std::min<long long>(want, std::max(1, blocks / WARPS));
+    // one wave of CTAs, each with at least a block for every warp
+    const long long want = std::max<long long>(1, (long long)CTAS_PER_SM * sm_count / ctas);
+    p.splits = (int)std::min<long long>(want, std::max(1, (blocks + WARPS - 1) / WARPS));
+    // More splits than a cluster has cost a second kernel, about as long as a warp takes for 6 blocks.
+    if (p.splits > MAX_CLUSTER && blocks <= 6 * WARPS * MAX_CLUSTER) p.splits = MAX_CLUSTER;
+    // A cluster lives in one of the 8 GPCs: what does not divide their places would wait for a second wave.
+    const int places = CTAS_PER_SM * sm_count / 8;
+    while (p.splits > 1 && p.splits <= MAX_CLUSTER && ctas > 8 * (places / p.splits)) p.splits--;
     return p;
 }
 
+// What each of n softmax states (m, l) weighs in their sum: f[i] = 2^(m_i - max), and the sum of l f.
+struct Sum {
+    float m, l;
+};
+template <typename M>
+ZWG_DEV Sum weigh(int n, M state, float* f, int step) {
+    Sum x{-INFINITY, 0.f};
+    for (int i = 0; i < n; i++) x.m = fmaxf(x.m, state(i).x);
+    const float base = x.m == -INFINITY ? 0.f : x.m;
+    for (int i = 0; i < n; i++) {
+        const float2 ml = state(i);
+        f[i * step] = exp2_approx(ml.x - base);
+        x.l += ml.y * f[i * step];
+    }
+    return x;
+}
+
+ZWG_DEV void add4(float4& a, float f, float4 x) {
+    a.x += f * x.x;
+    a.y += f * x.y;
+    a.z += f * x.z;
+    a.w += f * x.w;
+}
+
+// Four output elements of a row whose weights sum to l (0: no key was seen).
+ZWG_DEV void store4(float* out, float4 o, float inv, bool vec) {
+    const float4 y = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    if (vec) {
+        *reinterpret_cast<float4*>(out) = y;
+    } else {
+        out[0] = y.x;
+        out[1] = y.y;
+        out[2] = y.z;
+        out[3] = y.w;
+    }
+}
+ZWG_DEV void store4(__nv_bfloat16* out, float4 o, float inv, bool vec) {
+    __nv_bfloat162 y[2] = {__floats2bfloat162_rn(o.x * inv, o.y * inv), __floats2bfloat162_rn(o.z * inv, o.w * inv)};
+    if (vec) {
+        *reinterpret_cast<uint2*>(out) = *reinterpret_cast<uint2*>(y);
+    } else {
+        out[0] = y[0].x;
+        out[1] = y[0].y;
+        out[2] = y[1].x;
+        out[3] = y[1].y;
+    }
+}
+
+// 16 consecutive elements as f32.
+ZWG_DEV void load16(const float* q, float (&x)[16], bool vec) {
+    if (vec) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float4 v = reinterpret_cast<const float4*>(q)[i];
+            x[i * 4] = v.x, x[i * 4 + 1] = v.y, x[i * 4 + 2] = v.z, x[i * 4 + 3] = v.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; i++) x[i] = q[i];
+    }
+}
+ZWG_DEV void load16(const __nv_bfloat16* q, float (&x)[16], bool vec) {
+    if (vec) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const uint4 v = reinterpret_cast<const uint4*>(q)[i];
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                x[i * 8 + j * 2] = __uint_as_float(w[j] << 16);
+                x[i * 8 + j * 2 + 1] = __uint_as_float(w[j] & 0xffff0000u);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; i++) x[i] = __bfloat162float(q[i]);
+    }
+}
+
+// The blocks [from, to) of a split: the tile's keys first .. past + (the last row's query).
+struct Range {
+    int rows, row0, last_row, first, seen_by_all, from, to;
+};
+template <int R>
+ZWG_DEV Range range_of(Place at, int first, int group, int tile, int split, int splits) {
+    Range r;
+    r.rows = at.count * group;
+    r.row0 = tile * R;
+    r.last_row = min(r.rows, r.row0 + R) - 1;
+    r.first = first;
+    const int q0 = r.row0 / group, q1 = r.last_row / group;
+    r.seen_by_all = at.past + q0 + 1;  // keys the tile's first row sees
+    const int lo = first / KV8_BLOCK, n = max(0, (at.past + q1 + KV8_BLOCK) / KV8_BLOCK - lo);
+    const int each = n / splits, more = n - each * splits;
+    r.from = lo + split * each + min(split, more);
+    r.to = r.from + each + (split < more ? 1 : 0);
+    return r;
+}
+
+ZWG_DEV void bulk_hint(const void* src, uint32_t bytes) {
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(bytes) : "memory");
+}
+
+// A bulk copy into a stage of a warp's ring.
+ZWG_DEV void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                     sm100::smem_u32(dst)),
+                 "l"(src), "r"(bytes), "r"(sm100::smem_u32(bar))
+                 : "memory");
+}
+
 template <typename T, int D, int NT, int P>
-__global__ void __launch_bounds__(32 * WARPS) kv8_split_kernel(Kv8Attn p, int splits, float scale) {
+__global__ void __launch_bounds__(32 * WARPS)
+    kv8_split_kernel(Kv8Attn p, int splits, int clustered, int vec, float scale) {
     chain_release();
-    const int z = chain_wait();
     constexpr int R = 8 * NT, CH = D / 64, LDO = D + 4;
-    extern __shared__ float sm_o[];  // [WARPS][R][LDO], then m and l [WARPS][R]
-    float* sm_m = sm_o + WARPS * R * LDO;
-    float* sm_l = sm_m + WARPS * R;
-    const int split = blockIdx.x % splits, tile = blockIdx.x / splits;
-    const int bh = blockIdx.y, b = bh / p.c.n_head_kv, h = bh % p.c.n_head_kv;
+    constexpr int BYTES = KV8_BLOCK * D, STAGES = RING / (WARPS * 2 * BYTES);
+    static_assert(WARPS * R * LDO * sizeof(float) <= RING, "the merge fits the ring");
+    extern __shared__ __align__(128) unsigned char ring[];
+    __shared__ uint64_t full[WARPS][STAGES];
+    __shared__ float2 state[WARPS][R], merged[R];
+    __shared__ float weight[WARPS > MAX_CLUSTER ? WARPS : MAX_CLUSTER][R], inv_l[R];
+    const int tile = blockIdx.x / splits, split = blockIdx.x - tile * splits;
+    const int bh = blockIdx.y, b = bh / p.c.n_head_kv, h = bh - b * p.c.n_head_kv;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const int group = p.n_head / p.c.n_head_kv;
-    const Place at = place_of(p.s, b, p.c.blocks * KV8_BLOCK, threadIdx.x == 0 && blockIdx.x == 0 && h == 0 ? p.err : nullptr);
-    const int rows = at.count * group, row0 = tile * R;
-    if (row0 >= rows) return;
-    int first = p.s.first ? __ldcg(p.s.first + b + z) : 0;
+    const int group = p.n_head / p.c.n_head_kv, room = p.c.blocks * KV8_BLOCK;
+    const size_t head = (size_t)bh * p.c.blocks;
+    if (lane == 0) {
+        for (int s = 0; s < STAGES; s++) sm100::mbar_init(&full[warp][s], 1);
+        sm100::fence_mbar_init();
+        sm100::fence_proxy_async_smem();
+        // before the kernel ahead is through: a hint to L2 for the warp's first blocks, from places that
+        // kernel may still be changing (held within the cache, and read again below)
+        Place hint{p.s.past ? min(max(__ldcg(p.s.past + b), 0), room - 1) : p.s.n_past,
+                   p.s.count ? min(max(__ldcg(p.s.count + b), 1), p.s.n) : p.s.n};
+        const int f = p.s.first ? min(max(__ldcg(p.s.first + b), 0), room - 1) : 0;
+        const Range r = range_of<R>(hint, f, group, tile, split, splits);
+        for (int s = 0; s < STAGES; s++) {
+            const int blk = r.from + warp + s * WARPS;
+            if (blk < r.to && blk < p.c.blocks) {
+                bulk_hint(p.c.k + (head + blk) * BYTES, BYTES);
+                bulk_hint(p.c.v + (head + blk) * BYTES, BYTES);
+            }
+        }
+    }
+    const int z = chain_wait();
+    const Place at = place_of(p.s, b, room, threadIdx.x == 0 && blockIdx.x == 0 && h == 0 ? p.err : nullptr);
+    const int first = p.s.first ? __ldcg(p.s.first + b + z) : 0;
+    const Range rg = range_of<R>(at, max(first, 0), group, tile, split, splits);
+    const int rows = rg.rows, row0 = rg.row0, from = rg.from, to = rg.to;
+    if (row0 >= rows) return;  // the same for every CTA of a cluster
     if (first < 0) {
         if (threadIdx.x == 0) set_error(p.err, kErrBounds);
         return;
     }
-    const int last_row = min(rows, row0 + R) - 1;
-    const int seen = at.past + last_row / group + 1;  // keys the tile's last row sees
-    const int blk_lo = first / KV8_BLOCK, blk_hi = (seen + KV8_BLOCK - 1) / KV8_BLOCK;
-    const int n_blk = max(0, blk_hi - blk_lo);
-    const int from = blk_lo + (int)((long long)n_blk * split / splits);
-    const int to = blk_lo + (int)((long long)n_blk * (split + 1) / splits);
+
+    unsigned char* mine = ring + warp * (STAGES * 2 * BYTES);
+    const auto load = [&](int blk, int stage) {
+        sm100::mbar_arrive_expect_tx(&full[warp][stage], 2 * BYTES);
+        bulk_load(mine + stage * 2 * BYTES, p.c.k + (head + blk) * BYTES + z, BYTES, &full[warp][stage]);
+        bulk_load(mine + stage * 2 * BYTES + BYTES, p.c.v + (head + blk) * BYTES + z, BYTES, &full[warp][stage]);
+    };
+    if (lane == 0)
+        for (int s = 0; s < STAGES; s++)
+            if (from + warp + s * WARPS < to) load(from + warp + s * WARPS, s);
+    __syncwarp();
+    float next_ks = 0.f, next_vs = 0.f;
+    if (from + warp < to) {
+        next_ks = __ldcg(p.c.k_scale + head + from + warp + z);
+        next_vs = __ldcg(p.c.v_scale + head + from + warp + z);
+    }
 
     // queries: the B operand, lane (g, t) holds row g's 16 consecutive elements of each 64
     uint32_t qf[NT][CH][4][P][2];
@@ -136,18 +292,18 @@ __global__ void __launch_bounds__(32 * WARPS) kv8_split_kernel(Kv8Attn p, int sp
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
         const int row = row0 + nt * 8 + g;
-        float x[CH][16];
+        float x[CH][16] = {};
         float top = 0.f;
-        const bool live = row < rows;
-        const T* q = static_cast<const T*>(p.q.data) + z + b * p.q.bs +
-                     (live ? (row / group) * p.q.ts + (size_t)(h * group + row % group) * D : 0);
+        if (row < rows) {
+            const int i = row / group;
+            const T* q = static_cast<const T*>(p.q.data) + z + b * p.q.bs + i * p.q.ts + (size_t)(h * group + row - i * group) * D;
 #pragma unroll
-        for (int i = 0; i < CH; i++)
+            for (int c = 0; c < CH; c++) load16(q + c * 64 + t * 16, x[c], vec & 1);
+        }
 #pragma unroll
-            for (int e = 0; e < 16; e++) {
-                x[i][e] = live ? up(q[i * 64 + t * 16 + e]) : 0.f;
-                top = fmaxf(top, fabsf(x[i][e]));
-            }
+        for (int c = 0; c < CH; c++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) top = fmaxf(top, fabsf(x[c][e]));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         float pw, inv;
@@ -172,7 +328,7 @@ __global__ void __launch_bounds__(32 * WARPS) kv8_split_kernel(Kv8Attn p, int sp
     }
 
     float o[D / 16][NT][4] = {}, m[NT][2], l[NT][2];
-    float ref = 0.f;  // the largest vs so far
+    uint32_t ref = 0x00800000u;  // bits of a power of two above every vs so far (2^-126 at least)
 #pragma unroll
     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -181,17 +337,31 @@ __global__ void __launch_bounds__(32 * WARPS) kv8_split_kernel(Kv8Attn p, int sp
             l[nt][e] = 0.f;
         }
 
-    const size_t head = (size_t)bh * p.c.blocks;
+    int stage = 0;
+    uint32_t phase = 0;
     for (int blk = from + warp; blk < to; blk += WARPS) {
-        const int8_t* kb = p.c.k + (head + blk) * (KV8_BLOCK * D) + z;
-        const int8_t* vb = p.c.v + (head + blk) * (KV8_BLOCK * D) + z;
-        float ks = __ldcg(p.c.k_scale + head + blk + z), vs = __ldcg(p.c.v_scale + head + blk + z);
+        float ks = next_ks, vs = next_vs;
+        if (blk + WARPS < to) {
+            next_ks = __ldcg(p.c.k_scale + head + blk + WARPS + z);
+            next_vs = __ldcg(p.c.v_scale + head + blk + WARPS + z);
+        }
         if (vs != vs) {  // values that read as NaN: through the scores, which a mask covers
             ks = vs;
             vs = 0.f;
         }
+        if (!sm100::mbar_wait_warp(&full[warp][stage], phase, p.err)) {
+            // gave up: no further copies; those on their way end before the ring is used again
+            for (int s = 0; s < STAGES && blk + s * WARPS < to; s++) {
+                const int at_stage = (stage + s) % STAGES;
+                sm100::mbar_wait_drain(&full[warp][at_stage], at_stage < stage ? phase ^ 1 : phase);
+            }
+            break;
+        }
+        const unsigned char* kb = mine + stage * 2 * BYTES;
+        const unsigned char* vb = kb + BYTES;
         // S^T: rows are tokens, logical row (mt, hf, r) is token (r / 2) * 8 + mt * 4 + hf * 2 + r % 2
-        float s[2][NT][4] = {};
+        // (two sums for each: shorter chains of dependent products)
+        float s[2][NT][4] = {}, s2[2][NT][4] = {};
         uint4 kw[2][2][CH];
 #pragma unroll
         for (int mt = 0; mt < 2; mt++)
@@ -199,14 +369,8 @@ __global__ void __launch_bounds__(32 * WARPS) kv8_split_kernel(Kv8Attn p, int sp
             for (int hf = 0; hf < 2; hf++)
 #pragma unroll
                 for (int i = 0; i < CH; i++)
-                    kw[mt][hf][i] = __ldcg(reinterpret_cast<const uint4*>(
-                        kb + ((g >> 1) * 8 + mt * 4 + hf * 2 + (g & 1)) * D + i * 64 + t * 16));
-        uint2 vw[D / 16][2];
-#pragma unroll
-        for (int j = 0; j < D / 16; j++)
-#pragma unroll
-            for (int hf = 0; hf < 2; hf++)
-                vw[j][hf] = __ldcg(reinterpret_cast<const uint2*>(vb + (j * 16 + hf * 8 + g) * KV8_BLOCK + t * 8));
+                    kw[mt][hf][i] = *reinterpret_cast<const uint4*>(
+                        kb + ((g >> 1) * 8 + mt * 4 + hf * 2 + (g & 1)) * D + i * 64 + t * 16);
 #pragma unroll
         for (int i = 0; i < CH; i++)
 #pragma unroll
@@ -220,15 +384,23 @@ __global__ void __launch_bounds__(32 * WARPS) kv8_split_kernel(Kv8Attn p, int sp
                     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                         for (int c = 0; c < P; c++)
-                            mma(s[mt][nt], a0, a1, a2, a3, qf[nt][i][st][c][0], qf[nt][i][st][c][1]);
+                            mma((P == 2 ? c : i & 1) ? s2[mt][nt] : s[mt][nt], a0, a1, a2, a3, qf[nt][i][st][c][0],
+                                qf[nt][i][st][c][1]);
                 }
+#pragma unroll
+        for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) s[mt][nt][e] += s2[mt][nt][e];
         // softmax over the block, for the columns 2t and 2t + 1
-        const float top = fmaxf(ref, vs);
-        const float ratio = top > 0.f ? vs / top : 0.f;
-        const float shrink = top > 0.f ? ref / top : 1.f;
+        const uint32_t top = max(ref, (__float_as_uint(vs) & 0x7f800000u) + 0x00800000u);
+        const float inv_top = __uint_as_float(0x7f000000u - top);
+        const float ratio = vs * inv_top, shrink = __uint_as_float(ref) * inv_top;
         ref = top;
         uint32_t pt[2][2][NT][P];
         const int key0 = blk * KV8_BLOCK;
+        const bool masked = key0 + KV8_BLOCK > rg.seen_by_all || key0 < first;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
             float keep[2];
@@ -242,7 +414,8 @@ __global__ void __launch_bounds__(32 * WARPS) kv8_split_kernel(Kv8Attn p, int sp
                     for (int hf = 0; hf < 2; hf++) {
                         const int key = key0 + (g >> 1) * 8 + mt * 4 + hf * 2 + (g & 1);
                         float& x = s[mt][nt][hf * 2 + e];
-                        x = key < lim[nt][e] && key >= first ? x * f : -INFINITY;
+                        x *= f;
+                        if (masked && (key >= lim[nt][e] || key < first)) x = -INFINITY;
                         mx = fmaxf(mx, x);
                     }
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
@@ -263,10 +436,12 @@ __global__ void __launch_bounds__(32 * WARPS) kv8_split_kernel(Kv8Attn p, int sp
                 l[nt][e] = l[nt][e] * alpha + sum;
                 keep[e] = alpha * shrink;
             }
+            if (__any_sync(0xffffffffu, keep[0] != 1.f || keep[1] != 1.f)) {
 #pragma unroll
-            for (int j = 0; j < D / 16; j++)
+                for (int j = 0; j < D / 16; j++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) o[j][nt][e] *= keep[e & 1];
+                    for (int e = 0; e < 4; e++) o[j][nt][e] *= keep[e & 1];
+            }
             const float f = ratio * kUnit;
 #pragma unroll
             for (int mt = 0; mt < 2; mt++)
@@ -279,21 +454,34 @@ __global__ void __launch_bounds__(32 * WARPS) kv8_split_kernel(Kv8Attn p, int sp
                 }
         }
 #pragma unroll
-        for (int j = 0; j < D / 16; j++)
+        for (int j = 0; j < D / 16; j++) {
+            uint2 vw[2];
+#pragma unroll
+            for (int hf = 0; hf < 2; hf++)
+                vw[hf] = *reinterpret_cast<const uint2*>(vb + (j * 16 + hf * 8 + g) * KV8_BLOCK + t * 8);
 #pragma unroll
             for (int mt = 0; mt < 2; mt++) {
                 uint32_t a0, a1, a2, a3;
-                ints_to_f16(mt ? vw[j][0].y : vw[j][0].x, a0, a2);
-                ints_to_f16(mt ? vw[j][1].y : vw[j][1].x, a1, a3);
+                ints_to_f16(mt ? vw[0].y : vw[0].x, a0, a2);
+                ints_to_f16(mt ? vw[1].y : vw[1].x, a1, a3);
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                     for (int c = 0; c < P; c++) mma(o[j][nt], a0, a1, a2, a3, pt[mt][0][nt][c], pt[mt][1][nt][c]);
             }
+        }
+        __syncwarp();  // every lane has read the stage
+        if (lane == 0 && blk + STAGES * WARPS < to) load(blk + STAGES * WARPS, stage);
+        if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1;
+        }
     }
 
     // the warp's state: sums over the lanes, O in its true units
-    const float units = ref * (1.f / kUnit);
+    __syncthreads();  // every warp is through with the ring
+    float* sm_o = reinterpret_cast<float*>(ring);  // [WARPS][R][LDO]
+    const float units = __uint_as_float(ref) * (1.f / kUnit);
 #pragma unroll
     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -303,10 +491,7 @@ __global__ void __launch_bounds__(32 * WARPS) kv8_split_kernel(Kv8Attn p, int sp
             sum += __shfl_xor_sync(0xffffffffu, sum, 8);
             sum += __shfl_xor_sync(0xffffffffu, sum, 16);
             const int r = nt * 8 + 2 * t + e;
-            if (g == 0) {
-                sm_m[warp * R + r] = m[nt][e];
-                sm_l[warp * R + r] = sum;
-            }
+            if (g == 0) state[warp][r] = make_float2(m[nt][e], sum);
             float* row = sm_o + (warp * R + r) * LDO;
 #pragma unroll
             for (int j = 0; j < D / 16; j++) {
@@ -315,72 +500,143 @@ __global__ void __launch_bounds__(32 * WARPS) kv8_split_kernel(Kv8Attn p, int sp
             }
         }
     __syncthreads();
-    for (int idx = threadIdx.x; idx < R * D; idx += 32 * WARPS) {
-        const int r = idx / D, c = idx % D, row = row0 + r;
-        if (row >= rows) break;
-        float mx = -INFINITY;
+    if (threadIdx.x < R) {
+        const int r = threadIdx.x;
+        const Sum x = weigh(WARPS, [&](int w) { return state[w][r]; }, &weight[0][r], R);
+        merged[r] = make_float2(x.m, x.l);
+        inv_l[r] = x.l == 0.f ? 0.f : 1.f / x.l;
+    }
+    __syncthreads();
+    // a thread has the same four columns of every row it takes
+    constexpr int ROWS_AT_ONCE = 32 * WARPS / (D / 4);
+    const int live = rg.last_row - row0 + 1, c4 = threadIdx.x % (D / 4) * 4, r0 = threadIdx.x / (D / 4);
+    T* out = static_cast<T*>(const_cast<void*>(p.out.data)) + z + b * p.out.bs + (size_t)h * group * D + c4;
+    for (int r = r0; r < live; r += ROWS_AT_ONCE) {
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int w = 0; w < WARPS; w++) mx = fmaxf(mx, sm_m[w * R + r]);
-        const float base = mx == -INFINITY ? 0.f : mx;
-        float sum = 0.f, acc = 0.f;
-#pragma unroll
-        for (int w = 0; w < WARPS; w++) {
-            const float f = exp2_approx(sm_m[w * R + r] - base);
-            sum += sm_l[w * R + r] * f;
-            acc += sm_o[(w * R + r) * LDO + c] * f;
-        }
+        for (int w = 0; w < WARPS; w++)
+            add4(acc, weight[w][r], *reinterpret_cast<const float4*>(sm_o + (w * R + r) * LDO + c4));
         if (splits == 1) {
-            T* out = static_cast<T*>(const_cast<void*>(p.out.data)) + z + b * p.out.bs + (row / group) * p.out.ts +
-                     (size_t)(h * group + row % group) * D + c;
-            down(sum == 0.f ? 0.f : acc / sum, *out);
+            const int row = row0 + r, i = row / group;
+            store4(out + i * p.out.ts + (size_t)(row - i * group) * D, acc, inv_l[r], vec & 2);
+        } else if (clustered) {
+            *reinterpret_cast<float4*>(sm_o + r * LDO + c4) = acc;  // warp 0's, which no other thread reads
         } else {
-            float* ws = p.ws + z + (((size_t)bh * gridDim.x + blockIdx.x) * R + r) * (D + 2);
-            ws[2 + c] = acc;
-            if (c == 0) {
-                ws[0] = mx;
-                ws[1] = sum;
-            }
+            float* ws = p.ws + z + (((size_t)bh * gridDim.x + blockIdx.x) * R + r) * (D + 4);
+            *reinterpret_cast<float4*>(ws + 4 + c4) = acc;
+            if (c4 == 0) *reinterpret_cast<float2*>(ws) = merged[r];
         }
     }
+    if (splits == 1 || !clustered) return;
+    // the cluster's CTAs: row r's outputs are the CTA's of rank r modulo their number
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    if (threadIdx.x < R) {
+        const int r = threadIdx.x;
+        const Sum x = weigh(splits, [&](int s) { return *cluster.map_shared_rank(&merged[r], s); }, &weight[0][r], R);
+        inv_l[r] = x.l == 0.f ? 0.f : 1.f / x.l;
+    }
+    __syncthreads();
+    for (int r = split + splits * r0; r < live; r += splits * ROWS_AT_ONCE) {
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int s = 0; s < splits; s++)
+            add4(acc, weight[s][r], *reinterpret_cast<const float4*>(cluster.map_shared_rank(sm_o, s) + r * LDO + c4));
+        const int row = row0 + r, i = row / group;
+        store4(out + i * p.out.ts + (size_t)(row - i * group) * D, acc, inv_l[r], vec & 2);
+    }
+    cluster.sync();  // the others have read this CTA's shared memory
 }
 
-// One CTA of D threads per query row: the splits' partials to the output.
+// A CTA of 256 threads takes a query row: the splits' partials to the output. The weights of up to
+// CHUNK splits at a time meet in shared memory, then each group of D / 4 threads sums every so many
+// splits' O and the groups' sums are added.
 template <typename T, int D>
-__global__ void __launch_bounds__(D) kv8_combine_kernel(Kv8Attn p, int splits, int R) {
+__global__ void __launch_bounds__(256) kv8_combine_kernel(Kv8Attn p, int splits, int R, int vec) {
     chain_release();
     const int z = chain_wait();
-    const int bh = blockIdx.y, b = bh / p.c.n_head_kv, h = bh % p.c.n_head_kv, row = blockIdx.x, c = threadIdx.x;
-    const int group = p.n_head / p.c.n_head_kv;
+    constexpr int GROUPS = 256 / (D / 4);
+    extern __shared__ float f[];  // [splits]
+    __shared__ float part[8];
+    __shared__ float4 sums[GROUPS][D / 4];
+    const int bh = blockIdx.y, b = bh / p.c.n_head_kv, h = bh - b * p.c.n_head_kv, row = blockIdx.x;
+    const int group = p.n_head / p.c.n_head_kv, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const Place at = place_of(p.s, b, p.c.blocks * KV8_BLOCK, nullptr);
     if (row >= at.count * group || (p.s.first && __ldcg(p.s.first + b + z) < 0)) return;
     const int tiles = (p.s.n * group + R - 1) / R;
-    const float* ws = p.ws + z + (((size_t)bh * tiles + row / R) * splits * R + row % R) * (D + 2);
-    const size_t step = (size_t)R * (D + 2);
+    const size_t step = (size_t)R * (D + 4);
+    const float* ws = p.ws + z + ((size_t)bh * tiles + row / R) * splits * step + (row % R) * (D + 4);
     float mx = -INFINITY;
-    for (int s = 0; s < splits; s++) mx = fmaxf(mx, __ldcg(ws + s * step));
+    for (int s = threadIdx.x; s < splits; s += 256) mx = fmaxf(mx, __ldcg(ws + s * step));
+    mx = warp_max(mx);
+    if (lane == 0) part[warp] = mx;
+    __syncthreads();
+    mx = part[0];
+#pragma unroll
+    for (int w = 1; w < 8; w++) mx = fmaxf(mx, part[w]);
     const float base = mx == -INFINITY ? 0.f : mx;
-    float sum = 0.f, acc = 0.f;
-    for (int s = 0; s < splits; s++) {
-        const float f = exp2_approx(__ldcg(ws + s * step) - base);
-        sum += __ldcg(ws + s * step + 1) * f;
-        acc += __ldcg(ws + s * step + 2 + c) * f;
+    float sum = 0.f;
+    for (int s = threadIdx.x; s < splits; s += 256) {
+        const float2 ml = __ldcg(reinterpret_cast<const float2*>(ws + s * step));
+        f[s] = exp2_approx(ml.x - base);
+        sum += ml.y * f[s];
     }
-    T* out = static_cast<T*>(const_cast<void*>(p.out.data)) + z + b * p.out.bs + (row / group) * p.out.ts +
-             (size_t)(h * group + row % group) * D + c;
-    down(sum == 0.f ? 0.f : acc / sum, *out);
+    sum = warp_sum(sum);
+    __syncthreads();
+    if (lane == 0) part[warp] = sum;
+    __syncthreads();
+    sum = part[0];
+#pragma unroll
+    for (int w = 1; w < 8; w++) sum += part[w];
+    const int c = threadIdx.x % (D / 4), first = threadIdx.x / (D / 4);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int s = first; s < splits; s += GROUPS)
+        add4(acc, f[s], __ldcg(reinterpret_cast<const float4*>(ws + s * step + 4) + c));
+    sums[first][c] = acc;
+    __syncthreads();
+    if (first > 0) return;
+#pragma unroll
+    for (int w = 1; w < GROUPS; w++) add4(acc, 1.f, sums[w][c]);
+    const int i = row / group;
+    T* out = static_cast<T*>(const_cast<void*>(p.out.data)) + z + b * p.out.bs + i * p.out.ts +
+             (size_t)(h * group + row - i * group) * D + c * 4;
+    store4(out, acc, sum == 0.f ? 0.f : 1.f / sum, vec & 2);
+}
+
+// Rows whose elements can be read or written 16 bytes (of f32; 8 of bf16) at a time.
+bool wide(const Rows& r, size_t elem, size_t bytes) {
+    return ((uintptr_t)r.data | (r.bs * elem) | (r.ts * elem)) % bytes == 0;
 }
 
 template <typename T, int D, int NT, int P>
 int split_launch(const Kv8Attn& p, const Plan& plan, cudaStream_t st) {
-    constexpr size_t smem = WARPS * 8 * NT * (D + 4 + 2) * sizeof(float);
-    static_assert(smem <= 48 * 1024, "the merge fits without opting in");
     const float scale = (float)(1.0 / sqrt((double)D)) * kLog2e;
     const int rows = p.s.n * (p.n_head / p.c.n_head_kv);
     const unsigned segs = (unsigned)(p.s.n_batch * p.c.n_head_kv);
-    cudaError_t e = launch_chained_smem(kv8_split_kernel<T, D, NT, P>, dim3((unsigned)(plan.tiles * plan.splits), segs),
-                                        dim3(32 * WARPS), smem, st, p, plan.splits, scale);
-    if (e == cudaSuccess && plan.splits > 1)
-        e = launch_chained(kv8_combine_kernel<T, D>, dim3((unsigned)rows, segs), dim3(D), st, p, plan.splits, 8 * NT);
+    const int clustered = plan.splits <= MAX_CLUSTER;
+    const auto kern = kv8_split_kernel<T, D, NT, P>;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)RING) != cudaSuccess ||
+        cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+        return -1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(plan.tiles * plan.splits), segs);
+    cfg.blockDim = dim3(32 * WARPS);
+    cfg.dynamicSmemBytes = RING;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = clustered ? (unsigned)plan.splits : 1;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    const int vec = (wide(p.q, sizeof(T), 16) ? 1 : 0) | (wide(p.out, sizeof(T), 4 * sizeof(T)) ? 2 : 0);
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p, plan.splits, clustered, vec, scale);
+    if (e == cudaSuccess && !clustered)
+        e = launch_chained_smem(kv8_combine_kernel<T, D>, dim3((unsigned)rows, segs), dim3(256),
+                                plan.splits * sizeof(float), st, p, plan.splits, 8 * NT, vec);
     return e == cudaSuccess ? 0 : -1;
 }
 
@@ -388,8 +644,9 @@ template <typename T, int D>
 int attn(const Kv8Attn& p, int pieces, int sm_count, cudaStream_t st) {
     const Plan plan = plan_for(p.c, p.s, p.n_head, sm_count);
     const bool small = p.s.n * (p.n_head / p.c.n_head_kv) <= 8;
-    if (pieces == 1) return small ? split_launch<T, D, 1, 1>(p, plan, st) : split_launch<T, D, 2, 1>(p, plan, st);
-    return small ? split_launch<T, D, 1, 2>(p, plan, st) : split_launch<T, D, 2, 2>(p, plan, st);
+    if constexpr (sizeof(T) == 4)
+        if (pieces == 2) return small ? split_launch<T, D, 1, 2>(p, plan, st) : split_launch<T, D, 2, 2>(p, plan, st);
+    return small ? split_launch<T, D, 1, 1>(p, plan, st) : split_launch<T, D, 2, 1>(p, plan, st);
 }
 
 }  // namespace
@@ -398,8 +655,8 @@ size_t kv8_attn_workspace_bytes(const Kv8& c, const Seqs& s, int n_head, int sm_
     if (s.n_batch == 0 || s.n == 0) return 0;
     const Plan p = plan_for(c, s, n_head, sm_count);
     const int rows = s.n * (n_head / c.n_head_kv);
-    return p.splits == 1 ? 0
-                         : (size_t)s.n_batch * c.n_head_kv * p.tiles * p.splits * tile_rows(rows) * (c.d + 2) * sizeof(float);
+    return p.splits <= MAX_CLUSTER ? 0
+                         : (size_t)s.n_batch * c.n_head_kv * p.tiles * p.splits * tile_rows(rows) * (c.d + 4) * sizeof(float);
 }
 
 int kv8_attn_launch(const Kv8Attn& p, int type, int pieces, int sm_count, cudaStream_t st) {

@@ -23,6 +23,7 @@ states `DecoderState` and `LlmState`; the Q8 projections `quantize_q8`, `linear_
 from __future__ import annotations
 
 import ctypes
+import operator
 from dataclasses import dataclass
 from typing import Optional
 
@@ -834,59 +835,62 @@ def _row_type(t, name):
     torch = _torch()
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
-    if t.dtype == torch.float32:
+    if t.dtype is torch.float32:
         return _lib.ZWG_TYPE_F32
-    if t.dtype == torch.bfloat16:
+    if t.dtype is torch.bfloat16:
         return _lib.ZWG_TYPE_BF16
     raise ValueError(f"{name} must be float32 or bfloat16, got {t.dtype}")
 
 
-def _rows(t, like, heads: Optional[int], name: str) -> _lib.RowsC:
-    """Rows of heads [n_batch][n][heads][d] (any batch and token strides) of `like`'s batch, tokens,
-    d, type and device."""
-    if t.dim() != 4 or t.dtype != like.dtype or t.device != like.device:
-        raise ValueError(f"{name} must be a [n_batch][n][heads][d] tensor of {like.dtype} on {like.device}")
-    if t.shape[0] != like.shape[0] or t.shape[1] != like.shape[1] or t.shape[3] != like.shape[3]:
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, which does not go with {tuple(like.shape)}")
-    if heads is not None and t.shape[2] != heads:
-        raise ValueError(f"{name} must have {heads} heads, got {t.shape[2]}")
+def _rows(t, dtype, device, shape, name: str):
+    """A reference to the zwg_rows of t [n_batch][n][heads][d] (any batch and token strides), which
+    must have this type, device and shape."""
+    if t.dtype is not dtype or t.device != device or t.shape != shape:
+        raise ValueError(f"{name} must be {dtype} of shape {tuple(shape)} on {device}, got {t.dtype} of {tuple(t.shape)} on "
+                         f"{t.device}")
     sb, st, sh, sd = t.stride()
-    if (t.shape[3] > 1 and sd != 1) or (t.shape[2] > 1 and sh != t.shape[3]):
+    if (sd != 1 and shape[3] > 1) or (sh != shape[3] and shape[2] > 1):
         raise ValueError(f"{name}: a token's heads must lie one after another")
-    return _lib.RowsC(t.data_ptr(), sb, st)
+    return ctypes.byref(_lib.RowsC(t.data_ptr(), sb, st))
 
 
 def _int32_of(t, device, shape, name):
     torch = _torch()
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != device or tuple(t.shape) != shape:
+    if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or t.device != device or t.shape != shape:
         raise ValueError(f"{name} must be an int32 tensor of shape {shape} on {device}")
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
     return t.data_ptr()
 
 
-def _seqs(n_batch: int, n: int, n_past, count, first, max_past, device) -> _lib.SeqsC:
-    """zwg_seqs of a call: n_past a number, or an int32 tensor [n_batch] whose entries are at
-    most max_past."""
-    torch = _torch()
+def _seqs(n_batch: int, n: int, n_past, count, first, max_past, device):
+    """A reference to the zwg_seqs of a call: n_past a number, or an int32 tensor [n_batch] whose
+    entries are at most max_past."""
     past = None
-    if isinstance(n_past, torch.Tensor):
-        past = _int32_of(n_past, device, (n_batch,), "n_past")
-        n_past = max_past
+    if type(n_past) is not int:
+        if isinstance(n_past, _torch().Tensor):
+            past = _int32_of(n_past, device, (n_batch,), "n_past")
+            n_past = max_past
+        n_past = operator.index(n_past)
     if n_past < 0:
         raise ValueError(f"n_past must not be negative, got {n_past}")
-    return _lib.SeqsC(n_batch, n, n_past, past,
-                      None if count is None else _int32_of(count, device, (n_batch,), "count"),
-                      None if first is None else _int32_of(first, device, (n_batch,), "first"))
+    return ctypes.byref(_lib.SeqsC(n_batch, n, n_past, past,
+                                   None if count is None else _int32_of(count, device, (n_batch,), "count"),
+                                   None if first is None else _int32_of(first, device, (n_batch,), "first")))
 
 
-def _tables(cos, sin, device, interleaved: bool) -> _lib.RopeTablesC:
+def _stream_on(device):
+    """The current stream of a device, as _stream_of, without making a Stream object for it."""
+    return _torch()._C._cuda_getCurrentRawStream(device.index)
+
+
+def _tables(cos, sin, device, interleaved: bool):
     torch = _torch()
-    for t, name in ((cos, "cos"), (sin, "sin")):
-        if t.dim() != 2 or t.shape != cos.shape or t.device != device:
-            raise ValueError(f"{name} must be [n_ctx][rot / 2] on {device}, cos and sin alike")
-    return _lib.RopeTablesC(_dev_ptr(cos, torch.float32, "cos"), _dev_ptr(sin, torch.float32, "sin"), cos.shape[0],
-                            2 * cos.shape[1], 1 if interleaved else 0)
+    if cos.dim() != 2 or sin.shape != cos.shape or cos.device != device or sin.device != device:
+        raise ValueError(f"cos and sin must be [n_ctx][rot / 2] on {device}, both of one shape")
+    n_ctx, half = cos.shape
+    return ctypes.byref(_lib.RopeTablesC(_dev_ptr(cos, torch.float32, "cos"), _dev_ptr(sin, torch.float32, "sin"), n_ctx,
+                                         2 * half, 1 if interleaved else 0))
 
 
 def rope(q, cos, sin, n_past=0, k=None, interleaved: bool = False, count=None, inplace: bool = True, q_out=None,
@@ -900,28 +904,34 @@ def rope(q, cos, sin, n_past=0, k=None, interleaved: bool = False, count=None, i
     k_out (new tensors with inplace=False). Returns q, or (q, k)."""
     torch = _torch()
     kind = _row_type(q, "q")
-    if q.dim() != 4:
-        raise ValueError("q must be [n_batch][n][n_head][d]")
-    B, n, H, d = q.shape
-    heads_kv = 0 if k is None else k.shape[2] if k.dim() == 4 else -1
-    if not inplace:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else q_out
-        if k is not None and k_out is None:
-            k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    q_out = q if q_out is None else q_out
-    k_out = k if k_out is None else k_out
+    if q.dim() != 4 or (k is not None and k.dim() != 4):
+        raise ValueError("q and k must be [n_batch][n][heads][d]")
     if k is None and k_out is not None:
         raise ValueError("k_out without k")
-    qr, qo = _rows(q, q, H, "q"), _rows(q_out, q, H, "q_out")
-    kr = ko = None
+    B, n, H, d = shape = q.shape
+    dtype, dev = q.dtype, q.device
+    fresh = torch.contiguous_format
+    qo = ko = kr = None  # in place
+    if q_out is None and not inplace:
+        q_out = torch.empty_like(q, memory_format=fresh)
+    if q_out is not None:
+        qo = _rows(q_out, dtype, dev, shape, "q_out")
+    heads_kv = 0
     if k is not None:
-        kr, ko = ctypes.byref(_rows(k, q, None, "k")), ctypes.byref(_rows(k_out, q, heads_kv, "k_out"))
-    _lib.ensure_init(q.device.index or 0)
-    tables = _tables(cos, sin, q.device, interleaved)
-    sq = _seqs(B, n, n_past, count, None, cos.shape[0], q.device)
-    _lib.check(_lib.load().zwg_rope(ctypes.byref(sq), ctypes.byref(tables), kind, d, H, ctypes.byref(qr),
-                                    ctypes.byref(qo), heads_kv, kr, ko, _stream_of(q)))
-    return q_out if k is None else (q_out, k_out)
+        heads_kv = k.shape[2]
+        kv_shape = (B, n, heads_kv, d)
+        kr = _rows(k, dtype, dev, kv_shape, "k")
+        if k_out is None and not inplace:
+            k_out = torch.empty_like(k, memory_format=fresh)
+        if k_out is not None:
+            ko = _rows(k_out, dtype, dev, kv_shape, "k_out")
+    tables = _tables(cos, sin, dev, interleaved)
+    sq = _seqs(B, n, n_past, count, None, cos.shape[0], dev)
+    _lib.ensure_init(dev.index)
+    _lib.check(_lib.load().zwg_rope(sq, tables, kind, d, H, _rows(q, dtype, dev, shape, "q"), qo, heads_kv, kr, ko,
+                                    _stream_on(dev)))
+    q = q if q_out is None else q_out
+    return q if k is None else (q, k if k_out is None else k_out)
 
 
 class Kv8Cache:
@@ -937,6 +947,8 @@ class Kv8Cache:
             raise ValueError("k must be [n_batch][n_head_kv][n_ctx/32][32][d]")
         B, H, nb, _, d = k.shape
         self.n_batch, self.n_head_kv, self.d, self.n_ctx, self.device = B, H, d, 32 * nb, k.device
+        if not k.is_cuda:
+            raise ValueError("the cache's tensors must be on a CUDA device")
         want = (("k", k, torch.int8, (B, H, nb, 32, d)), ("k_scale", k_scale, torch.float32, (B, H, nb)),
                 ("v", v, torch.int8, (B, H, nb, d, 32)), ("v_scale", v_scale, torch.float32, (B, H, nb)),
                 ("k_open", k_open, torch.float32, (B, H, 32, d)), ("v_open", v_open, torch.float32, (B, H, 32, d)),
@@ -947,6 +959,7 @@ class Kv8Cache:
         self._keep = tuple(t for _, t, _, _ in want)
         self.k, self.k_scale, self.v, self.v_scale, self.k_open, self.v_open, self.open_block = self._keep
         self._c = _lib.Kv8C(*(_dev_ptr(t, dtype, name) for name, t, dtype, _ in want), B, H, d, 32 * nb)
+        self._ref = ctypes.byref(self._c)
 
     @classmethod
     def empty(cls, n_batch: int, n_head_kv: int, d: int, n_ctx: int, device: int = 0) -> "Kv8Cache":
@@ -960,8 +973,7 @@ class Kv8Cache:
                    z(n_batch, n_head_kv, 32, d, device=dev), z(n_batch, n_head_kv, 32, d, device=dev),
                    torch.full((n_batch, n_head_kv), -1, dtype=torch.int32, device=dev))
 
-    def _call(self, n: int, n_past, count, first, max_past) -> _lib.SeqsC:
-        _lib.ensure_init(self.device.index or 0)
+    def _call(self, n: int, n_past, count, first, max_past):
         return _seqs(self.n_batch, n, n_past, count, first, self.n_ctx if max_past is None else max_past, self.device)
 
     def append(self, k, v, n_past, count=None, rope=None) -> None:
@@ -969,60 +981,65 @@ class Kv8Cache:
         tensor [n_batch]); count (CUDA int32 [n_batch]): tokens of each sequence. rope: (cos,
         sin) or (cos, sin, interleaved), the rotation of k on its way in."""
         kind = _row_type(k, "k")
-        if k.dim() != 4 or k.shape[0] != self.n_batch or k.shape[2:] != (self.n_head_kv, self.d) or k.device != self.device:
-            raise ValueError(f"k must be [{self.n_batch}][n][{self.n_head_kv}][{self.d}] on {self.device}")
-        kr, vr = _rows(k, k, None, "k"), _rows(v, k, self.n_head_kv, "v")
-        s = self._call(k.shape[1], n_past, count, None, None)
-        t = None
-        if rope is not None:
-            t = ctypes.byref(_tables(rope[0], rope[1], self.device, len(rope) > 2 and rope[2]))
-        _lib.check(_lib.load().zwg_kv8_append(ctypes.byref(self._c), ctypes.byref(s), kind, ctypes.byref(kr),
-                                              ctypes.byref(vr), t, _stream_of(k)))
+        if k.dim() != 4:
+            raise ValueError("k and v must be [n_batch][n][n_head_kv][d]")
+        dev, dtype, n = self.device, k.dtype, k.shape[1]
+        shape = (self.n_batch, n, self.n_head_kv, self.d)
+        t = None if rope is None else _tables(rope[0], rope[1], dev, len(rope) > 2 and rope[2])
+        kr, vr = _rows(k, dtype, dev, shape, "k"), _rows(v, dtype, dev, shape, "v")
+        s = self._call(n, n_past, count, None, None)
+        _lib.ensure_init(dev.index)
+        _lib.check(_lib.load().zwg_kv8_append(self._ref, s, kind, kr, vr, t, _stream_on(dev)))
 
     def read(self, n: int, n_past, count=None, k=None, v=None):
-        """The values of n tokens from position n_past: (k, v) [n_batch][n][n_head_kv][d] f32."""
+        """The values of n tokens from position n_past: (k, v) [n_batch][n][n_head_kv][d] f32, rows
+        behind count[b] as they were (in new tensors: undefined)."""
         torch = _torch()
-        shape = (self.n_batch, n, self.n_head_kv, self.d)
-        out = []
-        for t, name in ((k, "k"), (v, "v")):
-            t = torch.empty(shape, dtype=torch.float32, device=self.device) if t is None else t
-            if tuple(t.shape) != shape or t.device != self.device:
-                raise ValueError(f"{name} must have shape {shape} on {self.device}")
-            out.append(t)
+        shape, dev = (self.n_batch, n, self.n_head_kv, self.d), self.device
+        k = torch.empty(shape, dtype=torch.float32, device=dev) if k is None else k
+        v = torch.empty_like(k) if v is None else v
+        if k.shape != shape or k.device != dev or v.shape != shape or v.device != dev:
+            raise ValueError(f"k and v must have shape {shape} on {dev}")
         s = self._call(n, n_past, count, None, None)
-        _lib.check(_lib.load().zwg_kv8_read(ctypes.byref(self._c), ctypes.byref(s),
-                                            _dev_ptr(out[0], torch.float32, "k"), _dev_ptr(out[1], torch.float32, "v"),
-                                            _stream_of(out[0])))
-        return tuple(out)
+        _lib.ensure_init(dev.index)
+        _lib.check(_lib.load().zwg_kv8_read(self._ref, s, _dev_ptr(k, torch.float32, "k"), _dev_ptr(v, torch.float32, "v"),
+                                            _stream_on(dev)))
+        return k, v
 
     def attn_workspace_bytes(self, n: int, n_head: int, n_past=None) -> int:
         """Workspace of attn for n tokens after n_past (None: the most there can be)."""
         s = self._call(n, max(self.n_ctx - n, 0) if n_past is None else n_past, None, None, None)
-        return int(_lib.load().zwg_kv8_attn_workspace(ctypes.byref(self._c), ctypes.byref(s), n_head))
+        _lib.ensure_init(self.device.index)
+        return int(_lib.load().zwg_kv8_attn_workspace(self._ref, s, n_head))
 
     def attn(self, q, n_past, count=None, first=None, max_past=None, out=None, workspace=None):
         """Attention (zwg_kv8_attn) of q [n_batch][n][n_head][d] (f32 or bf16) at positions n_past..
         (an int, or a CUDA int32 tensor [n_batch] whose entries are at most max_past) over the
         cache, which holds the call's own tokens already: query i of sequence b sees keys
         first[b] .. n_past + i. count, first: CUDA int32 [n_batch]; rows of out behind count[b]
-        stay as they are. Returns out, of q's shape and type."""
+        stay as they are. Returns out, of q's shape and type (a new one has zeros there)."""
         torch = _torch()
         kind = _row_type(q, "q")
-        if q.dim() != 4 or q.shape[0] != self.n_batch or q.shape[3] != self.d or q.device != self.device:
-            raise ValueError(f"q must be [{self.n_batch}][n][n_head][{self.d}] on {self.device}")
+        if q.dim() != 4:
+            raise ValueError("q must be [n_batch][n][n_head][d]")
         n, H = q.shape[1], q.shape[2]
+        dev, dtype, shape = self.device, q.dtype, (self.n_batch, n, H, self.d)
+        qr = _rows(q, dtype, dev, shape, "q")
         if out is None:
-            out = (torch.empty if count is None else torch.zeros)(q.shape, dtype=q.dtype, device=q.device)
-        qr, orow = _rows(q, q, H, "q"), _rows(out, q, H, "out")
+            out = (torch.empty_like if count is None else torch.zeros_like)(q, memory_format=torch.contiguous_format)
+        o = _rows(out, dtype, dev, shape, "out")
         s = self._call(n, n_past, count, first, max_past)
-        lib, c = _lib.load(), ctypes.byref(self._c)
+        _lib.ensure_init(dev.index)
+        lib = _lib.load()
+        ws, size = None, 0
         if workspace is None:
-            need = lib.zwg_kv8_attn_workspace(c, ctypes.byref(s), H)
-            if need:
-                workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-        ws, size = (workspace.data_ptr(), workspace.numel() * workspace.element_size()) if workspace is not None else (0, 0)
-        _lib.check(lib.zwg_kv8_attn(c, ctypes.byref(s), kind, H, ctypes.byref(qr), ctypes.byref(orow), ws, size,
-                                    _stream_of(q)))
+            size = lib.zwg_kv8_attn_workspace(self._ref, s, H)
+            if size:
+                workspace = torch.empty(size, dtype=torch.uint8, device=dev)
+                ws = workspace.data_ptr()
+        else:
+            ws, size = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        _lib.check(lib.zwg_kv8_attn(self._ref, s, kind, H, qr, o, ws, size, _stream_on(dev)))
         return out
 
 
@@ -1037,54 +1054,55 @@ def llm_logits(logits, recent=None, n_recent=None, window: Optional[int] = None,
     int32 words [n_vocab/32 rounded up], for all rows or [m][...]. Returns each row's first index
     of its largest logit, -1 where none is above -inf (CUDA int32 [m], or in `out`)."""
     torch = _torch()
-    if not isinstance(logits, torch.Tensor) or not logits.is_cuda or logits.dtype != torch.float32 or logits.dim() != 2:
+    if not isinstance(logits, torch.Tensor) or not logits.is_cuda or logits.dtype is not torch.float32 or logits.dim() != 2:
         raise ValueError("logits must be a CUDA float32 [m][n_vocab] tensor")
     m, V = logits.shape
-    if V > 1 and logits.stride(1) != 1:
+    stride, inner = logits.stride()
+    if V > 1 and inner != 1:
         raise ValueError("a row's logits must lie one after another")
     dev = logits.device
 
-    def lists(t, dtype, name, width=None):
+    def lists(t, dtype, name):
         """(pointer, row stride, entries) of a list for all rows, or one for each."""
-        if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != dev or t.dim() not in (1, 2):
+        if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.device != dev or t.dim() not in (1, 2):
             raise ValueError(f"{name} must be a {dtype} tensor [n] or [m][n] on {dev}")
-        if t.dim() == 2 and t.shape[0] != m:
-            raise ValueError(f"{name} must have {m} rows, got {t.shape[0]}")
-        if t.shape[-1] > 1 and t.stride(-1) != 1:
+        shape, strides = t.shape, t.stride()
+        if len(shape) == 2 and shape[0] != m:
+            raise ValueError(f"{name} must have {m} rows, got {shape[0]}")
+        if shape[-1] > 1 and strides[-1] != 1:
             raise ValueError(f"{name} must have unit stride along its entries")
-        if width is not None and t.shape[-1] < width:
-            raise ValueError(f"{name} must have {width} entries, got {t.shape[-1]}")
-        return t.data_ptr(), t.stride(0) if t.dim() == 2 else 0, t.shape[-1]
+        return t.data_ptr(), strides[0] if len(shape) == 2 else 0, shape[-1]
 
-    r = _lib.LogitRulesC()
-    r.repeat, r.presence, r.frequency = repeat, presence, frequency
+    r = _lib.LogitRulesC(repeat=repeat, presence=presence, frequency=frequency)
     if recent is not None:
-        r.recent, r.recent_stride, r.n_recent = lists(recent, torch.int32, "recent")
+        r.recent, r.recent_stride, entries = lists(recent, torch.int32, "recent")
+        r.n_recent = entries
         if isinstance(n_recent, torch.Tensor):
             r.n_recents = _int32_of(n_recent, dev, (m,), "n_recent")
         elif n_recent is not None:
-            if not 0 <= n_recent <= recent.shape[-1]:
-                raise ValueError(f"n_recent must be 0 .. {recent.shape[-1]}, got {n_recent}")
+            if not 0 <= n_recent <= entries:
+                raise ValueError(f"n_recent must be 0 .. {entries}, got {n_recent}")
             r.n_recent = n_recent
-        r.window = recent.shape[-1] if window is None else max(window, 0)
+        r.window = entries if window is None else max(window, 0)
     if (bias_ids is None) != (bias is None):
         raise ValueError("bias_ids and bias go together")
     if bias is not None:
-        if bias.shape != bias_ids.shape:
-            raise ValueError("bias_ids and bias must have the same shape")
-        r.bias_ids, stride, r.n_bias = lists(bias_ids, torch.int32, "bias_ids")
-        r.bias, r.bias_stride, _ = lists(bias, torch.float32, "bias")
-        if stride != r.bias_stride:
-            raise ValueError("bias_ids and bias must have the same strides")
+        r.bias_ids, ids_stride, r.n_bias = lists(bias_ids, torch.int32, "bias_ids")
+        r.bias, bias_stride, _ = lists(bias, torch.float32, "bias")
+        if bias.shape != bias_ids.shape or (ids_stride != bias_stride and m > 1):
+            raise ValueError("bias_ids and bias must have the same shape and strides")
+        r.bias_stride = bias_stride
     if allow is not None:
-        r.allow, r.allow_stride, _ = lists(allow, torch.int32, "allow", (V + 31) // 32)
+        r.allow, r.allow_stride, words = lists(allow, torch.int32, "allow")
+        if words < (V + 31) // 32:
+            raise ValueError(f"allow must have {(V + 31) // 32} words, got {words}")
     if out is None:
         out = torch.empty(m, dtype=torch.int32, device=dev)
-    if out.dtype != torch.int32 or tuple(out.shape) != (m,) or out.device != dev or (m > 1 and out.stride(0) < 1):
+    elif out.dtype is not torch.int32 or out.shape != (m,) or out.device != dev or (m > 1 and out.stride(0) < 1):
         raise ValueError(f"out must be an int32 tensor [{m}] on {dev}")
-    _lib.ensure_init(dev.index or 0)
-    _lib.check(_lib.load().zwg_llm_logits(logits.data_ptr(), m, V, logits.stride(0), ctypes.byref(r), out.data_ptr(),
-                                          out.stride(0) if m else 1, _stream_of(logits)))
+    _lib.ensure_init(dev.index)
+    _lib.check(_lib.load().zwg_llm_logits(logits.data_ptr(), m, V, stride, ctypes.byref(r), out.data_ptr(), out.stride(0),
+                                          _stream_on(dev)))
     return out
 
 
