@@ -16,7 +16,7 @@
 // and no shared memory or shuffle stands between memory and the tensor cores.
 // A warp takes whole blocks of the split's range, each one bulk copy of its keys and one of its
 // values into the warp's own ring in shared memory, so a warp never waits for another one before the
-// merge and loads run ahead of the arithmetic (24 KB an SM cover the latency of HBM; 3 CTAs hold 96).
+// merge, and loads run ahead of the arithmetic.
 // The splits of a (sequence, kv head, tile of query rows) that fit a cluster (8 CTAs) meet in each
 // other's shared memory; more of them write partials (m, l, O) for kv8_combine_kernel.
 #include <cuda_bf16.h>
@@ -85,30 +85,37 @@ ZWG_DEV void power_of(float x, float& p, float& inv) {
 
 struct Plan {
     int tiles;   // tiles of query rows of a (sequence, kv head)
+    int warps;   // of a CTA
     int splits;  // cuts of the keys
 };
 
-constexpr int WARPS = 4;
+constexpr int SMALL = 4;            // warps of a small CTA, three of which share an SM
 constexpr int MAX_CLUSTER = 8;
-constexpr int CTAS_PER_SM = 3;
-constexpr size_t RING = 64 * 1024;  // bytes a CTA's warps have for blocks on their way
+constexpr int WARP_RING = 16 * 1024;  // bytes a warp has for blocks on their way
 
 // Rows of a tile: one or two 8-wide N tiles.
 int tile_rows(int rows) { return rows <= 8 ? 8 : 16; }
+// Warps of a CTA that has an SM to itself; the registers of two N tiles leave room for 8.
+constexpr int big_warps(int tile_rows) { return tile_rows == 8 ? 12 : 8; }
 
 Plan plan_for(const Kv8& c, const Seqs& s, int n_head, int sm_count) {
-    const int rows = s.n * (n_head / c.n_head_kv);
+    const int rows = s.n * (n_head / c.n_head_kv), big = big_warps(tile_rows(rows));
     Plan p;
     p.tiles = (rows + tile_rows(rows) - 1) / tile_rows(rows);
     const long long ctas = (long long)s.n_batch * c.n_head_kv * p.tiles;
     const int blocks = (s.n_past + s.n + KV8_BLOCK - 1) / KV8_BLOCK;
-    // one wave of CTAs, each with at least a block for every warp
-    const long long want = std::max<long long>(1, (long long)CTAS_PER_SM * sm_count / ctas);
-    p.splits = (int)std::min<long long>(want, std::max(1, (blocks + WARPS - 1) / WARPS));
+    const int per_sm = big / SMALL;
+    const long long small_places = (long long)per_sm * sm_count;
+    // One wave, of big CTAs (fewer states to merge) unless they leave more places empty than small ones do
+    const long long n_big = sm_count / ctas, n_small = small_places / ctas;
+    const bool use_big = blocks > SMALL && n_big > 0 && n_big * ctas * small_places >= 0.85 * n_small * ctas * sm_count;
+    p.warps = use_big ? big : SMALL;
+    const long long want = std::max<long long>(1, use_big ? n_big : n_small);
+    p.splits = (int)std::min<long long>(want, std::max(1, (blocks + p.warps - 1) / p.warps));
     // More splits than a cluster has cost a second kernel, about as long as a warp takes for 6 blocks.
-    if (p.splits > MAX_CLUSTER && blocks <= 6 * WARPS * MAX_CLUSTER) p.splits = MAX_CLUSTER;
+    if (p.splits > MAX_CLUSTER && (p.splits <= 2 * MAX_CLUSTER && blocks <= 6 * p.warps * MAX_CLUSTER)) p.splits = MAX_CLUSTER;
     // A cluster lives in one of the 8 GPCs: what does not divide their places would wait for a second wave.
-    const int places = CTAS_PER_SM * sm_count / 8;
+    const int places = (use_big ? sm_count : (int)small_places) / 8;
     while (p.splits > 1 && p.splits <= MAX_CLUSTER && ctas > 8 * (places / p.splits)) p.splits--;
     return p;
 }
@@ -224,13 +231,13 @@ ZWG_DEV void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar
                  : "memory");
 }
 
-template <typename T, int D, int NT, int P>
+template <typename T, int D, int NT, int P, int WARPS>
 __global__ void __launch_bounds__(32 * WARPS)
     kv8_split_kernel(Kv8Attn p, int splits, int clustered, int vec, float scale) {
     chain_release();
     constexpr int R = 8 * NT, CH = D / 64, LDO = D + 4;
-    constexpr int BYTES = KV8_BLOCK * D, STAGES = RING / (WARPS * 2 * BYTES);
-    static_assert(WARPS * R * LDO * sizeof(float) <= RING, "the merge fits the ring");
+    constexpr int BYTES = KV8_BLOCK * D, STAGES = WARP_RING / (2 * BYTES);
+    static_assert(R * LDO * sizeof(float) <= WARP_RING, "the merge fits the ring");
     extern __shared__ __align__(128) unsigned char ring[];
     __shared__ uint64_t full[WARPS][STAGES];
     __shared__ float2 state[WARPS][R], merged[R];
@@ -609,16 +616,15 @@ bool wide(const Rows& r, size_t elem, size_t bytes) {
     return ((uintptr_t)r.data | (r.bs * elem) | (r.ts * elem)) % bytes == 0;
 }
 
-template <typename T, int D, int NT, int P>
+template <typename T, int D, int NT, int P, int WARPS>
 int split_launch(const Kv8Attn& p, const Plan& plan, cudaStream_t st) {
+    constexpr int RING = WARPS * WARP_RING;
     const float scale = (float)(1.0 / sqrt((double)D)) * kLog2e;
     const int rows = p.s.n * (p.n_head / p.c.n_head_kv);
     const unsigned segs = (unsigned)(p.s.n_batch * p.c.n_head_kv);
     const int clustered = plan.splits <= MAX_CLUSTER;
-    const auto kern = kv8_split_kernel<T, D, NT, P>;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)RING) != cudaSuccess ||
-        cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
-        return -1;
+    const auto kern = kv8_split_kernel<T, D, NT, P, WARPS>;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, RING) != cudaSuccess) return -1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(plan.tiles * plan.splits), segs);
     cfg.blockDim = dim3(32 * WARPS);
@@ -640,13 +646,19 @@ int split_launch(const Kv8Attn& p, const Plan& plan, cudaStream_t st) {
     return e == cudaSuccess ? 0 : -1;
 }
 
+template <typename T, int D, int NT, int P>
+int split_of(const Kv8Attn& p, const Plan& plan, cudaStream_t st) {
+    return plan.warps == SMALL ? split_launch<T, D, NT, P, SMALL>(p, plan, st)
+                               : split_launch<T, D, NT, P, big_warps(8 * NT)>(p, plan, st);
+}
+
 template <typename T, int D>
 int attn(const Kv8Attn& p, int pieces, int sm_count, cudaStream_t st) {
     const Plan plan = plan_for(p.c, p.s, p.n_head, sm_count);
-    const bool small = p.s.n * (p.n_head / p.c.n_head_kv) <= 8;
-    if constexpr (sizeof(T) == 4)
-        if (pieces == 2) return small ? split_launch<T, D, 1, 2>(p, plan, st) : split_launch<T, D, 2, 2>(p, plan, st);
-    return small ? split_launch<T, D, 1, 1>(p, plan, st) : split_launch<T, D, 2, 1>(p, plan, st);
+    const bool one = p.s.n * (p.n_head / p.c.n_head_kv) <= 8;
+    if constexpr (sizeof(T) == 4)  // bf16 queries are exact in one piece
+        if (pieces == 2) return one ? split_of<T, D, 1, 2>(p, plan, st) : split_of<T, D, 2, 2>(p, plan, st);
+    return one ? split_of<T, D, 1, 1>(p, plan, st) : split_of<T, D, 2, 1>(p, plan, st);
 }
 
 }  // namespace
