@@ -289,7 +289,7 @@ struct LogitRules {
     size_t allow_stride;
 };
 int logit_rules_launch(float* logits, size_t m, int n_vocab, size_t stride, const LogitRules& r, int32_t* out,
-                       size_t out_stride, int* err, cudaStream_t st);
+                       size_t out_stride, int sm_count, int* err, cudaStream_t st);
 
 // Elementwise helpers (misc.cu).
 int f32_to_bf16_launch(const float* x, uint16_t* y, size_t n, cudaStream_t st);

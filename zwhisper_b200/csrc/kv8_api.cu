@@ -160,7 +160,7 @@ extern "C" {
 
 int zwg_rope(const zwg_seqs* s, const zwg_rope_tables* t, int type, size_t d, size_t n_head, const zwg_rows* q,
              const zwg_rows* q_out, size_t n_head_kv, const zwg_rows* k, const zwg_rows* k_out, void* stream) {
-    if (d == 0 || d > 1024 || n_head == 0 || n_head >= kMost / d || n_head_kv >= kMost / d) return fail("rope: bad head sizes");
+    if (d == 0 || d > 1024 || n_head == 0 || n_head >= kMost / d || n_head_kv >= kMost / d || n_head + n_head_kv > 65536) return fail("rope: bad head sizes");
     int rc = check_type(type, "rope");
     if (!rc) rc = check_tables(t, d, "rope");
     if (!rc) rc = check_seqs(s, t->n_ctx, "rope");
@@ -173,6 +173,7 @@ int zwg_rope(const zwg_seqs* s, const zwg_rope_tables* t, int type, size_t d, si
     if (!rc && k) rc = check_rows(k_out, s, n_head_kv * d, type, true, "rope", "k_out");
     if (rc) return rc;
     if (!k && k_out) return fail("rope: k_out without k");
+    if (s->n * (n_head + (k ? n_head_kv : 0)) >= kMost / d) return fail("rope: too many elements in a sequence");
     Ctx* c = cur();
     if (!c) return ZWG_ERROR;
     const OnDevice on(c->device);
@@ -286,6 +287,8 @@ int zwg_llm_logits(float* logits, size_t m, size_t n_vocab, size_t stride, const
     if (stride < n_vocab && m > 1) return fail("llm_logits: row stride %zu below the vocabulary's %zu", stride, n_vocab);
     if (r->n_recent && !r->recent) return fail("llm_logits: null recent tokens");
     if (r->n_recent >= kMost) return fail("llm_logits: too many recent tokens");
+    if ((r->window < r->n_recent ? r->window : r->n_recent) >= (1u << 19))
+        return fail("llm_logits: a window of %zu tokens, at most 524287 are taken", r->window);
     if (r->n_bias > ZWG_MAX_BIAS) return fail("llm_logits: %zu biases, at most %d are taken", r->n_bias, ZWG_MAX_BIAS);
     if (r->n_bias && (!r->bias_ids || !r->bias)) return fail("llm_logits: null biases");
     if (!(r->repeat > 0.f) || !std::isfinite(r->repeat) || !std::isfinite(r->presence) || !std::isfinite(r->frequency))
@@ -301,7 +304,7 @@ int zwg_llm_logits(float* logits, size_t m, size_t n_vocab, size_t stride, const
     zwg::LogitRules p{r->recent, r->recent_stride, window ? (int)r->n_recent : 0, window ? r->n_recents : nullptr,
                       (int)window, r->repeat, r->presence, r->frequency, r->bias_ids, r->bias,
                       (int)r->n_bias, r->bias_stride, r->allow, r->allow_stride};
-    if (zwg::logit_rules_launch(logits, m, (int)n_vocab, stride, p, out, out_stride, c->err, (cudaStream_t)stream))
+    if (zwg::logit_rules_launch(logits, m, (int)n_vocab, stride, p, out, out_stride, c->sm_count, c->err, (cudaStream_t)stream))
         return cuda_fail("llm_logits launch", cudaGetLastError());
     return ZWG_OK;
 }
