@@ -273,6 +273,10 @@ size_t kv8_attn_workspace_bytes(const Kv8& c, const Seqs& s, int n_head, int sm_
 // pieces: f16 pieces of a query and a probability, 1 or 2.
 int kv8_attn_launch(const Kv8Attn& p, int type, int pieces, int sm_count, cudaStream_t st);
 
+// Its tcgen05 kernel for many query rows of a kv head (kv8_prefill.cu), `splits` cuts of the keys.
+constexpr int KV8_PREFILL_ROWS = 256, KV8_PREFILL_KEYS = 128;  // of a tile
+int kv8_prefill_launch(const Kv8Attn& p, int type, int pieces, int splits, cudaStream_t st);
+
 // Penalties, biases, mask and argmax on rows of logits (logits.cu).
 struct LogitRules {
     const int32_t* recent;

@@ -24,15 +24,15 @@
 #include "chain.cuh"
 #include "common.cuh"
 #include "kernels.h"
+#include "kv8_attn.cuh"
 #include "seqs.cuh"
 
 namespace zwg {
 namespace {
 
-constexpr int HALF = 256;  // threads for keys, and as many for values
+using namespace kv8;
 
-ZWG_DEV float up(float x) { return x; }
-ZWG_DEV float up(__nv_bfloat16 x) { return __bfloat162float(x); }
+constexpr int HALF = 256;  // threads for keys, and as many for values
 
 // rint(127 x / top) of four values whose f32 quotients come near a border (or overflow 127 / top).
 __device__ __noinline__ uint32_t exact4(float4 x, float top) {
@@ -57,17 +57,6 @@ ZWG_DEV uint32_t quantise4(float4 x, float inv, float top) {
     return __byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410);
 }
 
-// Four elements in a row, as f32.
-ZWG_DEV float4 four(const float* p, bool wide) {
-    return wide ? *reinterpret_cast<const float4*>(p) : make_float4(p[0], p[1], p[2], p[3]);
-}
-ZWG_DEV float4 four(const __nv_bfloat16* p, bool wide) {
-    if (!wide) return make_float4(up(p[0]), up(p[1]), up(p[2]), up(p[3]));
-    const uint2 w = *reinterpret_cast<const uint2*>(p);
-    return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16),
-                       __uint_as_float(w.y & 0xffff0000u));
-}
-
 // 4 x 4 bytes turned: byte i of word j becomes byte j of word i.
 ZWG_DEV void turn4x4(uint32_t (&w)[4]) {
     const uint32_t a = __byte_perm(w[0], w[1], 0x5140), b = __byte_perm(w[2], w[3], 0x5140);
@@ -82,16 +71,16 @@ ZWG_DEV void turn4x4(uint32_t (&w)[4]) {
 // column, so that a warp's columns meet in few banks.
 ZWG_DEV int turned(int column, int w) { return column * 8 + (w ^ ((column >> 2) & 7)); }
 
-// staged: keys are rotated or lie transposed.
-template <typename T, int D>
-__global__ void __launch_bounds__(2 * HALF, 2) kv8_append_kernel(Kv8Append p, int staged, int wide) {
+// STAGED: keys are rotated or lie transposed. WIDE: pieces of four elements are aligned.
+template <typename T, int D, bool STAGED, bool WIDE>
+__global__ void __launch_bounds__(2 * HALF, 2) kv8_append_kernel(Kv8Append p) {
     chain_release();
     const int z = chain_wait();
     constexpr int LD = D + 1;     // odd: neither rows nor columns of the staging meet in a bank
     constexpr int LANES = D / 4;  // threads to a row
     constexpr int GROUPS = HALF / LANES, ROWS = KV8_BLOCK / GROUPS;  // a thread's rows: GROUPS * i + its group
     static_assert(ROWS == 4 || ROWS == 2, "a thread's rows make whole or half words of a value column");
-    extern __shared__ float stage[];  // [32][LD] where staged
+    extern __shared__ float stage[];  // [32][LD] where STAGED
     __shared__ __align__(16) uint32_t columns[D * 8];
     __shared__ uint32_t top_of[2][HALF / 32];
     const int bh = blockIdx.y, b = bh / p.c.n_head_kv, h = bh - b * p.c.n_head_kv;
@@ -119,8 +108,15 @@ __global__ void __launch_bounds__(2 * HALF, 2) kv8_append_kernel(Kv8Append p, in
         float* scale = (is_k ? p.c.k_scale : p.c.v_scale) + at_blk + z;
         const bool from_open = opened == blk;
         const float old_scale = held && !from_open ? __ldcg(scale) : 0.f;
-        // rows of the block: [0, held) the cache's, [held, live) new, the others zero
+        // rows of the block: [0, held) the cache's, [held, live) new, the others zero. Every thread loads
+        // rows of the call for all of its own, the nearest ones for those that are not new.
         float4 x[ROWS];
+        Four<T> fresh[ROWS];
+        if (!(STAGED && is_k)) {
+#pragma unroll
+            for (int i = 0; i < ROWS; i++)
+                fresh[i] = load_four(src + (size_t)min(max(lo + row0 + i - at.past, 0), at.count - 1) * ts + c, WIDE);
+        }
 #pragma unroll
         for (int i = 0; i < ROWS; i++) {
             const int r = row0 + i;
@@ -133,11 +129,14 @@ __global__ void __launch_bounds__(2 * HALF, 2) kv8_append_kernel(Kv8Append p, in
                     const int e = is_k ? 1 : KV8_BLOCK;
                     x[i] = make_float4(q[0] * old_scale, q[e] * old_scale, q[2 * e] * old_scale, q[3 * e] * old_scale);
                 }
-            } else if (r < live && !(staged && is_k)) {
-                x[i] = four(src + (size_t)(lo + r - at.past) * ts + c, wide);
             }
         }
-        if (staged) {  // new keys, to where each thread's are, by way of shared memory
+        if (!(STAGED && is_k)) {
+#pragma unroll
+            for (int i = 0; i < ROWS; i++)
+                if (row0 + i >= held && row0 + i < live) x[i] = value_of(fresh[i]);
+        }
+        if constexpr (STAGED) {  // new keys, to where each thread's are, by way of shared memory
             const int n = live - held;
             if (is_k && p.k_es == 1) {
                 for (int e = tid; e < n * D; e += HALF) {
@@ -274,18 +273,18 @@ int touched(int n) { return (n + 2 * (KV8_BLOCK - 1)) / KV8_BLOCK; }
 
 template <typename T, int D>
 int append(const Kv8Append& p, cudaStream_t st) {
-    const int staged = p.rope.cos || p.k_es != 1;
+    const bool staged = p.rope.cos || p.k_es != 1;
     const size_t smem = staged ? KV8_BLOCK * (D + 1) * sizeof(float) : 0;
     // rows whose pieces of four elements are aligned
     const auto whole = [](const Rows& r, size_t hs) {
         return ((uintptr_t)r.data | (r.bs * sizeof(T)) | (r.ts * sizeof(T)) | (hs * sizeof(T))) % (4 * sizeof(T)) == 0;
     };
-    const int wide = (staged || whole(p.k, p.k_hs)) && whole(p.v, p.v_hs);
+    const bool wide = (staged || whole(p.k, p.k_hs)) && whole(p.v, p.v_hs);
     // CTA 0 takes the first and the last block
     const dim3 grid((unsigned)std::max(1, touched(p.s.n) - 1), (unsigned)(p.s.n_batch * p.c.n_head_kv));
-    return launch_chained_smem(kv8_append_kernel<T, D>, grid, dim3(2 * HALF), smem, st, p, staged, wide) == cudaSuccess
-               ? 0
-               : -1;
+    void (*kern)(Kv8Append) = staged ? (wide ? kv8_append_kernel<T, D, true, true> : kv8_append_kernel<T, D, true, false>)
+                                     : (wide ? kv8_append_kernel<T, D, false, true> : kv8_append_kernel<T, D, false, false>);
+    return launch_chained_smem(kern, grid, dim3(2 * HALF), smem, st, p) == cudaSuccess ? 0 : -1;
 }
 
 }  // namespace

@@ -19,9 +19,6 @@
 // merge, and loads run ahead of the arithmetic.
 // The splits of a (sequence, kv head, tile of query rows) that fit a cluster (8 CTAs) meet in each
 // other's shared memory; more of them write partials (m, l, O) for kv8_combine_kernel.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
 #include <algorithm>
 
 #include <cooperative_groups.h>
@@ -29,6 +26,7 @@
 #include "chain.cuh"
 #include "common.cuh"
 #include "kernels.h"
+#include "kv8_attn.cuh"
 #include "seqs.cuh"
 #include "sm100.cuh"
 
@@ -36,20 +34,9 @@ namespace zwg {
 namespace {
 
 namespace cg = cooperative_groups;
+using namespace kv8;
 
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kUnit = 32768.f;  // P's f16 pieces hold 2^15 p: small probabilities stay normal
-
-ZWG_DEV uint32_t h2u(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
-
-// Four int8 of a word -> two f16 pairs, exactly: 0x6400 | (x + 128) is 1024 + 128 + x.
-ZWG_DEV void ints_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
-    const uint32_t u = w ^ 0x80808080u;
-    const __half2 off = __half2(__half_raw{0x6480}, __half_raw{0x6480});
-    uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
-    lo = h2u(__hsub2(*reinterpret_cast<__half2*>(&a), off));
-    hi = h2u(__hsub2(*reinterpret_cast<__half2*>(&b), off));
-}
 
 ZWG_DEV void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
@@ -64,37 +51,19 @@ ZWG_DEV uint32_t transpose8x8(uint32_t x) {
     return y;
 }
 
-// x as f16 pieces: the nearest f16 and, with two, the nearest f16 of what is left.
-template <int P>
-ZWG_DEV void pieces_of(float x, float y, uint32_t (&w)[P]) {
-    const __half2 h = __floats2half2_rn(x, y);
-    w[0] = h2u(h);
-    if (P == 2) {
-        const float2 f = __half22float2(h);
-        w[P - 1] = h2u(__floats2half2_rn(x - f.x, y - f.y));
-    }
-}
-
-// The power of two of |x|'s exponent and its inverse; 1 for zero, tiny, infinite and NaN.
-ZWG_DEV void power_of(float x, float& p, float& inv) {
-    const uint32_t e = __float_as_uint(x) & 0x7f800000u;
-    const bool fine = e > 0x01000000u && e < 0x7e000000u;
-    p = fine ? __uint_as_float(e) : 1.f;
-    inv = fine ? __uint_as_float(0x7f000000u - e) : 1.f;
-}
-
 struct Plan {
     int tiles;   // tiles of query rows of a (sequence, kv head)
-    int warps;   // of a CTA
+    int warps;   // of a CTA; 0: the tcgen05 kernel's
     int splits;  // cuts of the keys
 };
 
 constexpr int SMALL = 4;            // warps of a small CTA, three of which share an SM
 constexpr int MAX_CLUSTER = 8;
+constexpr int MOST_SPLIT_ROWS = 32;  // query rows of a kv head above which the tcgen05 kernel runs
 constexpr int WARP_RING = 16 * 1024;  // bytes a warp has for blocks on their way
 
-// Rows of a tile: one or two 8-wide N tiles.
-int tile_rows(int rows) { return rows <= 8 ? 8 : 16; }
+// Rows of a tile: one or two 8-wide N tiles, or the tcgen05 kernel's.
+int tile_rows(int rows) { return rows <= 8 ? 8 : rows <= MOST_SPLIT_ROWS ? 16 : KV8_PREFILL_ROWS; }
 // Warps of a CTA that has an SM to itself; the registers of two N tiles leave room for 8.
 constexpr int big_warps(int tile_rows) { return tile_rows == 8 ? 12 : 8; }
 
@@ -104,6 +73,13 @@ Plan plan_for(const Kv8& c, const Seqs& s, int n_head, int sm_count) {
     p.tiles = (rows + tile_rows(rows) - 1) / tile_rows(rows);
     const long long ctas = (long long)s.n_batch * c.n_head_kv * p.tiles;
     const int blocks = (s.n_past + s.n + KV8_BLOCK - 1) / KV8_BLOCK;
+    if (rows > MOST_SPLIT_ROWS) {
+        // keys are cut while SMs stay empty, two tiles of keys to a cut at least
+        const int key_tiles = (blocks * KV8_BLOCK + KV8_PREFILL_KEYS - 1) / KV8_PREFILL_KEYS;
+        p.warps = 0;
+        p.splits = (int)std::min<long long>(std::max<long long>(1, sm_count / ctas), std::max(1, key_tiles / 2));
+        return p;
+    }
     const int per_sm = big / SMALL;
     const long long small_places = (long long)per_sm * sm_count;
     // One wave, of big CTAs (fewer states to merge) unless they leave more places empty than small ones do
@@ -142,61 +118,6 @@ ZWG_DEV void add4(float4& a, float f, float4 x) {
     a.y += f * x.y;
     a.z += f * x.z;
     a.w += f * x.w;
-}
-
-// Four output elements of a row whose weights sum to l (0: no key was seen).
-ZWG_DEV void store4(float* out, float4 o, float inv, bool vec) {
-    const float4 y = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-    if (vec) {
-        *reinterpret_cast<float4*>(out) = y;
-    } else {
-        out[0] = y.x;
-        out[1] = y.y;
-        out[2] = y.z;
-        out[3] = y.w;
-    }
-}
-ZWG_DEV void store4(__nv_bfloat16* out, float4 o, float inv, bool vec) {
-    __nv_bfloat162 y[2] = {__floats2bfloat162_rn(o.x * inv, o.y * inv), __floats2bfloat162_rn(o.z * inv, o.w * inv)};
-    if (vec) {
-        *reinterpret_cast<uint2*>(out) = *reinterpret_cast<uint2*>(y);
-    } else {
-        out[0] = y[0].x;
-        out[1] = y[0].y;
-        out[2] = y[1].x;
-        out[3] = y[1].y;
-    }
-}
-
-// 16 consecutive elements as f32.
-ZWG_DEV void load16(const float* q, float (&x)[16], bool vec) {
-    if (vec) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float4 v = reinterpret_cast<const float4*>(q)[i];
-            x[i * 4] = v.x, x[i * 4 + 1] = v.y, x[i * 4 + 2] = v.z, x[i * 4 + 3] = v.w;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 16; i++) x[i] = q[i];
-    }
-}
-ZWG_DEV void load16(const __nv_bfloat16* q, float (&x)[16], bool vec) {
-    if (vec) {
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const uint4 v = reinterpret_cast<const uint4*>(q)[i];
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                x[i * 8 + j * 2] = __uint_as_float(w[j] << 16);
-                x[i * 8 + j * 2 + 1] = __uint_as_float(w[j] & 0xffff0000u);
-            }
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 16; i++) x[i] = __bfloat162float(q[i]);
-    }
 }
 
 // The blocks [from, to) of a split: the tile's keys first .. past + (the last row's query).
@@ -611,16 +532,10 @@ __global__ void __launch_bounds__(256) kv8_combine_kernel(Kv8Attn p, int splits,
     store4(out, acc, sum == 0.f ? 0.f : 1.f / sum, vec & 2);
 }
 
-// Rows whose elements can be read or written 16 bytes (of f32; 8 of bf16) at a time.
-bool wide(const Rows& r, size_t elem, size_t bytes) {
-    return ((uintptr_t)r.data | (r.bs * elem) | (r.ts * elem)) % bytes == 0;
-}
-
 template <typename T, int D, int NT, int P, int WARPS>
-int split_launch(const Kv8Attn& p, const Plan& plan, cudaStream_t st) {
+int split_launch(const Kv8Attn& p, const Plan& plan, int vec, cudaStream_t st) {
     constexpr int RING = WARPS * WARP_RING;
     const float scale = (float)(1.0 / sqrt((double)D)) * kLog2e;
-    const int rows = p.s.n * (p.n_head / p.c.n_head_kv);
     const unsigned segs = (unsigned)(p.s.n_batch * p.c.n_head_kv);
     const int clustered = plan.splits <= MAX_CLUSTER;
     const auto kern = kv8_split_kernel<T, D, NT, P, WARPS>;
@@ -638,27 +553,39 @@ int split_launch(const Kv8Attn& p, const Plan& plan, cudaStream_t st) {
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    const int vec = (wide(p.q, sizeof(T), 16) ? 1 : 0) | (wide(p.out, sizeof(T), 4 * sizeof(T)) ? 2 : 0);
-    cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p, plan.splits, clustered, vec, scale);
-    if (e == cudaSuccess && !clustered)
-        e = launch_chained_smem(kv8_combine_kernel<T, D>, dim3((unsigned)rows, segs), dim3(256),
-                                plan.splits * sizeof(float), st, p, plan.splits, 8 * NT, vec);
-    return e == cudaSuccess ? 0 : -1;
+    return cudaLaunchKernelEx(&cfg, kern, p, plan.splits, clustered, vec, scale) == cudaSuccess ? 0 : -1;
 }
 
 template <typename T, int D, int NT, int P>
-int split_of(const Kv8Attn& p, const Plan& plan, cudaStream_t st) {
-    return plan.warps == SMALL ? split_launch<T, D, NT, P, SMALL>(p, plan, st)
-                               : split_launch<T, D, NT, P, big_warps(8 * NT)>(p, plan, st);
+int split_of(const Kv8Attn& p, const Plan& plan, int vec, cudaStream_t st) {
+    return plan.warps == SMALL ? split_launch<T, D, NT, P, SMALL>(p, plan, vec, st)
+                               : split_launch<T, D, NT, P, big_warps(8 * NT)>(p, plan, vec, st);
+}
+
+template <typename T, int D>
+int combine(const Kv8Attn& p, const Plan& plan, int rows, int tile_rows, int vec, cudaStream_t st) {
+    return launch_chained_smem(kv8_combine_kernel<T, D>, dim3((unsigned)rows, (unsigned)(p.s.n_batch * p.c.n_head_kv)), dim3(256),
+                               plan.splits * sizeof(float), st, p, plan.splits, tile_rows, vec) == cudaSuccess
+               ? 0
+               : -1;
 }
 
 template <typename T, int D>
 int attn(const Kv8Attn& p, int pieces, int sm_count, cudaStream_t st) {
     const Plan plan = plan_for(p.c, p.s, p.n_head, sm_count);
-    const bool one = p.s.n * (p.n_head / p.c.n_head_kv) <= 8;
-    if constexpr (sizeof(T) == 4)  // bf16 queries are exact in one piece
-        if (pieces == 2) return one ? split_of<T, D, 1, 2>(p, plan, st) : split_of<T, D, 2, 2>(p, plan, st);
-    return one ? split_of<T, D, 1, 1>(p, plan, st) : split_of<T, D, 2, 1>(p, plan, st);
+    const int rows = p.s.n * (p.n_head / p.c.n_head_kv), per_tile = tile_rows(rows);
+    const bool one = per_tile == 8, two_pieces = sizeof(T) == 4 && pieces == 2;  // bf16 queries are exact in one piece
+    const int vec = (wide(p.q, sizeof(T), 16) ? 1 : 0) | (wide(p.out, sizeof(T), 4 * sizeof(T)) ? 2 : 0);
+    int rc;
+    if (plan.warps == 0) {
+        rc = kv8_prefill_launch(p, sizeof(T) == 2 ? TYPE_BF16 : TYPE_F32, pieces, plan.splits, st);
+    } else if (two_pieces) {
+        if constexpr (sizeof(T) == 4) rc = one ? split_of<T, D, 1, 2>(p, plan, vec, st) : split_of<T, D, 2, 2>(p, plan, vec, st);
+    } else {
+        rc = one ? split_of<T, D, 1, 1>(p, plan, vec, st) : split_of<T, D, 2, 1>(p, plan, vec, st);
+    }
+    if (rc == 0 && plan.splits > (plan.warps ? MAX_CLUSTER : 1)) rc = combine<T, D>(p, plan, rows, per_tile, vec, st);
+    return rc;
 }
 
 }  // namespace
@@ -667,7 +594,7 @@ size_t kv8_attn_workspace_bytes(const Kv8& c, const Seqs& s, int n_head, int sm_
     if (s.n_batch == 0 || s.n == 0) return 0;
     const Plan p = plan_for(c, s, n_head, sm_count);
     const int rows = s.n * (n_head / c.n_head_kv);
-    return p.splits <= MAX_CLUSTER ? 0
+    return p.splits <= (p.warps ? MAX_CLUSTER : 1) ? 0
                          : (size_t)s.n_batch * c.n_head_kv * p.tiles * p.splits * tile_rows(rows) * (c.d + 4) * sizeof(float);
 }
 
