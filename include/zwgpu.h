@@ -671,9 +671,9 @@ ZWG_API int zwg_kv8_attn(const zwg_kv8* c, const zwg_seqs* s, int type, size_t n
                          const zwg_rows* out, void* workspace, size_t workspace_bytes, void* stream);
 
 /* The rules on a step's logits. For each row, in this order and in f32:
- *   1. a token that is c > 0 times among the row's last `window` (at most 524287) recent tokens: x / repeat
- *      (x > 0) or x * repeat (otherwise), once however often it is there (zwg_llm_greedy
- *      repeats it); then x - (c * frequency + presence);
+ *   1. a token that is c > 0 times among the row's last `window` (at most 524287) recent tokens:
+ *      x * (1 / repeat) (x > 0) or x * repeat (otherwise), once however often it is there
+ *      (zwg_llm_greedy repeats it); then x - (c * frequency + presence);
  *   2. x + bias[j] for each j with bias_ids[j] = the token, their sum taken in the order of j;
  *   3. -inf where the token's bit in `allow` is 0 (token t: bit t % 32 of word t / 32).
  * recent: device int32, row r at recent + r * recent_stride, its tokens 0 .. n_recent, or

@@ -122,7 +122,7 @@ def logits(x, recent, window, repeat, presence, frequency, bias_ids, bias, allow
     ids, times = np.unique(np.asarray(recent[max(0, len(recent) - window):], np.int64), return_counts=True)
     for t, c in zip(ids, times):
         if 0 <= t < len(x):
-            y = x[t] / f(repeat) if x[t] > 0 else x[t] * f(repeat)
+            y = x[t] * (f(1) / f(repeat)) if x[t] > 0 else x[t] * f(repeat)
             x[t] = y - (f(c) * f(frequency) + f(presence))
     add = np.zeros_like(x)
     for t, a in zip(bias_ids, bias):

@@ -292,6 +292,11 @@ def load():
         return lib
 
 
+def loaded():
+    """The library that load() has loaded (by way of ensure_init, for one)."""
+    return _lib
+
+
 def last_error() -> str:
     lib = load()
     buf = ctypes.create_string_buffer(512)
@@ -309,7 +314,6 @@ _bound = threading.local()
 
 def ensure_init(device: int) -> None:
     """Bind the calling thread to `device` (zwg_init), once per thread and device."""
-    lib = load()
-    if getattr(_bound, "device", None) != device:
-        check(lib.zwg_init(device))
+    if getattr(_bound, "device", None) != device or _lib is None:
+        check(load().zwg_init(device))
         _bound.device = device

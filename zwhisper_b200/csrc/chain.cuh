@@ -15,6 +15,9 @@
 // non-coherent read-only path (__ldg) is kept for constants such as the weights.
 #pragma once
 #include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <atomic>
 
 namespace zwg {
 
@@ -23,6 +26,19 @@ __device__ __forceinline__ int chain_wait() {
     int z;
     asm volatile("griddepcontrol.wait;\n\tmov.u32 %0, 0;" : "=r"(z) : : "memory");
     return z;
+}
+
+// Let a kernel have `bytes` of dynamic shared memory (and clusters of more than 8 CTAs), once for each
+// device: `done` is the kernel's own mask of devices.
+inline cudaError_t allow_smem(std::atomic<uint64_t>& done, const void* kern, int bytes, bool large_clusters = false) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    const uint64_t bit = 1ull << (dev & 63);
+    if (e != cudaSuccess || (done.load(std::memory_order_relaxed) & bit)) return e;
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && large_clusters) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
 }
 
 template <typename... KArgs, typename... Args>

@@ -284,7 +284,7 @@ struct LogitRules {
     int n_recent;
     const int32_t* n_recents;
     int window;
-    float repeat, presence, frequency;
+    float repeat, inv_repeat, presence, frequency;  // inv_repeat: 1 / repeat
     const int32_t* bias_ids;
     const float* bias;
     int n_bias;

@@ -291,7 +291,7 @@ int zwg_llm_logits(float* logits, size_t m, size_t n_vocab, size_t stride, const
         return fail("llm_logits: a window of %zu tokens, at most 524287 are taken", r->window);
     if (r->n_bias > ZWG_MAX_BIAS) return fail("llm_logits: %zu biases, at most %d are taken", r->n_bias, ZWG_MAX_BIAS);
     if (r->n_bias && (!r->bias_ids || !r->bias)) return fail("llm_logits: null biases");
-    if (!(r->repeat > 0.f) || !std::isfinite(r->repeat) || !std::isfinite(r->presence) || !std::isfinite(r->frequency))
+    if (!(r->repeat > 0.f) || !std::isfinite(r->repeat) || !std::isfinite(1.f / r->repeat) || !std::isfinite(r->presence) || !std::isfinite(r->frequency))
         return fail("llm_logits: repeat must be positive, all penalties finite");
     if (out && out_stride == 0 && m > 1) return fail("llm_logits: out needs a stride");
     if (!al(logits, 4) || !al(out, 4) || !al(r->recent, 4) || !al(r->n_recents, 4) || !al(r->bias_ids, 4) ||
@@ -302,7 +302,7 @@ int zwg_llm_logits(float* logits, size_t m, size_t n_vocab, size_t stride, const
     const OnDevice on(c->device);
     const size_t window = r->window < r->n_recent ? r->window : r->n_recent;
     zwg::LogitRules p{r->recent, r->recent_stride, window ? (int)r->n_recent : 0, window ? r->n_recents : nullptr,
-                      (int)window, r->repeat, r->presence, r->frequency, r->bias_ids, r->bias,
+                      (int)window, r->repeat, 1.f / r->repeat, r->presence, r->frequency, r->bias_ids, r->bias,
                       (int)r->n_bias, r->bias_stride, r->allow, r->allow_stride};
     if (zwg::logit_rules_launch(logits, m, (int)n_vocab, stride, p, out, out_stride, c->sm_count, c->err, (cudaStream_t)stream))
         return cuda_fail("llm_logits launch", cudaGetLastError());

@@ -140,18 +140,6 @@ ZWG_DEV Range range_of(Place at, int first, int group, int tile, int split, int 
     return r;
 }
 
-ZWG_DEV void bulk_hint(const void* src, uint32_t bytes) {
-    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(bytes) : "memory");
-}
-
-// A bulk copy into a stage of a warp's ring.
-ZWG_DEV void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                     sm100::smem_u32(dst)),
-                 "l"(src), "r"(bytes), "r"(sm100::smem_u32(bar))
-                 : "memory");
-}
-
 template <typename T, int D, int NT, int P, int WARPS>
 __global__ void __launch_bounds__(32 * WARPS)
     kv8_split_kernel(Kv8Attn p, int splits, int clustered, int vec, float scale) {
@@ -181,8 +169,8 @@ __global__ void __launch_bounds__(32 * WARPS)
         for (int s = 0; s < STAGES; s++) {
             const int blk = r.from + warp + s * WARPS;
             if (blk < r.to && blk < p.c.blocks) {
-                bulk_hint(p.c.k + (head + blk) * BYTES, BYTES);
-                bulk_hint(p.c.v + (head + blk) * BYTES, BYTES);
+                sm100::bulk_hint(p.c.k + (head + blk) * BYTES, BYTES);
+                sm100::bulk_hint(p.c.v + (head + blk) * BYTES, BYTES);
             }
         }
     }
@@ -200,8 +188,8 @@ __global__ void __launch_bounds__(32 * WARPS)
     unsigned char* mine = ring + warp * (STAGES * 2 * BYTES);
     const auto load = [&](int blk, int stage) {
         sm100::mbar_arrive_expect_tx(&full[warp][stage], 2 * BYTES);
-        bulk_load(mine + stage * 2 * BYTES, p.c.k + (head + blk) * BYTES + z, BYTES, &full[warp][stage]);
-        bulk_load(mine + stage * 2 * BYTES + BYTES, p.c.v + (head + blk) * BYTES + z, BYTES, &full[warp][stage]);
+        sm100::bulk_load(mine + stage * 2 * BYTES, p.c.k + (head + blk) * BYTES + z, BYTES, &full[warp][stage]);
+        sm100::bulk_load(mine + stage * 2 * BYTES + BYTES, p.c.v + (head + blk) * BYTES + z, BYTES, &full[warp][stage]);
     };
     if (lane == 0)
         for (int s = 0; s < STAGES; s++)
@@ -539,7 +527,8 @@ int split_launch(const Kv8Attn& p, const Plan& plan, int vec, cudaStream_t st) {
     const unsigned segs = (unsigned)(p.s.n_batch * p.c.n_head_kv);
     const int clustered = plan.splits <= MAX_CLUSTER;
     const auto kern = kv8_split_kernel<T, D, NT, P, WARPS>;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, RING) != cudaSuccess) return -1;
+    static std::atomic<uint64_t> done{0};
+    if (allow_smem(done, (const void*)kern, RING) != cudaSuccess) return -1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(plan.tiles * plan.splits), segs);
     cfg.blockDim = dim3(32 * WARPS);

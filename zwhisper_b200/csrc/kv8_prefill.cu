@@ -159,6 +159,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(Kv8Attn p, int 
             constexpr uint32_t idesc_s = idesc_f16(BM, BN, false, false, false);
             constexpr uint32_t idesc_o = idesc_f16(BM, D, false, false, false);
             bool ok = mbar_wait(&sm.q_full[t], 0, err);
+            // tile 1 starts a softmax behind tile 0, so that the one's exponentials run during the other's products
+            if (t == 1) ok = ok && mbar_wait(&sm.p_full[0], 0, err);
             for (int j = 0; ok && j < n_tiles; j++) {
                 const int ks = j % S::KS, vs = j % S::VS;
                 if (!(ok = mbar_wait(&sm.k_full[ks], j / S::KS & 1, err))) break;
@@ -477,7 +479,8 @@ int launch(const Kv8Attn& p, int splits, cudaStream_t st) {
     const auto kern = kv8_prefill_kernel<T, D, P>;
     constexpr int smem = sizeof(Smem<D, P>);
     static_assert(smem <= 227 * 1024, "shared memory of a CTA");
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -1;
+    static std::atomic<uint64_t> done{0};
+    if (allow_smem(done, (const void*)kern, smem) != cudaSuccess) return -1;
     const int rows = p.s.n * (p.n_head / p.c.n_head_kv), tiles = (rows + KV8_PREFILL_ROWS - 1) / KV8_PREFILL_ROWS;
     const float scale = (float)(1.0 / sqrt((double)D)) * kLog2e;
     const int vec = (wide(p.q, sizeof(T), 16) ? 1 : 0) | (wide(p.out, sizeof(T), 4 * sizeof(T)) ? 2 : 0);

@@ -78,6 +78,19 @@ ZWG_DEV bool mbar_wait_drain(uint64_t* bar, uint32_t parity) {
 
 // ---- TMA ---------------------------------------------------------------------------------
 
+// Untiled copy of `bytes` (a multiple of 16, both addresses 16-byte aligned) from global into this CTA's
+// shared memory, counted on an mbarrier.
+ZWG_DEV void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+                 "l"(src), "r"(bytes), "r"(smem_u32(bar))
+                 : "memory");
+}
+
+// A hint that `bytes` (a multiple of 16, from a 16-byte boundary) of global memory go to L2.
+ZWG_DEV void bulk_hint(const void* src, uint32_t bytes) {
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(bytes) : "memory");
+}
+
 ZWG_DEV void tma_load_3d(const CUtensorMap* map, uint64_t* bar, void* dst, int c0, int c1, int c2) {
     asm volatile(
         "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
@@ -314,6 +327,15 @@ ZWG_DEV void tmem_st128(uint32_t taddr, const uint32_t (&r)[128]) {
 }
 
 ZWG_DEV void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// The same wait, named on the registers of a load: no use of them can come before it, also where other
+// work stands between a load and its wait.
+ZWG_DEV void tmem_ld_wait16(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
+}
 ZWG_DEV void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Register reallocation between warpgroups (all four warps of a warpgroup execute it).

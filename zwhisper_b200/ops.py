@@ -186,9 +186,15 @@ def attention_scratch(n_q, n_kv, n_head, n_state) -> int:
 
 # ---- device (torch) entry points -----------------------------------------------------------
 
+_torch_module = None
+
+
 def _torch():
-    import torch
-    return torch
+    global _torch_module
+    if _torch_module is None:
+        import torch
+        _torch_module = torch
+    return _torch_module
 
 
 def _dev_ptr(t, dtype, name):
@@ -854,6 +860,16 @@ def _rows(t, dtype, device, shape, name: str):
     return ctypes.byref(_lib.RowsC(t.data_ptr(), sb, st))
 
 
+def _new_rows(like, shape):
+    """A new tensor like `like` (rows that have passed _rows), and a reference to its zwg_rows."""
+    t = _torch().empty_like(like)
+    sb, st, sh, sd = t.stride()
+    if (sd != 1 and shape[3] > 1) or (sh != shape[3] and shape[2] > 1):  # dense in another order
+        t = like.new_empty(shape)
+        sb, st, _, _ = t.stride()
+    return t, ctypes.byref(_lib.RowsC(t.data_ptr(), sb, st))
+
+
 def _int32_of(t, device, shape, name):
     torch = _torch()
     if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or t.device != device or t.shape != shape:
@@ -884,6 +900,12 @@ def _stream_on(device):
     return _torch()._C._cuda_getCurrentRawStream(device.index)
 
 
+def _ready(device):
+    """The library, with the calling thread bound to the device."""
+    _lib.ensure_init(device.index)
+    return _lib.loaded()
+
+
 def _tables(cos, sin, device, interleaved: bool):
     torch = _torch()
     if cos.dim() != 2 or sin.shape != cos.shape or cos.device != device or sin.device != device:
@@ -910,26 +932,24 @@ def rope(q, cos, sin, n_past=0, k=None, interleaved: bool = False, count=None, i
         raise ValueError("k_out without k")
     B, n, H, d = shape = q.shape
     dtype, dev = q.dtype, q.device
-    fresh = torch.contiguous_format
+    qr = _rows(q, dtype, dev, shape, "q")
     qo = ko = kr = None  # in place
-    if q_out is None and not inplace:
-        q_out = torch.empty_like(q, memory_format=fresh)
     if q_out is not None:
         qo = _rows(q_out, dtype, dev, shape, "q_out")
+    elif not inplace:
+        q_out, qo = _new_rows(q, shape)
     heads_kv = 0
     if k is not None:
         heads_kv = k.shape[2]
         kv_shape = (B, n, heads_kv, d)
         kr = _rows(k, dtype, dev, kv_shape, "k")
-        if k_out is None and not inplace:
-            k_out = torch.empty_like(k, memory_format=fresh)
         if k_out is not None:
             ko = _rows(k_out, dtype, dev, kv_shape, "k_out")
+        elif not inplace:
+            k_out, ko = _new_rows(k, kv_shape)
     tables = _tables(cos, sin, dev, interleaved)
     sq = _seqs(B, n, n_past, count, None, cos.shape[0], dev)
-    _lib.ensure_init(dev.index)
-    _lib.check(_lib.load().zwg_rope(sq, tables, kind, d, H, _rows(q, dtype, dev, shape, "q"), qo, heads_kv, kr, ko,
-                                    _stream_on(dev)))
+    _lib.check(_ready(dev).zwg_rope(sq, tables, kind, d, H, qr, qo, heads_kv, kr, ko, _stream_on(dev)))
     q = q if q_out is None else q_out
     return q if k is None else (q, k if k_out is None else k_out)
 
@@ -988,29 +1008,26 @@ class Kv8Cache:
         t = None if rope is None else _tables(rope[0], rope[1], dev, len(rope) > 2 and rope[2])
         kr, vr = _rows(k, dtype, dev, shape, "k"), _rows(v, dtype, dev, shape, "v")
         s = self._call(n, n_past, count, None, None)
-        _lib.ensure_init(dev.index)
-        _lib.check(_lib.load().zwg_kv8_append(self._ref, s, kind, kr, vr, t, _stream_on(dev)))
+        _lib.check(_ready(dev).zwg_kv8_append(self._ref, s, kind, kr, vr, t, _stream_on(dev)))
 
     def read(self, n: int, n_past, count=None, k=None, v=None):
         """The values of n tokens from position n_past: (k, v) [n_batch][n][n_head_kv][d] f32, rows
         behind count[b] as they were (in new tensors: undefined)."""
         torch = _torch()
         shape, dev = (self.n_batch, n, self.n_head_kv, self.d), self.device
-        k = torch.empty(shape, dtype=torch.float32, device=dev) if k is None else k
+        k = self.k_scale.new_empty(shape) if k is None else k
         v = torch.empty_like(k) if v is None else v
         if k.shape != shape or k.device != dev or v.shape != shape or v.device != dev:
             raise ValueError(f"k and v must have shape {shape} on {dev}")
         s = self._call(n, n_past, count, None, None)
-        _lib.ensure_init(dev.index)
-        _lib.check(_lib.load().zwg_kv8_read(self._ref, s, _dev_ptr(k, torch.float32, "k"), _dev_ptr(v, torch.float32, "v"),
+        _lib.check(_ready(dev).zwg_kv8_read(self._ref, s, _dev_ptr(k, torch.float32, "k"), _dev_ptr(v, torch.float32, "v"),
                                             _stream_on(dev)))
         return k, v
 
     def attn_workspace_bytes(self, n: int, n_head: int, n_past=None) -> int:
         """Workspace of attn for n tokens after n_past (None: the most there can be)."""
         s = self._call(n, max(self.n_ctx - n, 0) if n_past is None else n_past, None, None, None)
-        _lib.ensure_init(self.device.index)
-        return int(_lib.load().zwg_kv8_attn_workspace(self._ref, s, n_head))
+        return int(_ready(self.device).zwg_kv8_attn_workspace(self._ref, s, n_head))
 
     def attn(self, q, n_past, count=None, first=None, max_past=None, out=None, workspace=None):
         """Attention (zwg_kv8_attn) of q [n_batch][n][n_head][d] (f32 or bf16) at positions n_past..
@@ -1025,12 +1042,14 @@ class Kv8Cache:
         n, H = q.shape[1], q.shape[2]
         dev, dtype, shape = self.device, q.dtype, (self.n_batch, n, H, self.d)
         qr = _rows(q, dtype, dev, shape, "q")
-        if out is None:
-            out = (torch.empty_like if count is None else torch.zeros_like)(q, memory_format=torch.contiguous_format)
-        o = _rows(out, dtype, dev, shape, "out")
+        if out is not None:
+            o = _rows(out, dtype, dev, shape, "out")
+        else:
+            out, o = _new_rows(q, shape)
+            if count is not None:
+                out.zero_()
         s = self._call(n, n_past, count, first, max_past)
-        _lib.ensure_init(dev.index)
-        lib = _lib.load()
+        lib = _ready(dev)
         ws, size = None, 0
         if workspace is None:
             size = lib.zwg_kv8_attn_workspace(self._ref, s, H)
@@ -1097,11 +1116,10 @@ def llm_logits(logits, recent=None, n_recent=None, window: Optional[int] = None,
         if words < (V + 31) // 32:
             raise ValueError(f"allow must have {(V + 31) // 32} words, got {words}")
     if out is None:
-        out = torch.empty(m, dtype=torch.int32, device=dev)
+        out = torch.empty(m, dtype=torch.int32, device=dev) if recent is None else recent.new_empty(m)
     elif out.dtype is not torch.int32 or out.shape != (m,) or out.device != dev or (m > 1 and out.stride(0) < 1):
         raise ValueError(f"out must be an int32 tensor [{m}] on {dev}")
-    _lib.ensure_init(dev.index)
-    _lib.check(_lib.load().zwg_llm_logits(logits.data_ptr(), m, V, stride, ctypes.byref(r), out.data_ptr(), out.stride(0),
+    _lib.check(_ready(dev).zwg_llm_logits(logits.data_ptr(), m, V, stride, ctypes.byref(r), out.data_ptr(), out.stride(0),
                                           _stream_on(dev)))
     return out
 
