@@ -59,7 +59,7 @@ struct Plan {
 
 constexpr int SMALL = 4;            // warps of a small CTA, three of which share an SM
 constexpr int MAX_CLUSTER = 8;
-constexpr int MOST_SPLIT_ROWS = 32;  // query rows of a kv head above which the tcgen05 kernel runs
+constexpr int MOST_SPLIT_ROWS = 48;  // query rows of a kv head above which the tcgen05 kernel runs
 constexpr int WARP_RING = 16 * 1024;  // bytes a warp has for blocks on their way
 
 // Rows of a tile: one or two 8-wide N tiles, or the tcgen05 kernel's.
@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(32 * WARPS)
             ks = vs;
             vs = 0.f;
         }
-        if (!sm100::mbar_wait_warp(&full[warp][stage], phase, p.err)) {
+        if (!wait_for_warp(&full[warp][stage], phase, p.err)) {
             // gave up: no further copies; those on their way end before the ring is used again
             for (int s = 0; s < STAGES && blk + s * WARPS < to; s++) {
                 const int at_stage = (stage + s) % STAGES;

@@ -158,14 +158,14 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(Kv8Attn p, int 
         if (t < n_t && lane == 0 && n_tiles > 0) {
             constexpr uint32_t idesc_s = idesc_f16(BM, BN, false, false, false);
             constexpr uint32_t idesc_o = idesc_f16(BM, D, false, false, false);
-            bool ok = mbar_wait(&sm.q_full[t], 0, err);
+            bool ok = wait_for(&sm.q_full[t], 0, err);
             // tile 1 starts a softmax behind tile 0, so that the one's exponentials run during the other's products
-            if (t == 1) ok = ok && mbar_wait(&sm.p_full[0], 0, err);
+            if (t == 1) ok = ok && wait_for(&sm.p_full[0], 0, err);
             for (int j = 0; ok && j < n_tiles; j++) {
                 const int ks = j % S::KS, vs = j % S::VS;
-                if (!(ok = mbar_wait(&sm.k_full[ks], j / S::KS & 1, err))) break;
+                if (!(ok = wait_for(&sm.k_full[ks], j / S::KS & 1, err))) break;
                 // P of the tile before lies where S goes
-                if (j > 0 && !(ok = mbar_wait(&sm.pv_done[t], (j - 1) & 1, err))) break;
+                if (j > 0 && !(ok = wait_for(&sm.pv_done[t], (j - 1) & 1, err))) break;
                 tc_fence_after();
 #pragma unroll
                 for (int c = 0; c < P; c++)
@@ -178,8 +178,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(Kv8Attn p, int 
                 mma_commit(&sm.s_full[t]);
                 mma_commit(&sm.k_empty[ks]);
                 mbar_arrive(&sm.s_full[t]);
-                if (!(ok = mbar_wait(&sm.p_full[t], j & 1, err))) break;
-                if (!(ok = mbar_wait(&sm.v_full[vs], j / S::VS & 1, err))) break;
+                if (!(ok = wait_for(&sm.p_full[t], j & 1, err))) break;
+                if (!(ok = wait_for(&sm.v_full[vs], j / S::VS & 1, err))) break;
                 tc_fence_after();
 #pragma unroll
                 for (int c = 0; c < P; c++)
@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(Kv8Attn p, int 
         }
         for (int j = 0; j < n_tiles; j++) {
             const int ks = j % S::KS, vs = j % S::VS;
-            if (j >= S::KS && !mbar_wait_warp(&sm.k_empty[ks], (j / S::KS - 1) & 1, err)) break;
+            if (j >= S::KS && !wait_for_warp(&sm.k_empty[ks], (j / S::KS - 1) & 1, err)) break;
 #pragma unroll
             for (int i = 0; i < N; i++) {
                 const int e = tid + i * CONVERTERS, r = e / SEGS, seg = e % SEGS;
@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(Kv8Attn p, int 
             __syncwarp();
             if (lane == 0) mbar_arrive(&sm.k_full[ks]);
             if (j + 1 < n_tiles) load_k(j + 1);
-            if (j >= S::VS && !mbar_wait_warp(&sm.v_empty[vs], (j / S::VS - 1) & 1, err)) break;
+            if (j >= S::VS && !wait_for_warp(&sm.v_empty[vs], (j / S::VS - 1) & 1, err)) break;
 #pragma unroll
             for (int i = 0; i < N; i++) {
                 const int e = tid + i * CONVERTERS, blk = e / (D * 2), r = e / 2 % D;
@@ -291,8 +291,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(Kv8Attn p, int 
                     if (!(live_rows >> rr & 1)) x = make_float4(0.f, 0.f, 0.f, 0.f);
                     uint32_t top = max(max(__float_as_uint(fabsf(x.x)), __float_as_uint(fabsf(x.y))),
                                        max(__float_as_uint(fabsf(x.z)), __float_as_uint(fabsf(x.w))));
-#pragma unroll
-                    for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+                    top = __reduce_max_sync(LANES == 32 ? 0xffffffffu : lane < 16 ? 0xffffu : 0xffff0000u, top);
                     float p2, inv;
                     power_of(__uint_as_float(top), p2, inv);
                     if (lane % LANES == 0) sm.part[t][0][qr] = p2 * scale;
@@ -321,7 +320,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(Kv8Attn p, int 
             float m = -INFINITY, l = 0.f;
             uint32_t ref = 0x00800000u;  // bits of a power of two above every vs so far
             for (int j = 0; j < n_tiles; j++) {
-                ok = mbar_wait_warp(&sm.s_full[t], j & 1, err);
+                ok = wait_for_warp(&sm.s_full[t], j & 1, err);
                 tc_fence_after();
                 const float4 sc01 = *reinterpret_cast<const float4*>(sm.scale[j & 3]);
                 const float4 sc23 = *reinterpret_cast<const float4*>(sm.scale[j & 3] + 2);
@@ -423,7 +422,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(Kv8Attn p, int 
             // the rows' outputs, or their part of the keys' cuts: the two threads' sums, then O through the warp's
             // part of the queries' shared memory, 16 columns at a time, so that 4 lanes write 64 consecutive bytes
             // (of f32) of a row
-            if (ok && n_tiles > 0) ok = mbar_wait_warp(&sm.pv_done[t], (n_tiles - 1) & 1, err);
+            if (ok && n_tiles > 0) ok = wait_for_warp(&sm.pv_done[t], (n_tiles - 1) & 1, err);
             tc_fence_after();
             sm.part[t][half][r] = l;
             ok = all_of(pair, 64, ok);
