@@ -40,7 +40,11 @@ constexpr int THREADS = SOFTMAX + CONVERTERS + 64;
 constexpr float kUnit = 2048.f;   // P's pieces hold 2^11 p, and p < 2^4
 constexpr float kStale = 4.f;
 constexpr uint32_t TMEM_COLS = 512;
+// With one piece of d 64 there is room for P beside S: the next S is computed while the probabilities are.
+template <int D, int P>
+constexpr bool BESIDE = D == 64 && P == 1;
 __host__ __device__ constexpr uint32_t s_col(int t) { return t * 128u; }
+__host__ __device__ constexpr uint32_t beside_col(int t) { return 384u + t * 64u; }
 template <int D>
 __host__ __device__ constexpr uint32_t o_col(int t) { return 256u + t * D; }
 
@@ -52,7 +56,7 @@ struct Smem {
     uint8_t v[VS][BN / 64][D * 128];     // value columns: [d][64 f16 of tokens]
     float2 scale[4][BLOCKS];             // (ks, vs) of a tile's blocks: a tile's are read until its P is there
     float part[2][2][BM];                // what a row's two threads tell each other: [query tile][half]
-    uint64_t q_full[2], k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], s_full[2], p_full[2], pv_done[2], drained[2];
+    uint64_t q_full[2], k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], s_full[2], s_free[2], p_full[2], pv_done[2], drained[2];
     uint32_t tmem_base;
 };
 
@@ -129,6 +133,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(Kv8Attn p, int 
         for (int t = 0; t < 2; t++) {
             mbar_init(&sm.q_full[t], 8);
             mbar_init(&sm.s_full[t], 2);  // the products' completion, and the issuer's own: it has seen the scales
+            mbar_init(&sm.s_free[t], 8);
             mbar_init(&sm.p_full[t], 8);
             mbar_init(&sm.pv_done[t], 1);
             mbar_init(&sm.drained[t], 1);
@@ -161,11 +166,11 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(Kv8Attn p, int 
             bool ok = wait_for(&sm.q_full[t], 0, err);
             // tile 1 starts a softmax behind tile 0, so that the one's exponentials run during the other's products
             if (t == 1) ok = ok && wait_for(&sm.p_full[0], 0, err);
-            for (int j = 0; ok && j < n_tiles; j++) {
-                const int ks = j % S::KS, vs = j % S::VS;
-                if (!(ok = wait_for(&sm.k_full[ks], j / S::KS & 1, err))) break;
-                // P of the tile before lies where S goes
-                if (j > 0 && !(ok = wait_for(&sm.pv_done[t], (j - 1) & 1, err))) break;
+            const auto scores = [&](int j) {
+                const int ks = j % S::KS;
+                if (!wait_for(&sm.k_full[ks], j / S::KS & 1, err)) return false;
+                // S goes where the last S was read from, or its P, which the PV reads
+                if (j > 0 && !wait_for(BESIDE<D, P> ? &sm.s_free[t] : &sm.pv_done[t], (j - 1) & 1, err)) return false;
                 tc_fence_after();
 #pragma unroll
                 for (int c = 0; c < P; c++)
@@ -178,7 +183,14 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(Kv8Attn p, int 
                 mma_commit(&sm.s_full[t]);
                 mma_commit(&sm.k_empty[ks]);
                 mbar_arrive(&sm.s_full[t]);
-                if (!(ok = wait_for(&sm.p_full[t], j & 1, err))) break;
+                return true;
+            };
+            if (BESIDE<D, P>) ok = ok && scores(0);
+            for (int j = 0; ok && j < n_tiles; j++) {
+                const int vs = j % S::VS;
+                if (!BESIDE<D, P>) ok = scores(j);
+                else if (j + 1 < n_tiles) ok = scores(j + 1);
+                if (!ok || !(ok = wait_for(&sm.p_full[t], j & 1, err))) break;
                 if (!(ok = wait_for(&sm.v_full[vs], j / S::VS & 1, err))) break;
                 tc_fence_after();
 #pragma unroll
@@ -186,8 +198,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(Kv8Attn p, int 
 #pragma unroll
                     for (int kk = 0; kk < BN / 16; kk++) {
                         const uint64_t vb = smem_desc_sw128(smem_u32(sm.v[vs][kk / 4]) + kk % 4 * 32, 16, 1024);
-                        mma_f16_ts(tmem + o_col<D>(t), tmem + s_col(t) + kk * 16 + c * 8, vb, idesc_o,
-                                   j > 0 || c > 0 || kk > 0);
+                        const uint32_t pa = BESIDE<D, P> ? beside_col(t) + kk * 8 : s_col(t) + kk * 16 + c * 8;
+                        mma_f16_ts(tmem + o_col<D>(t), tmem + pa, vb, idesc_o, j > 0 || c > 0 || kk > 0);
                     }
                 mma_commit(&sm.pv_done[t]);
                 mma_commit(&sm.v_empty[vs]);
@@ -317,10 +329,11 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(Kv8Attn p, int 
             const int seen_by_all = at.past + (row0 + t * BM) / group + 1;     // by the tile's first row
             const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
             const uint32_t s_addr = tmem + lanes + s_col(t) + half * 64, o_addr = tmem + lanes + o_col<D>(t) + half * (D / 2);
+            const uint32_t p_addr = tmem + lanes + beside_col(t) + half * 32;
             float m = -INFINITY, l = 0.f;
             uint32_t ref = 0x00800000u;  // bits of a power of two above every vs so far
             for (int j = 0; j < n_tiles; j++) {
-                ok = wait_for_warp(&sm.s_full[t], j & 1, err);
+                ok = ok && wait_for_warp(&sm.s_full[t], j & 1, err);
                 tc_fence_after();
                 const float4 sc01 = *reinterpret_cast<const float4*>(sm.scale[j & 3]);
                 const float4 sc23 = *reinterpret_cast<const float4*>(sm.scale[j & 3] + 2);
@@ -375,7 +388,11 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(Kv8Attn p, int 
                 const float alpha = grow ? exp2_approx(was - base) : 1.f;
                 const float keep = alpha * (__uint_as_float(ref) * inv_ref);
                 ref = top_ref;
-                // S was computed after the PV before it: O is complete
+                // O is complete (and the last P read): S was computed after that PV, or waits for it here
+                if (BESIDE<D, P> && j > 0) {
+                    ok = wait_for_warp(&sm.pv_done[t], (j - 1) & 1, err);
+                    tc_fence_after();
+                }
                 if (j > 0 && __any_sync(0xffffffffu, keep != 1.f)) {
 #pragma unroll
                     for (int c = 0; c < D / 64; c++) {
@@ -410,8 +427,13 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(Kv8Attn p, int 
                         uint32_t o[8];
 #pragma unroll
                         for (int e = 0; e < 8; e++) o[e] = w[e][k];
-                        tmem_st8(s_addr + c + k * 8, o);
+                        tmem_st8(BESIDE<D, P> ? p_addr + c / 2 : s_addr + c + k * 8, o);
                     }
+                }
+                if (BESIDE<D, P>) {  // S has been read
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sm.s_free[t]);
                 }
                 l = l * alpha + (sum.x + sum.y);
                 tmem_st_wait();
