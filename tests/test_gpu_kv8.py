@@ -292,6 +292,9 @@ ATTN = [  # batch, heads, heads_kv, d, n, past
     (1, 6, 1, 128, 67, [90]),
     (1, 3, 3, 128, 256, [0]),
     (1, 40, 1, 64, 2, [31]),
+    (2, 16, 2, 128, 5, [300, 2]),
+    (1, 16, 2, 64, 6, [1500]),
+    (1, 13, 1, 128, 20, [40]),
 ]
 
 
@@ -338,6 +341,71 @@ def test_attention_sharp_and_flat_scores(env):
     for size in (0.0, 1e-30, 1e-4, 30.0, 200.0):
         check_attn(torch, ops, rng, cache, want, 4, [499, 499], 1, size=size, tensor=False)
         check_attn(torch, ops, rng, cache, want, 4, [460, 460], 40, size=size, tensor=False)
+
+
+@pytest.mark.parametrize("n", [1, 3, 70])
+def test_attention_scores_of_any_size_stay_finite(env, n):
+    """Scores up to the largest that f32 holds: the key they belong to takes all the weight, nothing overflows."""
+    torch, ops = env
+    rng = np.random.default_rng(n)
+    k, v = normal(rng, 1, 160, 1, 64), normal(rng, 1, 160, 1, 64)
+    k[0, 37] = 9 * np.sign(k[0, 37])
+    cache = ops.Kv8Cache.empty(1, 1, 64, 160)
+    cache.append(up(torch, k), up(torch, v), 0)
+    ck, cv = cache.read(160, 0)
+    for size in (1e3, 1e8, 1e20, 1e33):
+        q = up(torch, np.broadcast_to(np.sign(k[0, 37]), (1, n, 2, 64)) * np.float32(size))
+        out = cache.attn(q, 160 - n)
+        assert torch.equal(out, cv[0, 37].expand_as(out)) or torch.allclose(out, cv[0, 37].expand_as(out), rtol=1e-5, atol=0)
+    # values of very different sizes in the blocks that a query weighs alike
+    for scale in (1e-30, 1e30):
+        v2 = v.copy()
+        v2[0, 64:] *= np.float32(scale)
+        cache = ops.Kv8Cache.empty(1, 1, 64, 160)
+        cache.append(up(torch, k), up(torch, v2), 0)
+        _, cv = cache.read(160, 0)
+        q = torch.zeros(1, n, 2, 64, device="cuda:0")
+        out = cache.attn(q, 160 - n)
+        for i in range(n):
+            want = cv[0, :160 - n + i + 1].double().mean(0).float()
+            top = cv[0, :160 - n + i + 1].abs().max()
+            assert ((out[0, i] - want).abs() <= 1e-6 * top).all()
+    ops.sync()
+
+
+def test_attention_out_of_range_sequence_is_skipped(env):
+    torch, ops = env
+    from zwhisper_b200._lib import ZwgError
+    rng = np.random.default_rng(11)
+    cache, want = fill(torch, ops, rng, 4, 1, 64, 320, [300] * 4)
+    for n in (1, 70):
+        q = up(torch, normal(rng, 4, n, 2, 64))
+        good = cache.attn(q, i32(torch, [200] * 4), max_past=200)
+        out = torch.full_like(q, 5.0)
+        ops.sync()
+        cache.attn(q, i32(torch, [200, 201, -1, 200]), first=i32(torch, [0, 0, 0, -1]), max_past=200, out=out)
+        with pytest.raises(ZwgError):
+            ops.sync()
+        assert torch.equal(out[0], good[0]) and (out[1:] == 5).all()
+    ops.sync()
+
+
+def test_attention_on_two_streams_at_once(env):
+    torch, ops = env
+    rng = np.random.default_rng(12)
+    cache, _ = fill(torch, ops, rng, 2, 2, 64, 4096, [4000, 4000])
+    qs = [up(torch, normal(rng, 2, n, 8, 64)) for n in (1, 1, 40, 40)]
+    want = [cache.attn(q, 4000 - q.shape[1]) for q in qs]
+    streams = [torch.cuda.Stream() for _ in qs]
+    torch.cuda.synchronize()
+    got = [[] for _ in qs]
+    for _ in range(10):
+        for i, (q, s) in enumerate(zip(qs, streams)):
+            with torch.cuda.stream(s):
+                got[i].append(cache.attn(q, 4000 - q.shape[1]))
+    torch.cuda.synchronize()
+    for i, w in enumerate(want):
+        assert all(torch.equal(w, g) for g in got[i])
 
 
 def test_attention_nan_blocks_reach_only_the_queries_that_see_them(env):

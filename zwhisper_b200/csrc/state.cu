@@ -290,29 +290,33 @@ int zwg_llm_state_create_kv8(size_t n_layer, size_t n_batch, size_t n_head, size
     const size_t per = 2 * (ints + scales + open) + tags;
     const size_t stage = segs * d * zwg_llm_state::stage_pitch(n_chunk) * sizeof(float);
     int rc = ZWG_OK;
-    cudaError_t e = cudaMalloc(&st->kv8_mem, per * n_layer);
-    if (e == cudaSuccess) e = cudaMemset(st->kv8_mem, 0, per * n_layer);
-    if (e == cudaSuccess) e = cudaMalloc(&st->stage_kt, stage);
-    if (e == cudaSuccess) e = cudaMalloc(&st->stage_v, stage);
-    for (size_t l = 0; l < n_layer && e == cudaSuccess; l++) {
-        char* p = (char*)st->kv8_mem + l * per;
-        zwg_kv8 k{};
-        k.k = (int8_t*)p;
-        k.v = (int8_t*)(p + ints);
-        k.k_scale = (float*)(p + 2 * ints);
-        k.v_scale = (float*)(p + 2 * ints + scales);
-        k.k_open = (float*)(p + 2 * (ints + scales));
-        k.v_open = (float*)(p + 2 * (ints + scales) + open);
-        k.open_block = (int32_t*)(p + 2 * (ints + scales + open));
-        k.n_batch = n_batch;
-        k.n_head_kv = n_head_kv;
-        k.d = d;
-        k.n_ctx = n_ctx;
-        e = cudaMemset(k.open_block, 0xff, segs * sizeof(int32_t));
-        st->kv8.push_back(k);
+    try {
+        cudaError_t e = cudaMalloc(&st->kv8_mem, per * n_layer);
+        if (e == cudaSuccess) e = cudaMemset(st->kv8_mem, 0, per * n_layer);
+        if (e == cudaSuccess) e = cudaMalloc(&st->stage_kt, stage);
+        if (e == cudaSuccess) e = cudaMalloc(&st->stage_v, stage);
+        for (size_t l = 0; l < n_layer && e == cudaSuccess; l++) {
+            char* p = (char*)st->kv8_mem + l * per;
+            zwg_kv8 k{};
+            k.k = (int8_t*)p;
+            k.v = (int8_t*)(p + ints);
+            k.k_scale = (float*)(p + 2 * ints);
+            k.v_scale = (float*)(p + 2 * ints + scales);
+            k.k_open = (float*)(p + 2 * (ints + scales));
+            k.v_open = (float*)(p + 2 * (ints + scales) + open);
+            k.open_block = (int32_t*)(p + 2 * (ints + scales + open));
+            k.n_batch = n_batch;
+            k.n_head_kv = n_head_kv;
+            k.d = d;
+            k.n_ctx = n_ctx;
+            e = cudaMemset(k.open_block, 0xff, segs * sizeof(int32_t));
+            st->kv8.push_back(k);
+        }
+        if (e != cudaSuccess) rc = cuda_fail("llm state in 8 bits", e);
+        if (!rc) rc = make_tables(st, rope_base);
+    } catch (const std::bad_alloc&) {
+        rc = fail("llm state in 8 bits: out of host memory");
     }
-    if (e != cudaSuccess) rc = cuda_fail("llm state in 8 bits", e);
-    if (!rc) rc = make_tables(st, rope_base);
     // the most a call of up to n_chunk tokens needs, at the end of the context
     size_t ws = 0;
     for (size_t n = 1; n <= n_chunk && !rc; n++) {
