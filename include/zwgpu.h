@@ -656,7 +656,8 @@ ZWG_API int zwg_kv8_append(const zwg_kv8* c, const zwg_seqs* s, int type, const 
  * [n_batch][n][n_head_kv][d] f32, either may be NULL. */
 ZWG_API int zwg_kv8_read(const zwg_kv8* c, const zwg_seqs* s, float* k, float* v, void* stream);
 
-/* Bytes of workspace zwg_kv8_attn needs (0: none). */
+/* Bytes of workspace (0: none) that zwg_kv8_attn may need for this call and for calls of the same
+ * sizes that are shorter (a smaller n_past). */
 ZWG_API size_t zwg_kv8_attn_workspace(const zwg_kv8* c, const zwg_seqs* s, size_t n_head);
 
 /* Attention of the call's queries (n_head a multiple of n_head_kv; query head h reads kv head

@@ -333,6 +333,30 @@ def test_attention_long_context_splits(env, d):
     check_attn(torch, ops, rng, cache, want, 6, [8937, 4257], 64)
 
 
+@pytest.mark.parametrize("B,n,lengths", [(1, 1, (500, 770, 1000, 1600, 2050)), (6, 1, (900, 1500, 3000)), (8, 1, (1600, 3100)),
+                                         (12, 1, (1100, 1700)), (24, 1, (770, 1300)), (8, 2, (1000, 2200))])
+def test_attention_however_the_keys_are_cut(env, B, n, lengths):
+    """Batches and lengths on both sides of where the number and the size of the cuts change."""
+    torch, ops = env
+    rng = np.random.default_rng(B + n)
+    n_ctx = (max(lengths) + 31) // 32 * 32
+    cache, want = fill(torch, ops, rng, B, 2, 64, n_ctx, [max(lengths)] * B)
+    for past in lengths:
+        ends = [max(past - n - 37 * b, 0) for b in range(B)]
+        check_attn(torch, ops, rng, cache, want, 12, ends, n, max_past=past - n)
+    check_attn(torch, ops, rng, cache, want, 12, ends, n, bf16=True, max_past=past - n)
+
+
+def test_attention_workspace_serves_shorter_caches(env):
+    torch, ops = env
+    for B in (1, 2, 3, 5, 7, 8, 9, 12, 16, 24, 64):
+        cache = ops.Kv8Cache.empty(B, 2, 64, 32768 if B < 9 else 4096)
+        for n in (1, 2, 7, 200):
+            sizes = [cache.attn_workspace_bytes(n, 12, n_past=p) for p in range(0, cache.n_ctx - n, 151)]
+            assert sizes == sorted(sizes)
+            assert sizes[-1] <= cache.attn_workspace_bytes(n, 12)
+
+
 def test_attention_sharp_and_flat_scores(env):
     """One key that takes all the weight, equal keys, zero queries, queries of very different sizes."""
     torch, ops = env

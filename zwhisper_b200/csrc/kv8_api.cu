@@ -242,6 +242,7 @@ size_t zwg_kv8_attn_workspace(const zwg_kv8* cache, const zwg_seqs* s, size_t n_
     if (!c || check_cache(cache, "kv8_attn") || check_seqs(s, cache->n_ctx, "kv8_attn") || check_batch(cache, s, "kv8_attn") ||
         check_heads(cache, s, n_head, "kv8_attn"))
         return 0;
+    const OnDevice on(c->device);
     return attn_workspace(cache, s, n_head, c->sm_count);
 }
 
@@ -259,11 +260,11 @@ int zwg_kv8_attn(const zwg_kv8* cache, const zwg_seqs* s, int type, size_t n_hea
     if (rc) return rc;
     Ctx* c = cur();
     if (!c) return ZWG_ERROR;
+    const OnDevice on(c->device);
     const size_t need = attn_workspace(cache, s, n_head, c->sm_count);
     if (need && (!workspace || workspace_bytes < need))
         return fail("kv8_attn: workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : 0, need);
     if (!al(workspace, 16)) return fail("kv8_attn: workspace must be 16-byte aligned");
-    const OnDevice on(c->device);
     zwg::Kv8Attn p{};
     p.c = cache_of(cache);
     p.s = seqs_of(s);

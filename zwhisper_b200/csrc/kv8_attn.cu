@@ -55,6 +55,7 @@ struct Plan {
     int tiles;   // tiles of query rows of a (sequence, kv head)
     int warps;   // of a CTA; 0: the tcgen05 kernel's
     int splits;  // cuts of the keys
+    int most_splits;  // of this and of shorter caches: the workspace of a long cache serves shorter ones
 };
 
 constexpr int SMALL = 4;            // warps of a small CTA, three of which share an SM
@@ -67,6 +68,49 @@ int tile_rows(int rows) { return rows <= 8 ? 8 : rows <= MOST_SPLIT_ROWS ? 16 : 
 // Warps of a CTA that has an SM to itself; the registers of two N tiles leave room for 8.
 constexpr int big_warps(int tile_rows) { return tile_rows == 8 ? 12 : 8; }
 
+// Clusters of n CTAs that run at once on the current device: a cluster lives in one GPC, and the GPCs
+// have different numbers of SMs (n 4: 33 of 148 SMs, n 8: 15). Asked once for each device.
+int clusters_of(int tile_rows, bool big, int n);
+int clusters_at_once(int tile_rows, bool big, int n) {
+    static std::atomic<int> known[64][2][2][MAX_CLUSTER + 1];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 1;
+    std::atomic<int>& at = known[dev & 63][tile_rows == 8][big][n];
+    int count = at.load(std::memory_order_relaxed);
+    if (count == 0) at.store(count = std::max(1, clusters_of(tile_rows, big, n)), std::memory_order_relaxed);
+    return count;
+}
+
+// How the keys of `ctas` (sequence, kv head, tile of rows)s are cut for CTAs of one kind, and what it
+// costs: the blocks that follow each other in a warp, and 0.7 of one for the second kernel.
+struct Cut {
+    int splits, most_splits;  // most: with any shorter cache
+    float cost;
+};
+Cut cut_for(int tile_rows, bool big, long long ctas, int blocks, int combine_rows, int sm_count) {
+    const int warps = big ? big_warps(tile_rows) : SMALL, per_sm = big_warps(tile_rows) / warps;
+    const int useful = (blocks + warps - 1) / warps;
+    const auto rounds = [&](int n) { return (useful + n - 1) / n; };
+    // one wave of clusters: one that waits for a second wave doubles the time (8 sequences of 4512 tokens in
+    // clusters of 8, of which 15 fit: 19.5 us, of 6: 11.3)
+    int in_cluster = (int)std::min<long long>(std::min(MAX_CLUSTER, useful), std::max<long long>(1, (long long)per_sm * sm_count / ctas));
+    while (in_cluster > 1 && ctas > clusters_at_once(tile_rows, big, in_cluster)) in_cluster--;
+    // More splits than that, and the combining kernel, whose CTAs start early if places are left for them:
+    // 8 to an SM, 2 beside two small CTAs (2 sequences of 20001 tokens: all SMs taken 14.4 us, 108 of them 12.2)
+    const long long places = (long long)per_sm * sm_count - (combine_rows + 8 / per_sm - 1) / (8 / per_sm);
+    const int most = (int)std::min<long long>(useful, places / ctas);
+    Cut c{in_cluster, in_cluster, (float)rounds(in_cluster)};
+    if (most > MAX_CLUSTER) {
+        const int r = rounds(most);
+        if (r + 0.7f < c.cost) c = {std::max(MAX_CLUSTER + 1, (useful + r - 1) / r), most, r + 0.7f};
+        c.most_splits = most;
+    }
+    return c;
+}
+
+// Splits of small CTAs with one block for each warp.
+int one_each(int blocks) { return (blocks + SMALL - 1) / SMALL; }
+
 Plan plan_for(const Kv8& c, const Seqs& s, int n_head, int sm_count) {
     const int rows = s.n * (n_head / c.n_head_kv), big = big_warps(tile_rows(rows));
     Plan p;
@@ -77,22 +121,34 @@ Plan plan_for(const Kv8& c, const Seqs& s, int n_head, int sm_count) {
         // keys are cut while SMs stay empty, two tiles of keys to a cut at least
         const int key_tiles = (blocks * KV8_BLOCK + KV8_PREFILL_KEYS - 1) / KV8_PREFILL_KEYS;
         p.warps = 0;
-        p.splits = (int)std::min<long long>(std::max<long long>(1, sm_count / ctas), std::max(1, key_tiles / 2));
+        p.splits = p.most_splits = (int)std::min<long long>(std::max<long long>(1, sm_count / ctas), std::max(1, key_tiles / 2));
         return p;
     }
-    const int per_sm = big / SMALL;
-    const long long small_places = (long long)per_sm * sm_count;
-    // One wave, of big CTAs (fewer states to merge) unless they leave more places empty than small ones do
-    const long long n_big = sm_count / ctas, n_small = small_places / ctas;
-    const bool use_big = blocks > SMALL && n_big > 0 && n_big * ctas * small_places >= 0.85 * n_small * ctas * sm_count;
-    p.warps = use_big ? big : SMALL;
-    const long long want = std::max<long long>(1, use_big ? n_big : n_small);
-    p.splits = (int)std::min<long long>(want, std::max(1, (blocks + p.warps - 1) / p.warps));
-    // More splits than a cluster has cost a second kernel, about as long as a warp takes for 6 blocks.
-    if (p.splits > MAX_CLUSTER && (p.splits <= 2 * MAX_CLUSTER && blocks <= 6 * p.warps * MAX_CLUSTER)) p.splits = MAX_CLUSTER;
-    // A cluster lives in one of the 8 GPCs: what does not divide their places would wait for a second wave.
-    const int places = (use_big ? sm_count : (int)small_places) / 8;
-    while (p.splits > 1 && p.splits <= MAX_CLUSTER && ctas > 8 * (places / p.splits)) p.splits--;
+    const int combine_rows = (int)std::min<long long>((long long)s.n_batch * s.n * n_head, 8 * sm_count);
+    // most CTAs for which one block to each warp of small CTAs was the fastest plan: half the SMs
+    const int few = (int)(sm_count / 2 / ctas);
+    int most = 1;
+    if (blocks <= 2 * big && ctas <= sm_count) {
+        // no cut: merging two CTAs takes longer than a second block to each warp
+        p.warps = blocks <= SMALL ? SMALL : big;
+        p.splits = 1;
+    } else if (one_each(blocks) <= few || (one_each(blocks) <= MAX_CLUSTER && ctas <= clusters_at_once(tile_rows(rows), false, one_each(blocks)))) {
+        p.warps = SMALL;
+        p.splits = one_each(blocks);
+    } else {
+        // big CTAs (fewer states to merge) unless small ones leave fewer places empty
+        const Cut small = cut_for(tile_rows(rows), false, ctas, blocks, combine_rows, sm_count);
+        const Cut large = cut_for(tile_rows(rows), true, ctas, blocks, combine_rows, sm_count);
+        const bool use_big = ctas <= sm_count && large.cost <= small.cost;
+        p.warps = use_big ? big : SMALL;
+        p.splits = use_big ? large.splits : small.splits;
+        // big CTAs in clusters that put as many warps to work cost no more with any cache
+        const int in_cluster = cut_for(tile_rows(rows), true, ctas, big * MAX_CLUSTER, combine_rows, sm_count).splits;
+        const int small_most = cut_for(tile_rows(rows), false, ctas, 1 << 20, combine_rows, sm_count).most_splits;
+        const bool always_big = ctas <= sm_count && large.most_splits <= MAX_CLUSTER && in_cluster * big >= small_most * SMALL;
+        most = always_big ? 1 : std::max(large.most_splits, small.most_splits);
+    }
+    p.most_splits = std::max(most, std::max(p.splits, std::min(few, one_each(blocks))));
     return p;
 }
 
@@ -520,6 +576,32 @@ __global__ void __launch_bounds__(256) kv8_combine_kernel(Kv8Attn p, int splits,
     store4(out, acc, sum == 0.f ? 0.f : 1.f / sum, vec & 2);
 }
 
+template <int NT, int WARPS>
+int clusters_of_kind(int n) {
+    const auto kern = kv8_split_kernel<float, 128, NT, 2, WARPS>;  // the others need no more than it
+    static std::atomic<uint64_t> done{0};
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)n);
+    cfg.blockDim = dim3(32 * WARPS);
+    cfg.dynamicSmemBytes = WARPS * WARP_RING;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)n;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int count = 0;
+    if (allow_smem(done, (const void*)kern, WARPS * WARP_RING) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&count, kern, &cfg) != cudaSuccess)
+        (void)cudaGetLastError();
+    return count;
+}
+
+int clusters_of(int tile_rows, bool big, int n) {
+    if (tile_rows == 8) return big ? clusters_of_kind<1, big_warps(8)>(n) : clusters_of_kind<1, SMALL>(n);
+    return big ? clusters_of_kind<2, big_warps(16)>(n) : clusters_of_kind<2, SMALL>(n);
+}
+
 template <typename T, int D, int NT, int P, int WARPS>
 int split_launch(const Kv8Attn& p, const Plan& plan, int vec, cudaStream_t st) {
     constexpr int RING = WARPS * WARP_RING;
@@ -583,8 +665,8 @@ size_t kv8_attn_workspace_bytes(const Kv8& c, const Seqs& s, int n_head, int sm_
     if (s.n_batch == 0 || s.n == 0) return 0;
     const Plan p = plan_for(c, s, n_head, sm_count);
     const int rows = s.n * (n_head / c.n_head_kv);
-    return p.splits <= (p.warps ? MAX_CLUSTER : 1) ? 0
-                         : (size_t)s.n_batch * c.n_head_kv * p.tiles * p.splits * tile_rows(rows) * (c.d + 4) * sizeof(float);
+    if (p.most_splits <= (p.warps ? MAX_CLUSTER : 1)) return 0;
+    return (size_t)s.n_batch * c.n_head_kv * p.tiles * p.most_splits * tile_rows(rows) * (c.d + 4) * sizeof(float);
 }
 
 int kv8_attn_launch(const Kv8Attn& p, int type, int pieces, int sm_count, cudaStream_t st) {
