@@ -87,7 +87,9 @@ def attention(q, k, v, past, count, first, pieces, out_half_step=0.0):
       - all relative to sum p |v| / sum p, and the half step of the output's type;
       - a probability's last piece ends at f16's smallest step: 2^15 p vs / ref (ref the largest
         value scale the call's rows see, sum p >= 1) is off by half of 2^-24 at the least, which is
-        2^-40 of ref, so 2^-40 of the largest value, for each key and int8 unit of 127."""
+        2^-40 of ref, so 2^-40 of the largest value, for each key and int8 unit of 127. Calls of more
+        than 48 query rows to a kv head hold 2^11 p vs / ref with p up to 2^4 (a maximum that is at
+        most 4 too low, so sum p >= 1 as before): half of 2^-24 there is 2^-36 of ref."""
     B, n, H, d = q.shape
     group = H // k.shape[1]
     out, tol = np.full(q.shape, np.nan), np.zeros(q.shape)
@@ -111,7 +113,7 @@ def attention(q, k, v, past, count, first, pieces, out_half_step=0.0):
                 piece = {0: 0.0, 1: 2.0 ** -11, 2: 2.0 ** -22}[pieces]
                 ds = size * (piece + (d + 20) * 2.0 ** -23) + 2.0 ** -22 * (1 + np.abs(s).max())
                 rel = 2 * ds + (2.0 ** -11 if pieces < 2 else 2.0 ** -21) + (hi - lo + 32) * 2.0 ** -23
-                least = (hi - lo) * 2.0 ** -40 * np.abs(v[b, h // group, :p + m]).max()
+                least = (hi - lo) * (2.0 ** -40 if n * group <= 48 else 2.0 ** -36) * np.abs(v[b, h // group, :p + m]).max()
                 tol[b, i, h] = rel * (w @ np.abs(vv)) + out_half_step * np.abs(out[b, i, h]) + least
     return out, tol * 1.01 + 1e-30
 

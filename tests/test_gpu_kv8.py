@@ -357,6 +357,31 @@ def test_attention_workspace_serves_shorter_caches(env):
             assert sizes[-1] <= cache.attn_workspace_bytes(n, 12)
 
 
+@pytest.mark.parametrize("B,H,d,n,past,pad", [(40, 2, 64, 150, 2000, 0), (40, 2, 128, 131, 1700, 4), (1, 2, 128, 130, 4000, 0)])
+def test_attention_sums_do_not_drift_with_the_keys(env, B, H, d, n, past, pad):
+    """Two pieces keep the accuracy of f32 sums over thousands of keys: within 2.5e-6 of the exact output in
+    norm. Rows behind the 128th of a tile, unaligned rows (pad), whole and partial tiles."""
+    torch, ops = env
+    rng = np.random.default_rng(d)
+    n_ctx = (past + n + 31) // 32 * 32
+    k, v = (up(torch, normal(rng, B, past + n, 1, d)) for _ in range(2))
+    cache = ops.Kv8Cache.empty(B, 1, d, n_ctx)
+    cache.append(k, v, 0)
+    q = up(torch, normal(rng, B, n, H, d))
+    rows = torch.full((B, n, H * d + pad // 2), 7.0, device="cuda:0")
+    out = rows[..., :H * d].unflatten(-1, (H, d))
+    cache.attn(q, past, out=out)
+    kk, vv = (x[:, :, 0].double() for x in cache.read(past + n, 0))
+    s = torch.einsum("bnhd,bkd->bnhk", q.double(), kk) / d ** 0.5
+    hidden = torch.arange(past + n, device="cuda:0")[None] > past + torch.arange(n, device="cuda:0")[:, None]
+    exact = torch.einsum("bnhk,bkd->bnhd", s.masked_fill(hidden[:, None], float("-inf")).softmax(-1), vv)
+    # runs of 768 keys: 96 truncated sums (half a step of 2^-23 each, 48 of them behind an average key) and
+    # as many in the scores' and the last roundings' share: 48 * 0.36 * 2^-23 = 2.1e-6 at the most
+    assert (out.double() - exact).norm() < 2.5e-6 * exact.norm()
+    assert (rows[..., H * d:] == 7.0).all()
+    ops.sync()
+
+
 def test_attention_sharp_and_flat_scores(env):
     """One key that takes all the weight, equal keys, zero queries, queries of very different sizes."""
     torch, ops = env

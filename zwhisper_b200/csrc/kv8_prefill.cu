@@ -48,6 +48,19 @@ __host__ __device__ constexpr uint32_t beside_col(int t) { return 384u + t * 64u
 template <int D>
 __host__ __device__ constexpr uint32_t o_col(int t) { return 256u + t * D; }
 
+// The tensor cores truncate their sums, 2 x 128 / 16 of them to a key tile, which shrinks O by 2e-9 of it
+// for each key: 1.6e-5 after 8000 keys. So where two pieces ask for f32's accuracy, the sums of MOST_RUN
+// tiles at the most are drained into f32 sums that wait in the output's own place. 32 x 256 tokens after 1744
+// at d 128: 261 us and off by 4.1e-6 without, 288 us and 1.9e-6 in runs of 8, 300 us and 1.35e-6 of 6;
+// 1.5e-6 at any length. (The small query pieces go first for the same reason: 3e-7 less.)
+constexpr int MOST_RUN = 6;
+// Key tiles from one drain to the next, of n in all.
+template <int P>
+ZWG_DEV int run_of(int n) {
+    const int runs = (n + MOST_RUN - 1) / MOST_RUN;
+    return P == 1 || runs < 2 ? n : (n + runs - 1) / runs;
+}
+
 template <int D, int P>
 struct Smem {
     static constexpr int KS = 2, VS = D * P > 128 ? 1 : 2;  // buffers of keys and values
@@ -85,6 +98,15 @@ ZWG_DEV bool all_of(int id, int n, bool ok) {
         : "r"(ok ? 1u : 0u), "r"(id), "r"(n)
         : "memory");
     return all != 0;
+}
+
+// o f + (had g) h
+ZWG_DEV float4 summed(const uint32_t* o, float f, float4 had, float g, float h) {
+    return make_float4(__uint_as_float(o[0]) * f + had.x * g * h, __uint_as_float(o[1]) * f + had.y * g * h,
+                       __uint_as_float(o[2]) * f + had.z * g * h, __uint_as_float(o[3]) * f + had.w * g * h);
+}
+ZWG_DEV float4 had_at(const float* p, bool whole) {
+    return whole ? *reinterpret_cast<const float4*>(p) : make_float4(p[0], p[1], p[2], p[3]);
 }
 
 // 16 int8 -> two 16-byte units of f16.
@@ -176,7 +198,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(Kv8Attn p, int 
                 for (int c = 0; c < P; c++)
 #pragma unroll
                     for (int kk = 0; kk < D / 16; kk++) {
-                        const uint64_t qa = smem_desc_sw128(smem_u32(sm.q[t][c][kk / 4]) + kk % 4 * 32, 16, 1024);
+                        const uint64_t qa = smem_desc_sw128(smem_u32(sm.q[t][P - 1 - c][kk / 4]) + kk % 4 * 32, 16, 1024);
                         const uint64_t kb = smem_desc_sw128(smem_u32(sm.k[ks][kk / 4]) + kk % 4 * 32, 16, 1024);
                         mma_f16_ss(tmem + s_col(t), qa, kb, idesc_s, c > 0 || kk > 0);
                     }
@@ -186,7 +208,10 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(Kv8Attn p, int 
                 return true;
             };
             if (BESIDE<D, P>) ok = ok && scores(0);
+            const int run = run_of<P>(n_tiles);
+            int started = 0;  // the tile that O starts with
             for (int j = 0; ok && j < n_tiles; j++) {
+                if (j == started + run) started = j;
                 const int vs = j % S::VS;
                 if (!BESIDE<D, P>) ok = scores(j);
                 else if (j + 1 < n_tiles) ok = scores(j + 1);
@@ -199,7 +224,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(Kv8Attn p, int 
                     for (int kk = 0; kk < BN / 16; kk++) {
                         const uint64_t vb = smem_desc_sw128(smem_u32(sm.v[vs][kk / 4]) + kk % 4 * 32, 16, 1024);
                         const uint32_t pa = BESIDE<D, P> ? beside_col(t) + kk * 8 : s_col(t) + kk * 16 + c * 8;
-                        mma_f16_ts(tmem + o_col<D>(t), tmem + pa, vb, idesc_o, j > 0 || c > 0 || kk > 0);
+                        mma_f16_ts(tmem + o_col<D>(t), tmem + pa, vb, idesc_o, j > started || c > 0 || kk > 0);
                     }
                 mma_commit(&sm.pv_done[t]);
                 mma_commit(&sm.v_empty[vs]);
@@ -332,114 +357,162 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(Kv8Attn p, int 
             const uint32_t p_addr = tmem + lanes + beside_col(t) + half * 32;
             float m = -INFINITY, l = 0.f;
             uint32_t ref = 0x00800000u;  // bits of a power of two above every vs so far
-            for (int j = 0; j < n_tiles; j++) {
-                ok = ok && wait_for_warp(&sm.s_full[t], j & 1, err);
-                tc_fence_after();
-                const float4 sc01 = *reinterpret_cast<const float4*>(sm.scale[j & 3]);
-                const float4 sc23 = *reinterpret_cast<const float4*>(sm.scale[j & 3] + 2);
-                const uint32_t top_vs = max(max(__float_as_uint(sc01.y), __float_as_uint(sc01.w)),
-                                            max(__float_as_uint(sc23.y), __float_as_uint(sc23.w)));
-                const uint32_t top_ref = max(ref, (top_vs & 0x7f800000u) + 0x00800000u);
-                const float inv_ref = __uint_as_float(0x7f000000u - top_ref);
-                const float ks[MINE] = {half ? sc23.x : sc01.x, half ? sc23.z : sc01.z};
-                const float vs[MINE] = {half ? sc23.y : sc01.y, half ? sc23.w : sc01.w};
-                const int key0 = (blk0 + j * BLOCKS) * KV8_BLOCK;
-                const bool masked = key0 + BN > seen_by_all || key0 < first;
-                // scores in base-2 units, from column c of the thread's 64; -inf where a mask covers them
-                const auto scores = [&](auto& s, int c) {
-                    const float f = ks[c / KV8_BLOCK] * unit;
-                    constexpr int n = sizeof(s) / 4;
-#pragma unroll
-                    for (int e = 0; e < n; e += 2) {
-                        const float2 x = mul2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), make_float2(f, f));
-                        s[e] = __float_as_uint(x.x);
-                        s[e + 1] = __float_as_uint(x.y);
-                    }
-                    if (masked) {
-                        const int key = key0 + half * 64 + c;
-#pragma unroll
-                        for (int e = 0; e < n; e++)
-                            if (key + e >= lim || key + e < first) s[e] = __float_as_uint(-INFINITY);
-                    }
-                };
-                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int k = 0; k < MINE; k++) {
-                    uint32_t s[32];
-                    tmem_ld32(s_addr + k * 32, s);
-                    tmem_ld_wait();
-                    scores(s, k * 32);
-#pragma unroll
-                    for (int e = 0; e < 32; e += 8)
-#pragma unroll
-                        for (int c = 0; c < 4; c++)
-                            mx[c] = fmax3(mx[c], __uint_as_float(s[e + c]), __uint_as_float(s[e + 4 + c]));
-                }
-                float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                // (the next tile's S waits for both threads' P, so for both reads)
-                sm.part[t][half][r] = top;
-                ok = all_of(pair, 64, ok);
-                if (!ok) break;
-                top = fmaxf(top, sm.part[t][half ^ 1][r]);
-                const bool grow = top > m + kStale;  // from nothing, too
-                const float was = m;
-                if (grow) m = top;
-                const float base = m == -INFINITY ? 0.f : m;
-                const float alpha = grow ? exp2_approx(was - base) : 1.f;
-                const float keep = alpha * (__uint_as_float(ref) * inv_ref);
-                ref = top_ref;
-                // O is complete (and the last P read): S was computed after that PV, or waits for it here
-                if (BESIDE<D, P> && j > 0) {
-                    ok = wait_for_warp(&sm.pv_done[t], (j - 1) & 1, err);
+            const int run = run_of<P>(n_tiles);
+            float m_out = -INFINITY;  // the maximum that drained sums refer to
+            for (int j = 0, stop = min(run, n_tiles);; stop = min(stop + run, n_tiles)) {
+                for (; j < stop; j++) {
+                    ok = ok && wait_for_warp(&sm.s_full[t], j & 1, err);
                     tc_fence_after();
-                }
-                if (j > 0 && __any_sync(0xffffffffu, keep != 1.f)) {
+                    const float4 sc01 = *reinterpret_cast<const float4*>(sm.scale[j & 3]);
+                    const float4 sc23 = *reinterpret_cast<const float4*>(sm.scale[j & 3] + 2);
+                    const uint32_t top_vs = max(max(__float_as_uint(sc01.y), __float_as_uint(sc01.w)),
+                                                max(__float_as_uint(sc23.y), __float_as_uint(sc23.w)));
+                    const uint32_t top_ref = max(ref, (top_vs & 0x7f800000u) + 0x00800000u);
+                    const float inv_ref = __uint_as_float(0x7f000000u - top_ref);
+                    const float ks[MINE] = {half ? sc23.x : sc01.x, half ? sc23.z : sc01.z};
+                    const float vs[MINE] = {half ? sc23.y : sc01.y, half ? sc23.w : sc01.w};
+                    const int key0 = (blk0 + j * BLOCKS) * KV8_BLOCK;
+                    const bool masked = key0 + BN > seen_by_all || key0 < first;
+                    // scores in base-2 units, from column c of the thread's 64; -inf where a mask covers them
+                    const auto scores = [&](auto& s, int c) {
+                        const float f = ks[c / KV8_BLOCK] * unit;
+                        constexpr int n = sizeof(s) / 4;
 #pragma unroll
-                    for (int c = 0; c < D / 64; c++) {
-                        uint32_t o[32];
-                        tmem_ld32(o_addr + c * 32, o);
+                        for (int e = 0; e < n; e += 2) {
+                            const float2 x = mul2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), make_float2(f, f));
+                            s[e] = __float_as_uint(x.x);
+                            s[e + 1] = __float_as_uint(x.y);
+                        }
+                        if (masked) {
+                            const int key = key0 + half * 64 + c;
+#pragma unroll
+                            for (int e = 0; e < n; e++)
+                                if (key + e >= lim || key + e < first) s[e] = __float_as_uint(-INFINITY);
+                        }
+                    };
+                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int k = 0; k < MINE; k++) {
+                        uint32_t s[32];
+                        tmem_ld32(s_addr + k * 32, s);
                         tmem_ld_wait();
+                        scores(s, k * 32);
 #pragma unroll
-                        for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
-                        tmem_st32(o_addr + c * 32, o);
+                        for (int e = 0; e < 32; e += 8)
+#pragma unroll
+                            for (int c = 0; c < 4; c++)
+                                mx[c] = fmax3(mx[c], __uint_as_float(s[e + c]), __uint_as_float(s[e + 4 + c]));
                     }
-                }
-                const float2 nb = make_float2(-base, -base);
-                float2 sum = make_float2(0.f, 0.f);
-#pragma unroll
-                for (int c = 0; c < 64; c += 16) {
-                    const float u = vs[c / KV8_BLOCK] * inv_ref * kUnit;
-                    uint32_t s[16], w[8][P];
-                    tmem_ld16(s_addr + c, s);
-                    tmem_ld_wait();
-                    scores(s, c);
-#pragma unroll
-                    for (int e = 0; e < 16; e += 2) {
-                        float2 x = add2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), nb);
-                        x = make_float2(exp2_approx(x.x), exp2_approx(x.y));
-                        sum = add2(sum, x);
-                        x = mul2(x, make_float2(u, u));
-                        pieces_of<P>(x.x, x.y, w[e / 2]);
+                    float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                    // (the next tile's S waits for both threads' P, so for both reads)
+                    sm.part[t][half][r] = top;
+                    ok = all_of(pair, 64, ok);
+                    if (!ok) break;
+                    top = fmaxf(top, sm.part[t][half ^ 1][r]);
+                    const bool grow = top > m + kStale;  // from nothing, too
+                    const float was = m;
+                    if (grow) m = top;
+                    const float base = m == -INFINITY ? 0.f : m;
+                    const float alpha = grow ? exp2_approx(was - base) : 1.f;
+                    const float keep = alpha * (__uint_as_float(ref) * inv_ref);
+                    ref = top_ref;
+                    // O is complete (and the last P read): S was computed after that PV, or waits for it here
+                    if (BESIDE<D, P> && j > 0) {
+                        ok = wait_for_warp(&sm.pv_done[t], (j - 1) & 1, err);
+                        tc_fence_after();
                     }
-                    // over the same 16 keys' scores
+                    if (j > 0 && __any_sync(0xffffffffu, keep != 1.f)) {
 #pragma unroll
-                    for (int k = 0; k < P; k++) {
-                        uint32_t o[8];
+                        for (int c = 0; c < D / 64; c++) {
+                            uint32_t o[32];
+                            tmem_ld32(o_addr + c * 32, o);
+                            tmem_ld_wait();
 #pragma unroll
-                        for (int e = 0; e < 8; e++) o[e] = w[e][k];
-                        tmem_st8(BESIDE<D, P> ? p_addr + c / 2 : s_addr + c + k * 8, o);
+                            for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                            tmem_st32(o_addr + c * 32, o);
+                        }
                     }
-                }
-                if (BESIDE<D, P>) {  // S has been read
+                    const float2 nb = make_float2(-base, -base);
+                    float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+                    for (int c = 0; c < 64; c += 16) {
+                        const float u = vs[c / KV8_BLOCK] * inv_ref * kUnit;
+                        uint32_t s[16], w[8][P];
+                        tmem_ld16(s_addr + c, s);
+                        tmem_ld_wait();
+                        scores(s, c);
+#pragma unroll
+                        for (int e = 0; e < 16; e += 2) {
+                            float2 x = add2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), nb);
+                            x = make_float2(exp2_approx(x.x), exp2_approx(x.y));
+                            sum = add2(sum, x);
+                            x = mul2(x, make_float2(u, u));
+                            pieces_of<P>(x.x, x.y, w[e / 2]);
+                        }
+                        // over the same 16 keys' scores
+#pragma unroll
+                        for (int k = 0; k < P; k++) {
+                            uint32_t o[8];
+#pragma unroll
+                            for (int e = 0; e < 8; e++) o[e] = w[e][k];
+                            tmem_st8(BESIDE<D, P> ? p_addr + c / 2 : s_addr + c + k * 8, o);
+                        }
+                    }
+                    if (BESIDE<D, P>) {  // S has been read
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&sm.s_free[t]);
+                    }
+                    l = l * alpha + (sum.x + sum.y);
+                    tmem_st_wait();
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&sm.s_free[t]);
+                    if (lane == 0) mbar_arrive(&sm.p_full[t]);
                 }
-                l = l * alpha + (sum.x + sum.y);
-                tmem_st_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sm.p_full[t]);
+                if (P == 2 && ok && n_tiles > run) {
+                    // O's sums of the run: to where they wait, on top of those that wait there; the last run's O is
+                    // completed by them. They wait in their own columns, 16 at a time, of the tile's rows, 4 lanes to
+                    // 64 bytes of a row if all of the warp's rows are live (a thread finds its own again, in
+                    // whatever row), else each thread in its own.
+                    const bool spread = splits > 1 || live_rows == 0xffffffffu, whole = splits > 1 || (vec & 2), last = stop == n_tiles;
+                    float* at[4];
+#pragma unroll
+                    for (int u = 0; u < 4; u++) {
+                        const int rr = spread ? u * 8 + lane / 4 : lane, c = half * (D / 2) + (spread ? lane & 3 : u) * 4;
+                        const size_t off = __shfl_sync(0xffffffffu, i * p.out.ts + in_token, rr);
+                        at[u] = (splits > 1 ? p.ws + z + (((size_t)bh * gridDim.x + blockIdx.x) * 2 * BM + t * BM + quarter * 32 + rr) * (D + 4) + 4
+                                            : static_cast<float*>(const_cast<void*>(p.out.data)) + z + b * p.out.bs + off) + c;
+                    }
+                    const float old_f = m_out == m ? 1.f : exp2_approx(m_out - m);
+                    const float f = last ? 1.f : __uint_as_float(ref) * (1.f / kUnit), to_f = last ? __uint_as_float(0x7f000000u - ref) : 1.f;
+                    m_out = m;
+                    ok = wait_for_warp(&sm.pv_done[t], (stop - 1) & 1, err);
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int c = 0; c < D / 2; c += 16) {
+                        float4 had[4] = {};
+                        uint32_t o[16];
+                        if (stop > run && live) {
+#pragma unroll
+                            for (int u = 0; u < 4; u++) had[u] = had_at(at[u] + c, whole);
+                        }
+                        tmem_ld16(o_addr + c, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int u = 0; u < 4; u++) {
+                            const float4 y = summed(o + u * 4, f, had[u], to_f, last ? old_f * kUnit : old_f);
+                            o[u * 4] = __float_as_uint(y.x);
+                            o[u * 4 + 1] = __float_as_uint(y.y);
+                            o[u * 4 + 2] = __float_as_uint(y.z);
+                            o[u * 4 + 3] = __float_as_uint(y.w);
+                            if (ok && live && !last) store4(at[u] + c, y, 1.f, whole);
+                        }
+                        if (last) tmem_st16(o_addr + c, o);
+                    }
+                    tmem_st_wait();
+                    tc_fence_before();
+                }
+                if (!ok || stop == n_tiles) break;
             }
             // the rows' outputs, or their part of the keys' cuts: the two threads' sums, then O through the warp's
             // part of the queries' shared memory, 16 columns at a time, so that 4 lanes write 64 consecutive bytes
