@@ -10,7 +10,8 @@
 // where pairs are halves, both sides' pieces) of up to eight (four) heads of a token: they share its
 // table entries, its loads are whole 128-bit ones and all on their way before the first is used.
 // Rows that are not aligned for that, and rotated parts that do not divide into it, go one element
-// at a time.
+// at a time. 64 sequences x 256 tokens of 12 + 2 heads of d 128 in bf16 (117 MB in and out): 17.9 us,
+// 6.5 TB/s, what a copy gets (31 us an element at a time; 12.5 us out of L2, pairs of either kind); one token of 64 sequences: 1.6 us, a launch.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -117,6 +118,10 @@ __global__ void __launch_bounds__(N > 1 ? 256 : 1024) rope_kernel(RopeCall p, Di
             for (int j = 0; j < C; j++) {
                 if constexpr (sizeof(T) == 2 && ONE) {
                     *reinterpret_cast<__nv_bfloat162*>(&va[u].e[2 * j]) = __floats2bfloat162_rn(a[j], c[j]);
+                } else if constexpr (sizeof(T) == 2 && N > 1) {
+                    if (j % 2) continue;
+                    *reinterpret_cast<__nv_bfloat162*>(&va[u].e[j]) = __floats2bfloat162_rn(a[j], a[(j + 1) % C]);
+                    *reinterpret_cast<__nv_bfloat162*>(&vb[u].e[j]) = __floats2bfloat162_rn(c[j], c[(j + 1) % C]);
                 } else {
                     down(a[j], ONE ? va[u].e[(2 * j) % N] : va[u].e[j]);
                     down(c[j], ONE ? va[u].e[(2 * j + 1) % N] : vb[u].e[j]);
