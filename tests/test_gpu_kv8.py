@@ -382,6 +382,50 @@ def test_attention_sums_do_not_drift_with_the_keys(env, B, H, d, n, past, pad):
     ops.sync()
 
 
+@pytest.mark.parametrize("d,n", [(64, 17), (128, 17), (64, 43), (128, 43)])
+@pytest.mark.parametrize("mode", ["f32", "tf32", "bf16"])
+def test_attention_chunks_of_large_batches(env, d, n, mode):
+    """Batches large enough that 256 rows and 128 keys at a time are the faster way: ragged, padded, empty rows."""
+    torch, ops = env
+    rng = np.random.default_rng(d + n)
+    B, H = 96 if n < 40 else 48, 12
+    past = rng.integers(0, 300, B)
+    past[:3] = [0, 299, 128]
+    count = rng.integers(1, n + 1, B)
+    count[:4] = [n, n, 0, 1]
+    first = rng.integers(0, 40, B)
+    first[:5] = [0, 290, 0, 500, past[4] + n // 2]
+    cache, want = fill(torch, ops, rng, B, 2, d, 384, past + count)
+    check_attn(torch, ops, rng, cache, want, H, past, n, bf16=mode == "bf16", math="tf32" if mode == "tf32" else "f32",
+               count=count, first=first, max_past=299)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_nan_blocks_in_large_batches(env, d):
+    torch, ops = env
+    rng = np.random.default_rng(d)
+    B, n, H = 96, 17, 6
+    k, v = (normal(rng, B, 160, 1, d) for _ in range(2))
+    k[5, 40, 0, 3] = np.inf
+    v[7, 100, 0, 1] = np.nan
+    cache, want = ops.Kv8Cache.empty(B, 1, d, 192), O.Cache(B, 1, d, 192)
+    cache.append(up(torch, k), up(torch, v), 0)
+    q = normal(rng, B, n, H, d)
+    first = np.zeros(B, np.int64)
+    first[7] = 128  # behind the block of NaN
+    out = cache.attn(up(torch, q), 160 - n, first=i32(torch, first)).cpu().numpy()
+    assert np.isnan(out[5]).all()
+    others = np.arange(B) != 5
+    assert np.isfinite(out[others]).all()
+    k[5, 40, 0, 3] = 0
+    v[7, 100, 0, 1] = 0
+    want.append(k, v, [0] * B)
+    vals = want.values(np.float64)
+    exact, tol = O.attention(q, vals[0], vals[1], [160 - n] * B, None, first, 2, 2.0 ** -24)
+    assert (np.abs(out - exact) <= tol)[others].all()
+    ops.sync()
+
+
 def test_attention_sharp_and_flat_scores(env):
     """One key that takes all the weight, equal keys, zero queries, queries of very different sizes."""
     torch, ops = env

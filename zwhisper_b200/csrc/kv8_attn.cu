@@ -20,6 +20,7 @@
 // The splits of a (sequence, kv head, tile of query rows) that fit a cluster (8 CTAs) meet in each
 // other's shared memory; more of them write partials (m, l, O) for kv8_combine_kernel.
 #include <algorithm>
+#include <cmath>
 
 #include <cooperative_groups.h>
 
@@ -51,20 +52,20 @@ ZWG_DEV uint32_t transpose8x8(uint32_t x) {
     return y;
 }
 
-struct Plan {
-    int tiles;   // tiles of query rows of a (sequence, kv head)
-    int warps;   // of a CTA; 0: the tcgen05 kernel's
-    int splits;  // cuts of the keys
-    int most_splits;  // of this and of shorter caches: the workspace of a long cache serves shorter ones
-};
-
 constexpr int SMALL = 4;            // warps of a small CTA, three of which share an SM
 constexpr int MAX_CLUSTER = 8;
-constexpr int MOST_SPLIT_ROWS = 48;  // query rows of a kv head above which the tcgen05 kernel runs
+constexpr int MOST_SPLIT_ROWS = 48;  // query rows of a kv head above which the tcgen05 kernel may run
 constexpr int WARP_RING = 16 * 1024;  // bytes a warp has for blocks on their way
 
-// Rows of a tile: one or two 8-wide N tiles, or the tcgen05 kernel's.
-int tile_rows(int rows) { return rows <= 8 ? 8 : rows <= MOST_SPLIT_ROWS ? 16 : KV8_PREFILL_ROWS; }
+struct Plan {
+    int tile_rows, tiles;  // query rows of a tile, tiles of a (sequence, kv head)
+    int warps;   // of a CTA; 0: the tcgen05 kernel's
+    int splits;  // cuts of the keys
+    size_t ws;   // floats of workspace for this and shorter caches: a long cache's serves shorter ones
+    float us;    // about how long it takes, for a choice between the kernels
+    int in_place() const { return warps ? MAX_CLUSTER : 1; }  // cuts that need no workspace
+};
+
 // Warps of a CTA that has an SM to itself; the registers of two N tiles leave room for 8.
 constexpr int big_warps(int tile_rows) { return tile_rows == 8 ? 12 : 8; }
 
@@ -108,22 +109,39 @@ Cut cut_for(int tile_rows, bool big, long long ctas, int blocks, int combine_row
     return c;
 }
 
+size_t workspace_of(const Kv8& c, const Seqs& s, const Plan& p, int most_splits) {
+    if (most_splits <= p.in_place()) return 0;
+    return (size_t)s.n_batch * c.n_head_kv * p.tiles * most_splits * p.tile_rows * (c.d + 4);
+}
+
+// Blocks of keys that a query sees, on average.
+float blocks_seen(const Seqs& s) { return (s.n_past + 0.5f * s.n) / KV8_BLOCK + 1.f; }
+
+// The tcgen05 kernel: keys are cut while SMs stay empty, two tiles of keys to a cut at least.
+Plan plan_tc(const Kv8& c, const Seqs& s, int rows, int sm_count) {
+    Plan p{KV8_PREFILL_ROWS, (rows + KV8_PREFILL_ROWS - 1) / KV8_PREFILL_ROWS, 0, 1, 0, 0.f};
+    const long long ctas = (long long)s.n_batch * c.n_head_kv * p.tiles;
+    const int key_tiles = (s.n_past + s.n + KV8_PREFILL_KEYS - 1) / KV8_PREFILL_KEYS;
+    p.splits = (int)std::min<long long>(std::max<long long>(1, sm_count / ctas), std::max(1, key_tiles / 2));
+    p.ws = workspace_of(c, s, p, p.splits);
+    // a CTA's start and end and its key tiles, as measured with f32 queries; cuts go through memory twice
+    const float turns = std::ceil(blocks_seen(s) / (KV8_PREFILL_KEYS / KV8_BLOCK) / p.splits), two = rows > KV8_PREFILL_ROWS / 2;
+    const float cta = (two ? c.d == 64 ? 11.f : 13.f : c.d == 64 ? 8.5f : 9.5f) + turns * (two ? c.d == 64 ? 4.6f : 5.3f : c.d == 64 ? 3.f : 3.5f);
+    p.us = (float)((ctas * p.splits + sm_count - 1) / sm_count) * cta;
+    if (p.splits > 1) p.us += 3.f + 5.f * rows * s.n_batch * c.n_head_kv * p.splits * (c.d + 4) / 3e6f;
+    return p;
+}
+
 // Splits of small CTAs with one block for each warp.
 int one_each(int blocks) { return (blocks + SMALL - 1) / SMALL; }
 
-Plan plan_for(const Kv8& c, const Seqs& s, int n_head, int sm_count) {
-    const int rows = s.n * (n_head / c.n_head_kv), big = big_warps(tile_rows(rows));
-    Plan p;
-    p.tiles = (rows + tile_rows(rows) - 1) / tile_rows(rows);
+Plan plan_split(const Kv8& c, const Seqs& s, int rows, int n_head, int sm_count) {
+    Plan p{};
+    p.tile_rows = rows <= 8 ? 8 : 16;  // one or two 8-wide N tiles
+    p.tiles = (rows + p.tile_rows - 1) / p.tile_rows;
+    const int big = big_warps(p.tile_rows);
     const long long ctas = (long long)s.n_batch * c.n_head_kv * p.tiles;
     const int blocks = (s.n_past + s.n + KV8_BLOCK - 1) / KV8_BLOCK;
-    if (rows > MOST_SPLIT_ROWS) {
-        // keys are cut while SMs stay empty, two tiles of keys to a cut at least
-        const int key_tiles = (blocks * KV8_BLOCK + KV8_PREFILL_KEYS - 1) / KV8_PREFILL_KEYS;
-        p.warps = 0;
-        p.splits = p.most_splits = (int)std::min<long long>(std::max<long long>(1, sm_count / ctas), std::max(1, key_tiles / 2));
-        return p;
-    }
     const int combine_rows = (int)std::min<long long>((long long)s.n_batch * s.n * n_head, 8 * sm_count);
     // most CTAs for which one block to each warp of small CTAs was the fastest plan: half the SMs
     const int few = (int)(sm_count / 2 / ctas);
@@ -132,24 +150,42 @@ Plan plan_for(const Kv8& c, const Seqs& s, int n_head, int sm_count) {
         // no cut: merging two CTAs takes longer than a second block to each warp
         p.warps = blocks <= SMALL ? SMALL : big;
         p.splits = 1;
-    } else if (one_each(blocks) <= few || (one_each(blocks) <= MAX_CLUSTER && ctas <= clusters_at_once(tile_rows(rows), false, one_each(blocks)))) {
+    } else if (one_each(blocks) <= few || (one_each(blocks) <= MAX_CLUSTER && ctas <= clusters_at_once(p.tile_rows, false, one_each(blocks)))) {
         p.warps = SMALL;
         p.splits = one_each(blocks);
     } else {
         // big CTAs (fewer states to merge) unless small ones leave fewer places empty
-        const Cut small = cut_for(tile_rows(rows), false, ctas, blocks, combine_rows, sm_count);
-        const Cut large = cut_for(tile_rows(rows), true, ctas, blocks, combine_rows, sm_count);
+        const Cut small = cut_for(p.tile_rows, false, ctas, blocks, combine_rows, sm_count);
+        const Cut large = cut_for(p.tile_rows, true, ctas, blocks, combine_rows, sm_count);
         const bool use_big = ctas <= sm_count && large.cost <= small.cost;
         p.warps = use_big ? big : SMALL;
         p.splits = use_big ? large.splits : small.splits;
         // big CTAs in clusters that put as many warps to work cost no more with any cache
-        const int in_cluster = cut_for(tile_rows(rows), true, ctas, big * MAX_CLUSTER, combine_rows, sm_count).splits;
-        const int small_most = cut_for(tile_rows(rows), false, ctas, 1 << 20, combine_rows, sm_count).most_splits;
+        const int in_cluster = cut_for(p.tile_rows, true, ctas, big * MAX_CLUSTER, combine_rows, sm_count).splits;
+        const int small_most = cut_for(p.tile_rows, false, ctas, 1 << 20, combine_rows, sm_count).most_splits;
         const bool always_big = ctas <= sm_count && large.most_splits <= MAX_CLUSTER && in_cluster * big >= small_most * SMALL;
         most = always_big ? 1 : std::max(large.most_splits, small.most_splits);
     }
-    p.most_splits = std::max(most, std::max(p.splits, std::min(few, one_each(blocks))));
+    p.ws = workspace_of(c, s, p, std::max(most, std::max(p.splits, std::min(few, one_each(blocks)))));
+    // waves of CTAs, each with its start, its merge and the blocks that follow each other in a warp
+    const float turns = std::ceil(blocks_seen(s) / (p.splits * p.warps)), d64 = c.d == 64;
+    const float waves = (float)(ctas * p.splits) / (sm_count * (big / p.warps)), whole = std::floor(waves);
+    p.us = std::max(1.f, whole == waves ? waves : whole + 0.5f + 0.5f * (waves - whole)) * (d64 ? 3.5f + 1.2f * turns : 4.5f + 1.9f * turns);
+    if (p.splits > MAX_CLUSTER) p.us += 2.f;
     return p;
+}
+
+// The tcgen05 kernel has four times the other one's rate, but 10 us of start and end for a CTA of 256 rows and
+// 128 keys at a time. Up to 48 rows the other one was faster everywhere; above, the shorter estimate: 8 sequences
+// of 2000 tokens, d 128, 288 rows a head 39.3 us against 47.5, 1536 rows 208 against 97.5; a prompt's first 256
+// tokens (1536 rows) of one sequence 9.2 against 23.6, of 64 sequences 314 against 138.
+Plan plan_for(const Kv8& c, const Seqs& s, int n_head, int sm_count) {
+    const int rows = s.n * (n_head / c.n_head_kv);
+    Plan split = plan_split(c, s, rows, n_head, sm_count);
+    if (rows <= MOST_SPLIT_ROWS) return split;
+    Plan tc = plan_tc(c, s, rows, sm_count);
+    split.ws = tc.ws = std::max(split.ws, tc.ws);
+    return split.us < tc.us ? split : tc;
 }
 
 // What each of n softmax states (m, l) weighs in their sum: f[i] = 2^(m_i - max), and the sum of l f.
@@ -602,6 +638,38 @@ int clusters_of(int tile_rows, bool big, int n) {
     return big ? clusters_of_kind<2, big_warps(16)>(n) : clusters_of_kind<2, SMALL>(n);
 }
 
+// The same where rows are many: D / 4 threads take a row.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) kv8_combine_rows_kernel(Kv8Attn p, int splits, int R, int vec) {
+    chain_release();
+    const int z = chain_wait();
+    constexpr int GROUPS = 256 / (D / 4);
+    const int bh = blockIdx.y, b = bh / p.c.n_head_kv, h = bh - b * p.c.n_head_kv;
+    const int group = p.n_head / p.c.n_head_kv, row = blockIdx.x * GROUPS + threadIdx.x / (D / 4), c = threadIdx.x % (D / 4);
+    const Place at = place_of(p.s, b, p.c.blocks * KV8_BLOCK, nullptr);
+    if (row >= at.count * group || (p.s.first && __ldcg(p.s.first + b + z) < 0)) return;
+    const int tiles = (p.s.n * group + R - 1) / R;
+    const size_t step = (size_t)R * (D + 4);
+    const float* ws = p.ws + z + ((size_t)bh * tiles + row / R) * splits * step + (row % R) * (D + 4);
+    float mx = -INFINITY;
+#pragma unroll 8
+    for (int s = 0; s < splits; s++) mx = fmaxf(mx, __ldcg(ws + s * step));
+    const float base = mx == -INFINITY ? 0.f : mx;
+    float sum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int s = 0; s < splits; s++) {
+        const float2 ml = __ldcg(reinterpret_cast<const float2*>(ws + s * step));
+        const float f = exp2_approx(ml.x - base);
+        sum += ml.y * f;
+        add4(acc, f, __ldcg(reinterpret_cast<const float4*>(ws + s * step + 4) + c));
+    }
+    const int i = row / group;
+    T* out = static_cast<T*>(const_cast<void*>(p.out.data)) + z + b * p.out.bs + i * p.out.ts +
+             (size_t)(h * group + row - i * group) * D + c * 4;
+    store4(out, acc, sum == 0.f ? 0.f : 1.f / sum, vec & 2);
+}
+
 template <typename T, int D, int NT, int P, int WARPS>
 int split_launch(const Kv8Attn& p, const Plan& plan, int vec, cudaStream_t st) {
     constexpr int RING = WARPS * WARP_RING;
@@ -634,18 +702,25 @@ int split_of(const Kv8Attn& p, const Plan& plan, int vec, cudaStream_t st) {
 }
 
 template <typename T, int D>
-int combine(const Kv8Attn& p, const Plan& plan, int rows, int tile_rows, int vec, cudaStream_t st) {
-    return launch_chained_smem(kv8_combine_kernel<T, D>, dim3((unsigned)rows, (unsigned)(p.s.n_batch * p.c.n_head_kv)), dim3(256),
-                               plan.splits * sizeof(float), st, p, plan.splits, tile_rows, vec) == cudaSuccess
-               ? 0
-               : -1;
+int combine(const Kv8Attn& p, const Plan& plan, int rows, int vec, int sm_count, cudaStream_t st) {
+    const unsigned segs = (unsigned)(p.s.n_batch * p.c.n_head_kv);
+    cudaError_t e;
+    if ((long long)rows * segs > 8 * sm_count) {  // more than a CTA to a row fits at once
+        constexpr int GROUPS = 256 / (D / 4);
+        e = launch_chained(kv8_combine_rows_kernel<T, D>, dim3((unsigned)(rows + GROUPS - 1) / GROUPS, segs), dim3(256), st, p,
+                           plan.splits, plan.tile_rows, vec);
+    } else {
+        e = launch_chained_smem(kv8_combine_kernel<T, D>, dim3((unsigned)rows, segs), dim3(256), plan.splits * sizeof(float), st, p,
+                                plan.splits, plan.tile_rows, vec);
+    }
+    return e == cudaSuccess ? 0 : -1;
 }
 
 template <typename T, int D>
 int attn(const Kv8Attn& p, int pieces, int sm_count, cudaStream_t st) {
     const Plan plan = plan_for(p.c, p.s, p.n_head, sm_count);
-    const int rows = p.s.n * (p.n_head / p.c.n_head_kv), per_tile = tile_rows(rows);
-    const bool one = per_tile == 8, two_pieces = sizeof(T) == 4 && pieces == 2;  // bf16 queries are exact in one piece
+    const int rows = p.s.n * (p.n_head / p.c.n_head_kv);
+    const bool one = plan.tile_rows == 8, two_pieces = sizeof(T) == 4 && pieces == 2;  // bf16 queries are exact in one piece
     const int vec = (wide(p.q, sizeof(T), 16) ? 1 : 0) | (wide(p.out, sizeof(T), 4 * sizeof(T)) ? 2 : 0);
     int rc;
     if (plan.warps == 0) {
@@ -655,7 +730,7 @@ int attn(const Kv8Attn& p, int pieces, int sm_count, cudaStream_t st) {
     } else {
         rc = one ? split_of<T, D, 1, 1>(p, plan, vec, st) : split_of<T, D, 2, 1>(p, plan, vec, st);
     }
-    if (rc == 0 && plan.splits > (plan.warps ? MAX_CLUSTER : 1)) rc = combine<T, D>(p, plan, rows, per_tile, vec, st);
+    if (rc == 0 && plan.splits > plan.in_place()) rc = combine<T, D>(p, plan, rows, vec, sm_count, st);
     return rc;
 }
 
@@ -663,10 +738,7 @@ int attn(const Kv8Attn& p, int pieces, int sm_count, cudaStream_t st) {
 
 size_t kv8_attn_workspace_bytes(const Kv8& c, const Seqs& s, int n_head, int sm_count) {
     if (s.n_batch == 0 || s.n == 0) return 0;
-    const Plan p = plan_for(c, s, n_head, sm_count);
-    const int rows = s.n * (n_head / c.n_head_kv);
-    if (p.most_splits <= (p.warps ? MAX_CLUSTER : 1)) return 0;
-    return (size_t)s.n_batch * c.n_head_kv * p.tiles * p.most_splits * tile_rows(rows) * (c.d + 4) * sizeof(float);
+    return plan_for(c, s, n_head, sm_count).ws * sizeof(float);
 }
 
 int kv8_attn_launch(const Kv8Attn& p, int type, int pieces, int sm_count, cudaStream_t st) {
