@@ -1,7 +1,7 @@
 // C-ABI entry points of the decode step over a cache in 8 bits (include/zwgpu.h): zwg_rope,
 // zwg_kv8_append / _read / _attn, zwg_llm_logits, and the states that keep such caches. Every
-// call checks its arguments, before it asks for a context, then launches on the caller's stream: no allocation (but for a
-// state's creation), no synchronization.
+// call checks its arguments, before it asks for a context, then launches on the caller's stream:
+// no allocation (but for a state's creation), no synchronization.
 #include <cuda_runtime.h>
 
 #include <cmath>

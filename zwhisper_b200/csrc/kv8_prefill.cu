@@ -16,8 +16,14 @@
 // there is room (not beside two pieces of d 128).
 // O is rescaled in TMEM only where a row's maximum grows by more than 2^4 or the values' scale does:
 // probabilities stay below 2^4 and P's pieces hold 2^11 p.
-// Bound by the exponentials and the softmax's instructions (one piece), by them and the tensor cores
-// alike (two pieces double the products).
+//
+// 32 sequences x 256 tokens after 1744, 12 / 2 heads of d 128: 310 us in f32 (the products alone, of two
+// pieces, take 113 us at the rate of large library products), 218 us in bf16 (57); 16 x 250 after 1750,
+// 14 / 2 heads of d 64, bf16: 109 us. Bound by the latency of a tile's chain (S, its maximum, P, P V) over only
+// two tiles at a time: with an eighth of the products 208 us (f32, before its drains: 261), without exponentials
+// 252, without converting K and V 261. Tile 1 starts a softmax behind tile 0, so that the one's products run
+// during the other's exponentials (294 us side by side). One key and two value buffers: 278 us. CTAs of 256 rows
+// also leave SMs empty at the end: 384 CTAs on 148 SMs are 2.6 waves.
 #include <algorithm>
 
 #include "chain.cuh"
@@ -51,9 +57,9 @@ __host__ __device__ constexpr uint32_t o_col(int t) { return 256u + t * D; }
 // The tensor cores truncate their sums, 2 x 128 / 16 of them to a key tile, which shrinks O by 2e-9 of it
 // for each key: 1.6e-5 after 8000 keys. So where two pieces ask for f32's accuracy, the sums of MOST_RUN
 // tiles at the most are drained into f32 sums that wait in the output's own place. 32 x 256 tokens after 1744
-// at d 128: 261 us and off by 4.1e-6 without, 288 us and 1.9e-6 in runs of 8, 300 us and 1.35e-6 of 6;
-// 1.5e-6 at any length. (The small query pieces go first for the same reason: 3e-7 less.)
-constexpr int MOST_RUN = 6;
+// at d 128: 261 us and off by 4.1e-6 without, 288 us and 1.9e-6 in runs of 8, 300 us and 1.35e-6 of 6, 310 us
+// and 1.2e-6 of 5, at any length (the f32 library form of the same sums: 1.2e-6). (The small query pieces go first for the same reason: 3e-7 less.)
+constexpr int MOST_RUN = 5;
 // Key tiles from one drain to the next, of n in all.
 template <int P>
 ZWG_DEV int run_of(int n) {
@@ -469,7 +475,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(Kv8Attn p, int 
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sm.p_full[t]);
                 }
-                if (P == 2 && ok && n_tiles > run) {
+                if (!ok) break;  // both threads of a row know
+                if (P == 2 && n_tiles > run) {
                     // O's sums of the run: to where they wait, on top of those that wait there; the last run's O is
                     // completed by them. They wait in their own columns, 16 at a time, of the tile's rows, 4 lanes to
                     // 64 bytes of a row if all of the warp's rows are live (a thread finds its own again, in
@@ -512,7 +519,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(Kv8Attn p, int 
                     tmem_st_wait();
                     tc_fence_before();
                 }
-                if (!ok || stop == n_tiles) break;
+                if (stop == n_tiles) break;  // (a wait that gave up here is known to both after the next exchange)
             }
             // the rows' outputs, or their part of the keys' cuts: the two threads' sums, then O through the warp's
             // part of the queries' shared memory, 16 columns at a time, so that 4 lanes write 64 consecutive bytes
