@@ -11,7 +11,8 @@
 // table entries, its loads are whole 128-bit ones and all on their way before the first is used.
 // Rows that are not aligned for that, and rotated parts that do not divide into it, go one element
 // at a time. 64 sequences x 256 tokens of 12 + 2 heads of d 128 in bf16 (117 MB in and out): 17.9 us,
-// 6.5 TB/s, what a copy gets (31 us an element at a time; 12.5 us out of L2, pairs of either kind); one token of 64 sequences: 1.6 us, a launch.
+// 6.5 TB/s, what a copy gets (31 us an element at a time; 12.5 us out of L2, pairs of either kind); one
+// token of 16 sequences: 1.6 us, a launch.
 #include <cuda_bf16.h>
 
 #include <algorithm>
