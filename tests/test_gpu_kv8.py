@@ -566,6 +566,41 @@ def test_attention_strides_streams_and_graphs(env):
     ops.sync()
 
 
+@pytest.mark.parametrize("B,n,past,kv", [(40, 150, 2000, 1), (8, 96, 2000, 2), (1, 64, 4000, 1), (2, 1, 9000, 1)])
+def test_attention_chunks_captured_and_on_another_stream(env, B, n, past, kv):
+    """Calls that drain sums, cut keys into a workspace or join many partials: a replayed graph, another stream and
+    a second replay give what the plain call gave, bit for bit; the graph follows positions on the device."""
+    torch, ops = env
+    d, H = 64, 6 * kv
+    n_ctx = (past + n + 63) // 32 * 32
+    g = torch.Generator(device="cuda:0").manual_seed(B)
+    rows = lambda heads, tokens: torch.randn(B, tokens, heads, d, device="cuda:0", generator=g)
+    cache = ops.Kv8Cache.empty(B, kv, d, n_ctx)
+    cache.append(rows(kv, past + n), rows(kv, past + n), 0)
+    q = rows(H, n)
+    at = torch.full((B,), past, dtype=torch.int32, device="cuda:0")
+    want = cache.attn(q, at, max_past=past)
+    short = cache.attn(q, at - 77, max_past=past)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = cache.attn(q, at, max_past=past)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(other, want)
+    out = torch.zeros_like(q)
+    ws = torch.empty(max(1, cache.attn_workspace_bytes(n, H, n_past=past)), dtype=torch.uint8, device="cuda:0")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.attn(q, at, max_past=past, out=out, workspace=ws)
+    for shift, expect in ((0, want), (77, short), (0, want)):
+        at.fill_(past - shift)
+        out.fill_(5.0)
+        graph.replay()
+        assert torch.equal(out, expect)
+    ops.sync()
+
+
 def test_attention_is_the_same_every_time(env):
     torch, ops = env
     rng = np.random.default_rng(9)
