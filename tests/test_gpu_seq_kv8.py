@@ -639,6 +639,18 @@ def test_python_refusals(env):
     ops.sync()
 
 
+def test_workspace_elsewhere_is_refused(env):
+    torch, ops = env
+    cache = ops.Kv8Cache.empty(1, 1, 64, 32768)
+    q = torch.zeros(1, 1, 4, 64, device="cuda:0")
+    size = cache.attn_workspace_bytes(1, 4, n_past=32000)
+    assert size > 0
+    for ws in (torch.empty(size, dtype=torch.uint8), torch.empty(2 * size, dtype=torch.uint8, device="cuda:0")[::2]):
+        with pytest.raises(ValueError):
+            cache.attn(q, 32000, workspace=ws)
+    ops.sync()
+
+
 # ---- the states that keep such caches ----------------------------------------------------
 
 @pytest.mark.parametrize("d,B,math", [(64, 2, "f32"), (128, 1, "f32"), (64, 2, "tf32")])

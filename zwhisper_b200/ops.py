@@ -1034,7 +1034,8 @@ class Kv8Cache:
         (an int, or a CUDA int32 tensor [n_batch] whose entries are at most max_past) over the
         cache, which holds the call's own tokens already: query i of sequence b sees keys
         first[b] .. n_past + i. count, first: CUDA int32 [n_batch]; rows of out behind count[b]
-        stay as they are. Returns out, of q's shape and type (a new one has zeros there)."""
+        stay as they are. workspace: a contiguous CUDA tensor of attn_workspace_bytes (None: one is
+        made). Returns out, of q's shape and type (a new one has zeros there)."""
         torch = _torch()
         kind = _row_type(q, "q")
         if q.dim() != 4:
@@ -1057,6 +1058,8 @@ class Kv8Cache:
                 workspace = torch.empty(size, dtype=torch.uint8, device=dev)
                 ws = workspace.data_ptr()
         else:
+            if workspace.device != dev or not workspace.is_contiguous():
+                raise ValueError(f"workspace must be a contiguous tensor on {dev}")
             ws, size = workspace.data_ptr(), workspace.numel() * workspace.element_size()
         _lib.check(lib.zwg_kv8_attn(self._ref, s, kind, H, qr, o, ws, size, _stream_on(dev)))
         return out
