@@ -76,6 +76,7 @@ struct Smem {
     float2 scale[4][BLOCKS];             // (ks, vs) of a tile's blocks: a tile's are read until its P is there
     float part[2][2][BM];                // what a row's two threads tell each other: [query tile][half]
     uint64_t q_full[2], k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], s_full[2], s_free[2], p_full[2], pv_done[2], drained[2];
+    uint64_t started;  // tile 0's first P is there
     uint32_t tmem_base;
 };
 
@@ -174,6 +175,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(Kv8Attn p, int 
             mbar_init(&sm.v_full[i], CONVERTERS / 32);
             mbar_init(&sm.v_empty[i], n_t);
         }
+        mbar_init(&sm.started, 1);
         fence_mbar_init();
     }
     if (warp == ISSUER) {
@@ -193,7 +195,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(Kv8Attn p, int 
             constexpr uint32_t idesc_o = idesc_f16(BM, D, false, false, false);
             bool ok = wait_for(&sm.q_full[t], 0, err);
             // tile 1 starts a softmax behind tile 0, so that the one's exponentials run during the other's products
-            if (t == 1) ok = ok && wait_for(&sm.p_full[0], 0, err);
+            // (a barrier of its own: p_full's phases go on, and one that is two ahead looks like none)
+            if (t == 1) ok = ok && wait_for(&sm.started, 0, err);
             const auto scores = [&](int j) {
                 const int ks = j % S::KS;
                 if (!wait_for(&sm.k_full[ks], j / S::KS & 1, err)) return false;
@@ -222,6 +225,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(Kv8Attn p, int 
                 if (!BESIDE<D, P>) ok = scores(j);
                 else if (j + 1 < n_tiles) ok = scores(j + 1);
                 if (!ok || !(ok = wait_for(&sm.p_full[t], j & 1, err))) break;
+                if (t == 0 && j == 0) mbar_arrive(&sm.started);
                 if (!(ok = wait_for(&sm.v_full[vs], j / S::VS & 1, err))) break;
                 tc_fence_after();
 #pragma unroll
