@@ -143,7 +143,7 @@ def test_the_kernel_waits_once_only_on_barriers_that_complete_once():
     with open(os.path.join(ROOT, "zwhisper_b200", "csrc", "kv8_prefill.cu")) as f:
         code = f.read()
     once, many = set(), set()
-    for call in re.findall(r"(?:wait_for|wait_for_warp|mbar_wait_drain)\((.*?)\)", code):
+    for call in re.findall(r"mbar_wait(?:_warp|_drain)?\((.*?)\)", code):
         names = re.findall(r"&sm\.(\w+)", call)
         assert names, call
         parity = re.sub(r".*\]|.*&sm\.\w+", "", call.split("err")[0]).strip(" ,")

@@ -11,15 +11,19 @@ namespace zwg {
 enum : int {
     kErrNone = 0,
     kErrTimeout = 1,   // a bounded wait ran out
-    kErrBounds = 2,    // a checked index was out of range (ZWG_CHECK builds)
+    kErrBounds = 2,    // an entry or index was out of range, and what it stands for was left out
 };
 
 // Iteration limit for every spin-wait on an mbarrier. With the back-off below this is
 // several seconds, far above any legitimate wait in these kernels.
 constexpr uint32_t kSpinLimit = 1u << 26;
 
+// The first error stays, but for a timeout, which takes any other's place: it means results that are
+// not there, and tells the waits of other CTAs to give up.
 ZWG_DEV void set_error(int* err, int code) {
-    if (err) atomicCAS(err, 0, code);
+    if (!err) return;
+    if (code == kErrTimeout) atomicExch(err, code);
+    else atomicCAS(err, 0, code);
 }
 
 // Online-softmax helpers -----------------------------------------------------------------

@@ -364,7 +364,7 @@ __global__ void __launch_bounds__(32 * WARPS)
             ks = vs;
             vs = 0.f;
         }
-        if (!wait_for_warp(&full[warp][stage], phase, p.err)) {
+        if (!sm100::mbar_wait_warp(&full[warp][stage], phase, p.err)) {
             // gave up: no further copies; those on their way end before the ring is used again
             for (int s = 0; s < STAGES && blk + s * WARPS < to; s++) {
                 const int at_stage = (stage + s) % STAGES;

@@ -11,23 +11,6 @@
 namespace zwg {
 namespace kv8 {
 
-// sm100::mbar_wait, but a wait that has run out elsewhere is the only error that ends it early: an entry
-// of past, count or first that is out of range is an error too, and leaves the other sequences alone.
-ZWG_DEV bool wait_for(uint64_t* bar, uint32_t parity, int* err) {
-    for (uint32_t i = 0; i < (1u << 22); i++) {
-        if (sm100::mbar_try_wait(bar, parity)) return true;
-        if (i >= 4096) {
-            __nanosleep(1000);
-            if ((i & 1023) == 0 && err && *(volatile int*)err == kErrTimeout) return false;
-        }
-    }
-    set_error(err, kErrTimeout);
-    return false;
-}
-ZWG_DEV bool wait_for_warp(uint64_t* bar, uint32_t parity, int* err) {
-    return __all_sync(0xffffffffu, wait_for(bar, parity, err));
-}
-
 constexpr float kLog2e = 1.4426950408889634f;
 
 ZWG_DEV uint32_t h2u(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }

@@ -193,15 +193,15 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(Kv8Attn p, int 
         if (t < n_t && lane == 0 && n_tiles > 0) {
             constexpr uint32_t idesc_s = idesc_f16(BM, BN, false, false, false);
             constexpr uint32_t idesc_o = idesc_f16(BM, D, false, false, false);
-            bool ok = wait_for(&sm.q_full[t], 0, err);
+            bool ok = mbar_wait(&sm.q_full[t], 0, err);
             // tile 1 starts a softmax behind tile 0, so that the one's exponentials run during the other's products
             // (a barrier of its own: p_full's phases go on, and one that is two ahead looks like none)
-            if (t == 1) ok = ok && wait_for(&sm.started, 0, err);
+            if (t == 1) ok = ok && mbar_wait(&sm.started, 0, err);
             const auto scores = [&](int j) {
                 const int ks = j % S::KS;
-                if (!wait_for(&sm.k_full[ks], j / S::KS & 1, err)) return false;
+                if (!mbar_wait(&sm.k_full[ks], j / S::KS & 1, err)) return false;
                 // S goes where the last S was read from, or its P, which the PV reads
-                if (j > 0 && !wait_for(BESIDE<D, P> ? &sm.s_free[t] : &sm.pv_done[t], (j - 1) & 1, err)) return false;
+                if (j > 0 && !mbar_wait(BESIDE<D, P> ? &sm.s_free[t] : &sm.pv_done[t], (j - 1) & 1, err)) return false;
                 tc_fence_after();
 #pragma unroll
                 for (int c = 0; c < P; c++)
@@ -224,9 +224,9 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(Kv8Attn p, int 
                 const int vs = j % S::VS;
                 if (!BESIDE<D, P>) ok = scores(j);
                 else if (j + 1 < n_tiles) ok = scores(j + 1);
-                if (!ok || !(ok = wait_for(&sm.p_full[t], j & 1, err))) break;
+                if (!ok || !(ok = mbar_wait(&sm.p_full[t], j & 1, err))) break;
                 if (t == 0 && j == 0) mbar_arrive(&sm.started);
-                if (!(ok = wait_for(&sm.v_full[vs], j / S::VS & 1, err))) break;
+                if (!(ok = mbar_wait(&sm.v_full[vs], j / S::VS & 1, err))) break;
                 tc_fence_after();
 #pragma unroll
                 for (int c = 0; c < P; c++)
@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(Kv8Attn p, int 
         }
         for (int j = 0; j < n_tiles; j++) {
             const int ks = j % S::KS, vs = j % S::VS;
-            if (j >= S::KS && !wait_for_warp(&sm.k_empty[ks], (j / S::KS - 1) & 1, err)) break;
+            if (j >= S::KS && !mbar_wait_warp(&sm.k_empty[ks], (j / S::KS - 1) & 1, err)) break;
 #pragma unroll
             for (int i = 0; i < N; i++) {
                 const int e = tid + i * CONVERTERS, r = e / SEGS, seg = e % SEGS;
@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(Kv8Attn p, int 
             __syncwarp();
             if (lane == 0) mbar_arrive(&sm.k_full[ks]);
             if (j + 1 < n_tiles) load_k(j + 1);
-            if (j >= S::VS && !wait_for_warp(&sm.v_empty[vs], (j / S::VS - 1) & 1, err)) break;
+            if (j >= S::VS && !mbar_wait_warp(&sm.v_empty[vs], (j / S::VS - 1) & 1, err)) break;
 #pragma unroll
             for (int i = 0; i < N; i++) {
                 const int e = tid + i * CONVERTERS, blk = e / (D * 2), r = e / 2 % D;
@@ -371,7 +371,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(Kv8Attn p, int 
             float m_out = -INFINITY;  // the maximum that drained sums refer to
             for (int j = 0, stop = min(run, n_tiles);; stop = min(stop + run, n_tiles)) {
                 for (; j < stop; j++) {
-                    ok = ok && wait_for_warp(&sm.s_full[t], j & 1, err);
+                    ok = ok && mbar_wait_warp(&sm.s_full[t], j & 1, err);
                     tc_fence_after();
                     const float4 sc01 = *reinterpret_cast<const float4*>(sm.scale[j & 3]);
                     const float4 sc23 = *reinterpret_cast<const float4*>(sm.scale[j & 3] + 2);
@@ -428,7 +428,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(Kv8Attn p, int 
                     ref = top_ref;
                     // O is complete (and the last P read): S was computed after that PV, or waits for it here
                     if (BESIDE<D, P> && j > 0) {
-                        ok = wait_for_warp(&sm.pv_done[t], (j - 1) & 1, err);
+                        ok = mbar_wait_warp(&sm.pv_done[t], (j - 1) & 1, err);
                         tc_fence_after();
                     }
                     if (j > 0 && __any_sync(0xffffffffu, keep != 1.f)) {
@@ -497,7 +497,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(Kv8Attn p, int 
                     const float old_f = m_out == m ? 1.f : exp2_approx(m_out - m);
                     const float f = last ? 1.f : __uint_as_float(ref) * (1.f / kUnit), to_f = last ? __uint_as_float(0x7f000000u - ref) : 1.f;
                     m_out = m;
-                    ok = wait_for_warp(&sm.pv_done[t], (stop - 1) & 1, err);
+                    ok = mbar_wait_warp(&sm.pv_done[t], (stop - 1) & 1, err);
                     tc_fence_after();
 #pragma unroll 1
                     for (int c = 0; c < D / 2; c += 16) {
@@ -528,7 +528,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(Kv8Attn p, int 
             // the rows' outputs, or their part of the keys' cuts: the two threads' sums, then O through the warp's
             // part of the queries' shared memory, 16 columns at a time, so that 4 lanes write 64 consecutive bytes
             // (of f32) of a row
-            if (ok && n_tiles > 0) ok = wait_for_warp(&sm.pv_done[t], (n_tiles - 1) & 1, err);
+            if (ok && n_tiles > 0) ok = mbar_wait_warp(&sm.pv_done[t], (n_tiles - 1) & 1, err);
             tc_fence_after();
             sm.part[t][half][r] = l;
             ok = all_of(pair, 64, ok);

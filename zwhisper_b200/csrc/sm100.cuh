@@ -44,14 +44,15 @@ ZWG_DEV bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
 // Bounded wait for the phase with the given parity to complete. Gives up after a few
 // seconds, records kErrTimeout in the error word and returns false; callers then skip
 // to the kernel's teardown instead of waiting forever.
-// A wait also gives up early once any other CTA has recorded an error, so one failure
-// cannot make every later CTA of the grid sit out its own full timeout.
+// A wait also gives up early once any other CTA's has run out, so one failure cannot make
+// every later CTA of the grid sit out its own full timeout. Other errors do not end it: an
+// entry out of range is left out, and the rest of the work is valid.
 ZWG_DEV bool mbar_wait(uint64_t* bar, uint32_t parity, int* err) {
     for (uint32_t i = 0; i < (1u << 22); i++) {
         if (mbar_try_wait(bar, parity)) return true;
         if (i >= 4096) {
             __nanosleep(1000);
-            if ((i & 1023) == 0 && err && *(volatile int*)err != 0) return false;
+            if ((i & 1023) == 0 && err && *(volatile int*)err == kErrTimeout) return false;
         }
     }
     set_error(err, kErrTimeout);
