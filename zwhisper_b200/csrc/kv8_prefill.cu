@@ -373,16 +373,22 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(Kv8Attn p, int 
                 for (; j < stop; j++) {
                     ok = ok && mbar_wait_warp(&sm.s_full[t], j & 1, err);
                     tc_fence_after();
-                    const float4 sc01 = *reinterpret_cast<const float4*>(sm.scale[j & 3]);
-                    const float4 sc23 = *reinterpret_cast<const float4*>(sm.scale[j & 3] + 2);
+                    float4 sc01 = *reinterpret_cast<const float4*>(sm.scale[j & 3]);
+                    float4 sc23 = *reinterpret_cast<const float4*>(sm.scale[j & 3] + 2);
+                    const int key0 = (blk0 + j * BLOCKS) * KV8_BLOCK;
+                    const bool masked = key0 + BN > seen_by_all || key0 < first;
+                    if (masked) {  // blocks that only later rows see have no part in the row's reference: their values may be far larger
+                        if (key0 >= lim) sc01.y = 0.f;
+                        if (key0 + KV8_BLOCK >= lim) sc01.w = 0.f;
+                        if (key0 + 2 * KV8_BLOCK >= lim) sc23.y = 0.f;
+                        if (key0 + 3 * KV8_BLOCK >= lim) sc23.w = 0.f;
+                    }
                     const uint32_t top_vs = max(max(__float_as_uint(sc01.y), __float_as_uint(sc01.w)),
                                                 max(__float_as_uint(sc23.y), __float_as_uint(sc23.w)));
                     const uint32_t top_ref = max(ref, (top_vs & 0x7f800000u) + 0x00800000u);
                     const float inv_ref = __uint_as_float(0x7f000000u - top_ref);
                     const float ks[MINE] = {half ? sc23.x : sc01.x, half ? sc23.z : sc01.z};
                     const float vs[MINE] = {half ? sc23.y : sc01.y, half ? sc23.w : sc01.w};
-                    const int key0 = (blk0 + j * BLOCKS) * KV8_BLOCK;
-                    const bool masked = key0 + BN > seen_by_all || key0 < first;
                     // scores in base-2 units, from column c of the thread's 64; -inf where a mask covers them
                     const auto scores = [&](auto& s, int c) {
                         const float f = ks[c / KV8_BLOCK] * unit;
