@@ -648,7 +648,8 @@ typedef struct zwg_kv8 {
 
 /* Append k and v of the call's tokens (heads n_head_kv, `type`), which end the sequences: what
  * a sequence held from its position on is replaced. With rope, k is rotated on the way in
- * (as zwg_rope, kept in f32). One call at a time on a cache. */
+ * (as zwg_rope, kept in f32), and s->n_past may be no more than the tables' n_ctx either. One
+ * call at a time on a cache. */
 ZWG_API int zwg_kv8_append(const zwg_kv8* c, const zwg_seqs* s, int type, const zwg_rows* k, const zwg_rows* v,
                            const zwg_rope_tables* rope, void* stream);
 

@@ -1,0 +1,59 @@
+"""Calls on the 8-bit cache that its documentation allows and that are easily refused or answered wrongly."""
+import numpy as np
+import pytest
+
+from oracle import kv8 as O
+from tests.conftest import has_gpu
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def env():
+    if not has_gpu():
+        pytest.fail("needs a CUDA device")
+    import torch
+
+    from zwhisper_b200 import ops
+    ops.set_math("f32")
+    return torch, ops
+
+
+def i32(torch, a):
+    return torch.tensor(list(a), dtype=torch.int32, device="cuda:0")
+
+
+def test_ragged_append_with_tables_shorter_than_the_cache(env):
+    """Sequences within the tables are appended; those that end or start behind them are left out and reported."""
+    torch, ops = env
+    from zwhisper_b200._lib import ZwgError
+    rng = np.random.default_rng(0)
+    B, n, past = 5, 3, [0, 29, 30, 33, 7]  # of 32 positions
+    cos, sin = (torch.from_numpy(a).cuda() for a in ops.rope_tables(32, 64, 1e4))
+    k, v = (rng.standard_normal((B, n, 1, 64), dtype=np.float32) for _ in range(2))
+    cache, want = ops.Kv8Cache.empty(B, 1, 64, 64), O.Cache(B, 1, 64, 64)
+    ops.sync()
+    # within the tables: no error
+    cache.append(torch.from_numpy(k).cuda(), torch.from_numpy(v).cuda(), i32(torch, [0, 29, 0, 0, 7]), count=i32(torch, [3, 3, 0, 0, 3]),
+                 rope=(cos, sin))
+    ops.sync()
+    cache = ops.Kv8Cache.empty(B, 1, 64, 64)
+    cache.append(torch.from_numpy(k).cuda(), torch.from_numpy(v).cuda(), i32(torch, past), rope=(cos, sin))
+    with pytest.raises(ZwgError):
+        ops.sync()
+    turned = k.copy()
+    for b in (0, 1, 4):
+        turned[b] = O.rope(k[b], cos.cpu().numpy(), sin.cpu().numpy(), past[b] + np.arange(n), False)
+    want.append(turned, v, past, [3, 3, 0, 0, 3])
+    np.testing.assert_array_equal(cache.k.cpu().numpy().reshape(B, 1, 64, 64), want.ints[0])
+    np.testing.assert_array_equal(cache.v_scale.cpu().numpy(), want.scale[1])
+    np.testing.assert_array_equal(cache.open_block.cpu().numpy(), want.tag)
+    # a bound of the caller's own, as attn has
+    cache = ops.Kv8Cache.empty(B, 1, 64, 64)
+    cache.append(torch.from_numpy(k).cuda(), torch.from_numpy(v).cuda(), i32(torch, past), rope=(cos, sin), max_past=7)
+    with pytest.raises(ZwgError):
+        ops.sync()
+    assert cache.open_block.flatten().tolist() == [0, -1, -1, -1, 0]
+    with pytest.raises(ZwgError):
+        cache.append(torch.from_numpy(k).cuda(), torch.from_numpy(v).cuda(), i32(torch, past), rope=(cos, sin), max_past=33)
+    ops.sync()

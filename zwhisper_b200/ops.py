@@ -996,10 +996,11 @@ class Kv8Cache:
     def _call(self, n: int, n_past, count, first, max_past):
         return _seqs(self.n_batch, n, n_past, count, first, self.n_ctx if max_past is None else max_past, self.device)
 
-    def append(self, k, v, n_past, count=None, rope=None) -> None:
+    def append(self, k, v, n_past, count=None, rope=None, max_past=None) -> None:
         """Append k, v [n_batch][n][n_head_kv][d] (f32 or bf16) at n_past (an int, or a CUDA int32
-        tensor [n_batch]); count (CUDA int32 [n_batch]): tokens of each sequence. rope: (cos,
-        sin) or (cos, sin, interleaved), the rotation of k on its way in."""
+        tensor [n_batch] whose entries are at most max_past; None: the cache's end, or the
+        tables'); count (CUDA int32 [n_batch]): tokens of each sequence. rope: (cos, sin) or
+        (cos, sin, interleaved), the rotation of k on its way in."""
         kind = _row_type(k, "k")
         if k.dim() != 4:
             raise ValueError("k and v must be [n_batch][n][n_head_kv][d]")
@@ -1007,7 +1008,9 @@ class Kv8Cache:
         shape = (self.n_batch, n, self.n_head_kv, self.d)
         t = None if rope is None else _tables(rope[0], rope[1], dev, len(rope) > 2 and rope[2])
         kr, vr = _rows(k, dtype, dev, shape, "k"), _rows(v, dtype, dev, shape, "v")
-        s = self._call(n, n_past, count, None, None)
+        if max_past is None and rope is not None:
+            max_past = min(self.n_ctx, rope[0].shape[0])
+        s = self._call(n, n_past, count, None, max_past)
         _lib.check(_ready(dev).zwg_kv8_append(self._ref, s, kind, kr, vr, t, _stream_on(dev)))
 
     def read(self, n: int, n_past, count=None, k=None, v=None):
