@@ -57,3 +57,22 @@ def test_ragged_append_with_tables_shorter_than_the_cache(env):
     with pytest.raises(ZwgError):
         cache.append(torch.from_numpy(k).cuda(), torch.from_numpy(v).cuda(), i32(torch, past), rope=(cos, sin), max_past=33)
     ops.sync()
+
+
+@pytest.mark.parametrize("B,n_ctx", [(1, 2048), (1, 4096), (2, 1024), (3, 1056), (8, 4096), (12, 2048), (64, 2048)])
+@pytest.mark.parametrize("n", [1, 2, 40, 200])
+def test_workspace_for_any_length_serves_positions_on_the_device(env, B, n_ctx, n):
+    """attn_workspace_bytes without a length is enough for a call whose positions only the device knows."""
+    torch, ops = env
+    g = torch.Generator(device="cuda:0").manual_seed(n)
+    cache = ops.Kv8Cache.empty(B, 2, 64, n_ctx)
+    k, v = (torch.randn(B, n_ctx, 2, 64, device="cuda:0", generator=g) for _ in range(2))
+    cache.append(k, v, 0)
+    q = torch.randn(B, n, 12, 64, device="cuda:0", generator=g)
+    size = cache.attn_workspace_bytes(n, 12)
+    ws = torch.full((size + 256,), 77, dtype=torch.uint8, device="cuda:0")
+    at = i32(torch, [n_ctx - n] * B)
+    out = cache.attn(q, at, workspace=ws[:size])
+    assert torch.equal(out, cache.attn(q, at))
+    assert (ws[size:] == 77).all()
+    ops.sync()

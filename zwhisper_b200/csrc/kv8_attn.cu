@@ -121,6 +121,10 @@ size_t workspace_of(const Kv8& c, const Seqs& s, const Plan& p, int most_splits)
     return (size_t)s.n_batch * c.n_head_kv * p.tiles * most_splits * p.tile_rows * (c.d + 4);
 }
 
+// Keys that the longest sequence can have at the call's end: no more than the cache, wherever n_past, the most
+// that any past[b] may be, lies.
+int keys_of(const Kv8& c, const Seqs& s) { return (int)std::min<long long>((long long)s.n_past + s.n, (long long)c.blocks * KV8_BLOCK); }
+
 // Blocks of keys that a query sees, on average.
 float blocks_seen(const Seqs& s) { return (s.n_past + 0.5f * s.n) / KV8_BLOCK + 1.f; }
 
@@ -128,7 +132,7 @@ float blocks_seen(const Seqs& s) { return (s.n_past + 0.5f * s.n) / KV8_BLOCK + 
 Plan plan_tc(const Kv8& c, const Seqs& s, int rows, int sm_count) {
     Plan p{KV8_PREFILL_ROWS, (rows + KV8_PREFILL_ROWS - 1) / KV8_PREFILL_ROWS, 0, 1, 0, 0.f};
     const long long ctas = (long long)s.n_batch * c.n_head_kv * p.tiles;
-    const int key_tiles = (s.n_past + s.n + KV8_PREFILL_KEYS - 1) / KV8_PREFILL_KEYS;
+    const int key_tiles = (keys_of(c, s) + KV8_PREFILL_KEYS - 1) / KV8_PREFILL_KEYS;
     p.splits = (int)std::min<long long>(std::max<long long>(1, sm_count / ctas), std::max(1, key_tiles / 2));
     p.ws = workspace_of(c, s, p, p.splits);
     // a CTA's start and end and its key tiles, as measured with f32 queries; cuts go through memory twice
@@ -148,7 +152,7 @@ Plan plan_split(const Kv8& c, const Seqs& s, int rows, int n_head, int sm_count)
     p.tiles = (rows + p.tile_rows - 1) / p.tile_rows;
     const int big = big_warps(p.tile_rows);
     const long long ctas = (long long)s.n_batch * c.n_head_kv * p.tiles;
-    const int blocks = (s.n_past + s.n + KV8_BLOCK - 1) / KV8_BLOCK;
+    const int blocks = (keys_of(c, s) + KV8_BLOCK - 1) / KV8_BLOCK;
     const int combine_rows = (int)std::min<long long>((long long)s.n_batch * s.n * n_head, 8 * sm_count);
     // most CTAs for which one block to each warp of small CTAs was the fastest plan: half the SMs
     const int few = (int)(sm_count / 2 / ctas);
