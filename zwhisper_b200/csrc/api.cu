@@ -533,7 +533,7 @@ int zwg_rope_kt_append(size_t n_batch, size_t n, size_t n_past, size_t n_head, s
     Ctx* c = cur();
     if (!c) return ZWG_ERROR;
     if (d == 0 || d % 2) return fail("rope: d must be even");
-    if (n_past + n > n_ctx) return fail("rope: context full (%zu + %zu > %zu)", n_past, n, n_ctx);
+    if (!fits(n_past, n, n_ctx)) return fail("rope: context full (%zu + %zu > %zu)", n_past, n, n_ctx);
     if (n_head_kv == 0 || n_head % n_head_kv) return fail("rope: bad head counts");
     cudaStream_t st = (cudaStream_t)stream;  // NULL: the legacy default stream
     zwg::RopeParams p{q, k, v, cache_kt, cache_v, cos_tab, sin_tab, n, n_past, n_head, n_head_kv, d, n_ctx,

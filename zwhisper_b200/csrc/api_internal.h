@@ -83,6 +83,9 @@ struct Tickets {
     }
 };
 
+// Whether n tokens after n_past have room, for any n_past (a negative one of the host language's comes as a huge one).
+inline bool fits(size_t n_past, size_t n, size_t room) { return n <= room && n_past <= room - n; }
+
 // The calling thread's context (zwg_init), or nullptr with the last error set.
 Ctx* cur();
 // The device error word of the calling thread's context when that context is on the current

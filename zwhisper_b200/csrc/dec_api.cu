@@ -141,7 +141,7 @@ int zwg_dec_forward_q8(zwg_dec_state* st, const zwg_dec_weights* w, const int32_
                        float* x, float* logits, void* scratch, size_t scratch_bytes, void* stream) {
     if (!st || !w || !w->layers) return fail("dec_forward_q8: null state or weights");
     if (n == 0) return ZWG_OK;
-    if (n_past + n > st->n_text_ctx) return fail("dec_forward_q8: context full (%zu + %zu > %zu)", n_past, n, st->n_text_ctx);
+    if (!fits(n_past, n, st->n_text_ctx)) return fail("dec_forward_q8: context full (%zu + %zu > %zu)", n_past, n, st->n_text_ctx);
     Ctx* c = ctx_for(st->device);
     if (!c) return ZWG_ERROR;
     const size_t ns = st->n_state, nb = st->n_batch, M = nb * n;

@@ -50,7 +50,7 @@ Ctx* state_call(const zwg_llm_state* st, size_t layer, size_t n_past, size_t n, 
         fail("%s: bad state or layer", what);
         return nullptr;
     }
-    if (n_past + n > st->n_ctx) {
+    if (!fits(n_past, n, st->n_ctx)) {
         fail("%s: context full (%zu + %zu > %zu)", what, n_past, n, st->n_ctx);
         return nullptr;
     }

@@ -81,7 +81,7 @@ int zwg::capi::llm_attn(zwg_llm_state* st, size_t layer, const float* q, size_t 
     if (!st || layer >= st->n_layer) return fail("llm attention: bad state or layer");
     if (n == 0) return ZWG_OK;
     if (!q || !out) return fail("llm attention: null q/out");
-    if (n_past + n > st->n_ctx) return fail("llm attention: context full (%zu + %zu > %zu)", n_past, n, st->n_ctx);
+    if (!fits(n_past, n, st->n_ctx)) return fail("llm attention: context full (%zu + %zu > %zu)", n_past, n, st->n_ctx);
     Ctx* c = ctx_for(st->device);
     if (!c) return ZWG_ERROR;
     if (!st->kv8.empty()) return kv8_llm_attn(st, layer, q, n_past, n, out, (cudaStream_t)stream);
@@ -194,7 +194,7 @@ int zwg_dec_step_attn(zwg_dec_state* st, size_t layer, int kind, const float* q,
     const float *kp, *vp;
     if (kind == ZWG_DEC_SELF) {
         if (!k_new != !v_new) return fail("dec_step_attn: k_new and v_new must both be given or both be null");
-        if (n_past + n > st->n_text_ctx) return fail("dec_step_attn: context full (%zu + %zu > %zu)", n_past, n, st->n_text_ctx);
+        if (!fits(n_past, n, st->n_text_ctx)) return fail("dec_step_attn: context full (%zu + %zu > %zu)", n_past, n, st->n_text_ctx);
         // the new rows land at n_past.. of every window's cache (src/decoder.zig:182-183);
         // both null: the caller's kernel has written them there already
         if (k_new) {
@@ -365,7 +365,7 @@ int zwg_llm_append_rope(zwg_llm_state* st, size_t layer, float* q, const float* 
     if (!st || layer >= st->n_layer) return fail("llm_append_rope: bad state or layer");
     if (n == 0) return ZWG_OK;
     if (!q || !k || !v) return fail("llm_append_rope: null q/k/v");
-    if (n_past + n > st->n_ctx) return fail("llm_append_rope: context full (%zu + %zu > %zu)", n_past, n, st->n_ctx);
+    if (!fits(n_past, n, st->n_ctx)) return fail("llm_append_rope: context full (%zu + %zu > %zu)", n_past, n, st->n_ctx);
     Ctx* c = ctx_for(st->device);
     if (!c) return ZWG_ERROR;
     if (!st->kv8.empty()) return kv8_llm_append(st, layer, q, k, v, n_past, n, (cudaStream_t)stream);
