@@ -76,3 +76,15 @@ def test_workspace_for_any_length_serves_positions_on_the_device(env, B, n_ctx, 
     assert torch.equal(out, cache.attn(q, at))
     assert (ws[size:] == 77).all()
     ops.sync()
+
+
+def test_rotary_tables_on_another_device_are_refused(env):
+    torch, ops = env
+    st = ops.LlmState(1, 1, 2, 1, 64, 64, kv8=True)
+    t = torch.ones(64, 32, device="cuda:0")
+    st.set_rope(t, t)
+    st.device = 1  # as if the state were there
+    with pytest.raises(ValueError, match="cuda:1"):
+        st.set_rope(t, t)
+    st.device = 0
+    st.close()

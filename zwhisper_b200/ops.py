@@ -488,10 +488,12 @@ class LlmState:
                         view(c.open_block, "<i4", B, H))
 
     def set_rope(self, cos, sin) -> None:
-        """Replace the rotary tables by cos, sin [n_ctx][d/2] f32 (CUDA tensors), for example
-        scaled_rope_tables'."""
+        """Replace the rotary tables by cos, sin [n_ctx][d/2] f32 (CUDA tensors on the state's
+        device), for example scaled_rope_tables'."""
         torch = _torch()
         for t, name in ((cos, "cos"), (sin, "sin")):
+            if t.is_cuda and t.device.index != self.device:  # its copy would not be in this device's streams' order
+                raise ValueError(f"{name} must be on cuda:{self.device}, got {t.device}")
             if t.numel() != self.n_ctx * (self.d // 2):
                 raise ValueError(f"{name} must hold n_ctx * d / 2 floats, got {t.numel()}")
         _lib.check(_lib.load().zwg_llm_state_set_rope(self._h, _dev_ptr(cos, torch.float32, "cos"),
