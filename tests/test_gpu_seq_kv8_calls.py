@@ -88,3 +88,39 @@ def test_rotary_tables_on_another_device_are_refused(env):
         st.set_rope(t, t)
     st.device = 0
     st.close()
+
+
+def test_a_cache_whose_offsets_pass_32_bits(env):
+    """A sequence of more than 2^28 tokens of d 128 (34 GB of keys, as many of values): append, read, a step and a chunk."""
+    torch, ops = env
+    rng = np.random.default_rng(1)
+    d, n_ctx, past = 128, 2 ** 28 + 4096, 2 ** 28 + 1003
+    cache = ops.Kv8Cache.empty(1, 1, d, n_ctx)
+    cache.k_scale.fill_(1.0)
+    cache.v.fill_(64)
+    cache.v_scale.fill_(1.0 / 64)
+    k, v = (rng.standard_normal((1, 5, 1, d), dtype=np.float32) for _ in range(2))
+    cache.append(torch.from_numpy(k).cuda(), torch.from_numpy(v).cuda(), past)
+    assert int(cache.open_block[0, 0]) == past // 32 and past // 32 == (past + 4) // 32
+    # the open block goes on from the cache's own values in front of the new tokens: zeros and ones
+    want = O.Cache(1, 1, d, 32)
+    want.append(np.zeros((1, past % 32, 1, d), np.float32), np.ones((1, past % 32, 1, d), np.float32), [0])
+    want.append(k, v, [past % 32])
+    gk, gv = cache.read(5, past)
+    for got, side in ((gk, 0), (gv, 1)):
+        np.testing.assert_array_equal(got[0, :, 0].cpu().numpy(), want.values()[side][0, 0, past % 32:past % 32 + 5])
+    # a step that sees the last 200 tokens alone
+    q = rng.standard_normal((1, 1, 6, d), dtype=np.float32)
+    out = cache.attn(torch.from_numpy(q).cuda(), past + 4, first=i32(torch, [past - 195])).cpu().numpy()
+    kk, vv = (x[0, :, 0].cpu().numpy()[None, None].astype(np.float64) for x in cache.read(200, past - 195))
+    exact, tol = O.attention(q, kk, vv, [199], None, None, 2, 2.0 ** -24)
+    assert (np.abs(out - exact) <= tol).all()
+    # block 5 alone has keys that count: every query of a step and of a chunk gives its values
+    cache.k[0, 0, 5] = 100
+    cache.v[0, 0, 5] = 32
+    for n in (1, 16):
+        out = cache.attn(torch.ones(1, n, 6, d, device="cuda:0"), past)
+        assert (out - 0.5).abs().max() < 1e-6
+    ops.sync()
+    del cache
+    torch.cuda.empty_cache()

@@ -253,7 +253,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(Kv8Attn p, int 
         uint4 kb[N], vb[N];
         float2 sc = make_float2(0.f, 0.f);
         const auto load = [&](uint4 (&buf)[N], const int8_t* from, int j) {
-            const int blk = blk0 + j * BLOCKS, pieces = (blk_hi - blk) * (BYTES / 16);  // behind them: masked, but finite
+            const int blk = blk0 + j * BLOCKS, pieces = min(blk_hi - blk, BLOCKS) * (BYTES / 16);  // behind them: masked, but finite
             const uint4* src = reinterpret_cast<const uint4*>(from + (head + blk) * BYTES + z);
 #pragma unroll
             for (int i = 0; i < N; i++) {
