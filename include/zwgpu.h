@@ -582,9 +582,10 @@ ZWG_API int zwg_gemm_f16(const uint16_t* a, size_t lda, size_t a_bs, const uint1
  * be. count (device int32 [n_batch], or NULL): sequence b has count[b] <= n tokens in this
  * call, and rows i >= count[b] of every buffer are neither read nor written. first (device
  * int32 [n_batch], or NULL; zwg_kv8_attn only): keys before first[b] are not seen (a batch
- * padded on the left). A sequence whose past[b], count[b] or first[b] is out of range (below 0,
- * past[b] > n_past, count[b] > n, beyond the cache or the tables) is skipped: its rows stay as
- * they were, and the device error word is set (reported by zwg_sync). */
+ * padded on the left); first[b] may lie behind them all, so that a query sees none. A sequence
+ * whose past[b] or count[b] is out of range (below 0, past[b] > n_past, count[b] > n, beyond the
+ * cache or the tables), or whose first[b] is below 0, is skipped: its rows stay as they were, and
+ * the device error word is set (reported by zwg_sync). */
 typedef struct zwg_seqs {
     size_t n_batch;
     size_t n;
@@ -666,9 +667,14 @@ ZWG_API size_t zwg_kv8_attn_workspace(const zwg_kv8* c, const zwg_seqs* s, size_
  * own token included, so the call's tokens are appended before it. Softmax of q . k / sqrt(d)
  * in f32, sums in f32. A query that sees no key gives zeros. The context's math mode applies to
  * f32 queries: ZWG_MATH_F32 holds each query and probability in two f16 pieces (22 bits)
- * against the exact int8 values, ZWG_MATH_TF32 in one (11 bits, as that mode's operands);
- * bf16 queries are exact in one piece. The workspace belongs to one call at a time: calls that
- * may overlap (other streams, graphs replayed side by side) need their own. */
+ * against the exact int8 values, ZWG_MATH_TF32 in one (11 bits, as that mode's operands).
+ * For bf16 rows both are in one piece in either mode: the queries as they are, the probabilities
+ * in 11 bits (off by 2^-12 at most, where the output's own rounding is off by up to 2^-8). Beside much
+ * larger ones all end sooner: a query's element is held to 2^-25 of its largest, a probability
+ * times its block's value scale to 2^-39 (calls of more than 48 query rows to a kv head: 2^-35) of
+ * the largest value scale that the query sees. out may be q, but may not
+ * overlap it in another way. The workspace belongs to one call at a time: calls that may overlap
+ * (other streams, graphs replayed side by side) need their own. */
 ZWG_API int zwg_kv8_attn(const zwg_kv8* c, const zwg_seqs* s, int type, size_t n_head, const zwg_rows* q,
                          const zwg_rows* out, void* workspace, size_t workspace_bytes, void* stream);
 

@@ -90,6 +90,21 @@ def test_rotary_tables_on_another_device_are_refused(env):
     st.close()
 
 
+@pytest.mark.parametrize("B,n,past,d", [(1, 1, 4000, 64), (2, 1, 20000, 128), (3, 5, 300, 64), (1, 64, 4000, 64), (40, 150, 2000, 64),
+                                        (12, 256, 1700, 128)])
+@pytest.mark.parametrize("bf16", [False, True])
+def test_output_in_the_place_of_the_queries(env, B, n, past, d, bf16):
+    """Whole, cut and joined keys, and sums that wait in the output's place."""
+    torch, ops = env
+    g = torch.Generator(device="cuda:0").manual_seed(n)
+    cache = ops.Kv8Cache.empty(B, 1, d, (past + n + 31) // 32 * 32)
+    cache.append(*(torch.randn(B, past + n, 1, d, device="cuda:0", generator=g) for _ in range(2)), 0)
+    q = torch.randn(B, n, 6, d, device="cuda:0", generator=g).to(torch.bfloat16 if bf16 else torch.float32)
+    want = cache.attn(q, past)
+    assert cache.attn(q, past, out=q) is q and torch.equal(q, want)
+    ops.sync()
+
+
 def test_a_cache_whose_offsets_pass_32_bits(env):
     """A sequence of more than 2^28 tokens of d 128 (34 GB of keys, as many of values): append, read, a step and a chunk."""
     torch, ops = env

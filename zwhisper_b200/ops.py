@@ -924,8 +924,8 @@ def rope(q, cos, sin, n_past=0, k=None, interleaved: bool = False, count=None, i
     sequence b at position n_past + i (n_past an int, or a CUDA int32 tensor [n_batch]). cos,
     sin [n_ctx][rot/2] f32 (rope_tables, scaled_rope_tables): the first rot elements of a head
     are rotated, in pairs (i, i + rot/2) or, interleaved, (2i, 2i + 1). count (CUDA int32
-    [n_batch]): tokens of each sequence, the rows behind them stay. In place, or into q_out and
-    k_out (new tensors with inplace=False). Returns q, or (q, k)."""
+    [n_batch]): tokens of each sequence, the rows behind them stay (in new tensors: undefined). In
+    place, or into q_out and k_out (new tensors with inplace=False). Returns q, or (q, k)."""
     torch = _torch()
     kind = _row_type(q, "q")
     if q.dim() != 4 or (k is not None and k.dim() != 4):
@@ -1038,8 +1038,8 @@ class Kv8Cache:
         """Attention (zwg_kv8_attn) of q [n_batch][n][n_head][d] (f32 or bf16) at positions n_past..
         (an int, or a CUDA int32 tensor [n_batch] whose entries are at most max_past) over the
         cache, which holds the call's own tokens already: query i of sequence b sees keys
-        first[b] .. n_past + i. count, first: CUDA int32 [n_batch]; rows of out behind count[b]
-        stay as they are. workspace: a contiguous CUDA tensor of attn_workspace_bytes (None: one is
+        first[b] .. n_past + i (none: zeros). count, first: CUDA int32 [n_batch]; rows of out behind
+        count[b] stay as they are. workspace: a contiguous CUDA tensor of attn_workspace_bytes (None: one is
         made). Returns out, of q's shape and type (a new one has zeros there)."""
         torch = _torch()
         kind = _row_type(q, "q")
