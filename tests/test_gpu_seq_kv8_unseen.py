@@ -47,3 +47,31 @@ def test_values_that_a_query_does_not_see(d, B, H, n, mode):
         checked += not large
     assert 0 < checked < n
     ops.sync()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("B,n", [(1, 3), (96, 40)])  # both kernels
+@pytest.mark.parametrize("size_q,size_k", [(2e38, 3e-39), (4e37, 1e-38), (2e-38, 2e37), (1e-39, 3e38)])
+def test_queries_at_the_ends_of_f32(d, B, n, size_q, size_k):
+    """Queries whose largest element is near f32's largest or smallest numbers, and keys that make ordinary scores of them."""
+    if not has_gpu():
+        pytest.fail("needs a CUDA device")
+    import torch
+
+    from zwhisper_b200 import ops
+    rng = np.random.default_rng(d + n)
+    H, past = 6, 60
+    clipped = lambda *s: np.clip(rng.standard_normal(s), -1.1, 1.1)  # noqa: E731
+    k, v = (clipped(B, past + n, 1, d) * size_k).astype(np.float32), clipped(B, past + n, 1, d).astype(np.float32)
+    q = (clipped(B, n, H, d) * size_q).astype(np.float32)
+    cache, held = ops.Kv8Cache.empty(B, 1, d, 128), O.Cache(1, 1, d, 128)
+    cache.append(torch.from_numpy(k).cuda(), torch.from_numpy(v).cuda(), 0)
+    held.append(k[:1], v[:1], [0])
+    ops.set_math("f32")
+    out = cache.attn(torch.from_numpy(q).cuda(), past).cpu().numpy()
+    kk, vv = held.values(np.float64)
+    exact, tol = O.attention(q[:1], kk, vv, [past], None, None, 2, 2.0 ** -24)
+    # the factor of a row's scores, down to 2^-129, is rounded to a multiple of 2^-149: 2^-21 of a score of at most 8
+    tol = tol + 2 * 2.0 ** -21 * 8 * np.abs(v).max()
+    assert (np.abs(out[:1] - exact) <= tol).all(), np.abs(out[:1] - exact).max()
+    ops.sync()

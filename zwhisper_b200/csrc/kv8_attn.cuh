@@ -35,12 +35,12 @@ ZWG_DEV void pieces_of(float x, float y, uint32_t (&w)[P]) {
     }
 }
 
-// The power of two of |x|'s exponent and its inverse; 1 for zero, tiny, infinite and NaN.
+// The power of two of |x|'s exponent and its inverse, both normal numbers: 2^-126 for zero and what is smaller,
+// 2^126 for what is larger (x / 2^126 is below 4), infinite or NaN.
 ZWG_DEV void power_of(float x, float& p, float& inv) {
-    const uint32_t e = __float_as_uint(x) & 0x7f800000u;
-    const bool fine = e > 0x01000000u && e < 0x7e000000u;
-    p = fine ? __uint_as_float(e) : 1.f;
-    inv = fine ? __uint_as_float(0x7f000000u - e) : 1.f;
+    const uint32_t e = min(max(__float_as_uint(x) & 0x7f800000u, 0x00800000u), 0x7e800000u);
+    p = __uint_as_float(e);
+    inv = __uint_as_float(0x7f000000u - e);
 }
 
 ZWG_DEV float up(float x) { return x; }
