@@ -658,8 +658,8 @@ ZWG_API int zwg_kv8_append(const zwg_kv8* c, const zwg_seqs* s, int type, const 
  * [n_batch][n][n_head_kv][d] f32, either may be NULL. */
 ZWG_API int zwg_kv8_read(const zwg_kv8* c, const zwg_seqs* s, float* k, float* v, void* stream);
 
-/* Bytes of workspace (0: none) that zwg_kv8_attn may need for this call and for calls of the same
- * sizes that are shorter (a smaller n_past). */
+/* Bytes of workspace (0: none, or arguments that zwg_kv8_attn refuses) that zwg_kv8_attn may need
+ * for this call and for calls of the same sizes that are shorter (a smaller n_past). */
 ZWG_API size_t zwg_kv8_attn_workspace(const zwg_kv8* c, const zwg_seqs* s, size_t n_head);
 
 /* Attention of the call's queries (n_head a multiple of n_head_kv; query head h reads kv head
@@ -713,7 +713,8 @@ ZWG_API int zwg_llm_logits(float* logits, size_t m, size_t n_vocab, size_t strid
 
 /* An LLM state whose layers keep their keys and values in 8 bits (zwg_kv8), for calls of up to
  * n_chunk tokens. Every zwg_llm_* call on a state takes it (d 64 or 128, n_ctx a multiple of 32);
- * zwg_llm_state_cache does not, zwg_llm_state_kv8 gives a layer's cache instead. */
+ * zwg_llm_state_cache does not, zwg_llm_state_kv8 gives a layer's cache instead. As with any state,
+ * its calls share its buffers: one after another, also those that graphs replay. */
 ZWG_API int zwg_llm_state_create_kv8(size_t n_layer, size_t n_batch, size_t n_head, size_t n_head_kv, size_t d,
                                      size_t n_ctx, size_t n_chunk, double rope_base, zwg_llm_state** out);
 ZWG_API int zwg_llm_state_kv8(const zwg_llm_state* st, size_t layer, zwg_kv8* out);

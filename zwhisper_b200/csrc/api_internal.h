@@ -83,6 +83,18 @@ struct Tickets {
     }
 };
 
+// The context's device for the length of a call, whatever the current device is.
+struct OnDevice {
+    int before = -1, device;
+    explicit OnDevice(int d) : device(d) {
+        if (cudaGetDevice(&before) != cudaSuccess) before = -1;
+        if (before != device) cudaSetDevice(device);
+    }
+    ~OnDevice() {
+        if (before >= 0 && before != device) cudaSetDevice(before);
+    }
+};
+
 // Whether n tokens after n_past have room, for any n_past (a negative one of the host language's comes as a huge one).
 inline bool fits(size_t n_past, size_t n, size_t room) { return n <= room && n_past <= room - n; }
 

@@ -15,18 +15,6 @@ using namespace zwg::capi;
 
 namespace {
 
-// The context's device for the length of a call, whatever the current device is.
-struct OnDevice {
-    int before = -1, device;
-    explicit OnDevice(int d) : device(d) {
-        if (cudaGetDevice(&before) != cudaSuccess) before = -1;
-        if (before != device) cudaSetDevice(device);
-    }
-    ~OnDevice() {
-        if (before >= 0 && before != device) cudaSetDevice(before);
-    }
-};
-
 constexpr size_t kMost = (size_t)1 << 30;
 
 size_t type_size(int type) { return type == ZWG_TYPE_F32 ? 4 : type == ZWG_TYPE_BF16 ? 2 : 0; }
