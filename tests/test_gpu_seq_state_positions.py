@@ -57,3 +57,15 @@ def test_rope_append(env):
         rc = _lib.load().zwg_rope_kt_append(1, n, past, 1, 1, 64, 32, x, x, x, x, x, x, x, 64 * n, 64 * n, 64 * 32, None)
         assert rc == _lib.ZWG_ERROR and "context full" in _lib.last_error()
     ops.sync()
+
+
+def test_sizes_whose_products_wrap_are_refused(env):
+    torch, ops = env
+    from zwhisper_b200._lib import ZwgError
+    fine = dict(n_layer=1, n_batch=1, n_head=2, n_head_kv=1, d=64, n_ctx=64, kv8=True, n_chunk=8)
+    ops.LlmState(**fine).close()
+    for bad in (dict(n_batch=1 << 33, n_head=1 << 33, n_head_kv=1 << 33), dict(n_batch=1 << 63, n_head_kv=2), dict(n_layer=1 << 62),
+                dict(n_layer=65535, n_batch=60000, n_ctx=1 << 25), dict(n_chunk=-1), dict(n_chunk=0)):
+        with pytest.raises(ZwgError, match="bad sizes|too large"):
+            ops.LlmState(**{**fine, **bad})
+    ops.sync()

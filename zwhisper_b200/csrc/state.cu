@@ -269,10 +269,12 @@ int zwg_llm_state_create_kv8(size_t n_layer, size_t n_batch, size_t n_head, size
     Ctx* c = cur();
     if (!c) return ZWG_ERROR;
     if (!n_layer || !n_batch || !n_head || !n_head_kv || n_head % n_head_kv || (d != 64 && d != 128) || !n_ctx ||
-        n_ctx % 32 || n_ctx >= (1u << 30) || !n_chunk || n_chunk > n_ctx || n_batch * n_head_kv > 65535 || !(rope_base > 0))
+        n_ctx % 32 || n_ctx >= (1u << 30) || !n_chunk || n_chunk > n_ctx || n_batch > 65535 || n_head_kv > 65535 ||
+        n_batch * n_head_kv > 65535 || n_layer > 65535 || !(rope_base > 0))
         return fail("llm state in 8 bits: bad sizes (n_head %zu, n_head_kv %zu, d %zu, n_ctx %zu, n_chunk %zu)", n_head,
                     n_head_kv, d, n_ctx, n_chunk);
     const OnDevice on(c->device);
+    if (n_ctx * d >= ((size_t)1 << 44) / (n_batch * n_head_kv) / n_layer) return fail("llm state in 8 bits: too large");
     zwg_llm_state* st = new (std::nothrow) zwg_llm_state();
     if (!st) return fail("llm state: out of memory");
     st->device = c->device;
