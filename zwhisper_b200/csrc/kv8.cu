@@ -13,7 +13,10 @@
 // Bound by memory and by issue alike for a chunk of a prompt (f32 in, a quarter of it out; the exact
 // quotients and byte turns take 62 % of the issue slots): 64 sequences x 256 tokens, 2 heads of d 128, f32,
 // 42 MB: 14.5 us, 2.9 TB/s, and reading them back 6.2 us out of L2 (10.8 from memory). Staging every row in
-// shared memory and turning values byte by byte there took 92 us for both. Bound by the latency of one CTA's
+// shared memory and turning values byte by byte there took 92 us for both. Cold, under a profiler: 21.0 us (bf16 rows
+// 22.9), 35.5 where the keys lie transposed in the staging of the q/k/v product and 63 where they are rotated here: both
+// go through shared memory one element at a time, in 64 registers with 176 to 204 bytes of spills read back in a
+// thread at d 128 (the direct forms: 4 at most). Bound by the latency of one CTA's
 // chain of loads and barriers for a step: 4.0 us for 64 sequences' token.
 //
 // Rounding: the rounded quotient is found from 127 x * (1 / max |x|) in f32 unless that is

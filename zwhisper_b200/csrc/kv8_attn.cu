@@ -21,11 +21,13 @@
 // other's shared memory; more of them write partials (m, l, O) for kv8_combine_kernel.
 //
 // A decode step is bound by the cache's bytes: 64 sequences, 12 / 2 heads of d 128, f32 queries, in a graph
-// 16.5 us at 2256 tokens (75 MB, 4.5 TB/s), 30.2 at 4512, 52.8 at 9024 (298 MB, 5.6 TB/s; 6.6 TB/s from one
+// 17.5 us at 2256 tokens (75 MB, 4.3 TB/s), 30.1 at 4512, 52.4 at 9024 (298 MB, 5.7 TB/s; 6.6 TB/s from one
 // length to the next, so what is left is the start, the merge and the launch, 5 us). Few sequences are bound
-// by latency: one of 2256 tokens 7.6 us, of 65001 15.6 us. A block's products start from zero and are added to O
-// rounded, since the tensor cores truncate their sums: off by 2.5e-7 at any length; summed in O itself 1.4e-6 after
-// 100000 keys, and 0 to 4 % faster at d 128, 2 to 4 % slower at d 64 (O was rescaled apart).
+// by latency: one of 2256 tokens 7.5 us, of 65536 16.3 us. Two of 131001 in bf16 31.2 us: 6.0 TB/s to the next length,
+// so 22 us of bytes and 9 of start, partials and second kernel. A block's products start from zero and are added to O
+// rounded, since the tensor cores truncate their sums: off by 2.3e-7 to 2.6e-7 from 500 to 100000 keys, by 2.9e-7 to
+// 5.7e-7 where the keys have a few strong channels (the f32 library form: 0.4e-6 to 1.6e-6); summed in O itself 1.4e-6
+// after 100000 keys, and 0 to 4 % faster at d 128, 2 to 4 % slower at d 64 (O was rescaled apart).
 #include <algorithm>
 #include <cmath>
 
@@ -187,9 +189,13 @@ Plan plan_split(const Kv8& c, const Seqs& s, int rows, int n_head, int sm_count)
 }
 
 // The tcgen05 kernel has four times the other one's rate, but 10 us of start and end for a CTA of 256 rows and
-// 128 keys at a time. Up to 48 rows the other one was faster everywhere; above, the shorter estimate: 8 sequences
-// of 2000 tokens, d 128, 288 rows a head 39.3 us against 47.5, 1536 rows 208 against 97.5; a prompt's first 256
-// tokens (1536 rows) of one sequence 9.2 against 23.6, of 64 sequences 314 against 138.
+// 128 keys at a time. Both were timed for 24 to 1536 rows a head, 1 to 64 sequences, 200 to 8000 tokens, both d and
+// f32, tf32 and bf16. Up to 48 rows the other one was at most 3 % the slower one (64 sequences of 200 tokens, 48 rows,
+// d 128, bf16 14.6 us against 15.0; of 2000 62 against 86 in f32, 55 against 57 in bf16; one of 8000 13 against 24); above,
+// the shorter estimate: 16 sequences of 2000 tokens, d 128, 288 rows 75 us against 69, 1536 rows 408 against 228; one
+// of 200 tokens, 1536 rows 12.9 against 28.9. Its constants are f32's; with one piece both kernels take 0.6 to 0.85 of
+// that, and the choice is as good: on average 1.4 % from the better in every type, at worst 1.5 times (f32) and 1.6 times
+// (16 sequences of 8000 tokens, 144 rows, d 64, bf16: 98 us for 60).
 Plan plan_for(const Kv8& c, const Seqs& s, int n_head, int sm_count) {
     const int rows = s.n * (n_head / c.n_head_kv);
     Plan split = plan_split(c, s, rows, n_head, sm_count);

