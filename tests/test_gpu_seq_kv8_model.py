@@ -84,3 +84,30 @@ def test_forward_is_its_pieces(env, d, B):
     whole.close()
     parts.close()
     ops.sync()
+
+
+@pytest.mark.parametrize("d,B,n", [(64, 16, 1), (128, 16, 1), (64, 3, 50), (128, 8, 33)])
+def test_forward_replayed(env, d, B, n):
+    """A captured pass, whose kernels start before their predecessors end and share the state's staging and
+    workspace, gives the eager pass's bits at every replay."""
+    torch, ops = env
+    m = qwen.make_model(d, n_layer=4, n_vocab=96, n_head=4, n_head_kv=2, d=d, n_ff=128, n_ctx=640)
+    W = ops.LlmWeightsQ8(m["layers"], m["embd"], None, m["output_norm"], m["cfg"]["eps"])
+    rng = np.random.default_rng(d)
+    st = ops.LlmState(4, B, 4, 2, d, 640, rope_base=m["cfg"]["rope_base"], kv8=True, n_chunk=64)
+    for past in range(0, 512, 64):
+        st.forward_q8(W, torch.from_numpy(rng.integers(0, 96, (B, 64)).astype(np.int32)).cuda(), past)
+    t = torch.from_numpy(rng.integers(0, 96, (B, n)).astype(np.int32)).cuda()
+    x, logits = (a.clone() for a in st.forward_q8(W, t, 512))
+    xo, lo, scratch = torch.empty_like(x), torch.empty_like(logits), st.scratch(n, W.n_ff)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        st.forward_q8(W, t, 512, x=xo, logits=lo, scratch=scratch)
+    for _ in range(20):
+        lo.fill_(float("nan"))
+        graph.replay()
+        assert torch.equal(xo, x) and torch.equal(lo, logits)
+    del graph
+    st.close()
+    ops.sync()
