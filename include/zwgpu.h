@@ -575,6 +575,7 @@ ZWG_API int zwg_gemm_f16(const uint16_t* a, size_t lda, size_t a_bs, const uint1
  * captured into a graph. They run on the calling thread's device (zwg_init), whatever the
  * current device is. */
 #define ZWG_TYPE_F32 0
+#define ZWG_TYPE_F16 1 /* of a cache in pages only */
 #define ZWG_TYPE_BF16 2
 
 /* The tokens of one call: token i of sequence b is at position p = n_past + i, or past[b] + i
@@ -677,6 +678,87 @@ ZWG_API size_t zwg_kv8_attn_workspace(const zwg_kv8* c, const zwg_seqs* s, size_
  * (other streams, graphs replayed side by side) need their own. */
 ZWG_API int zwg_kv8_attn(const zwg_kv8* c, const zwg_seqs* s, int type, size_t n_head, const zwg_rows* q,
                          const zwg_rows* out, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- a cache in pages, and trees of drafted tokens ----------------------------------------
+ * No reference counterpart. Keys and values in 16 bits, in pages of a pool that each sequence's
+ * row of a table names, so that sequences of any lengths share the memory, and a prefix that
+ * several begin with is held once. Calls as those of the cache in 8 bits above: device pointers,
+ * no allocation, launches on `stream` that may be captured into a graph, on the calling thread's
+ * device (zwg_init). Slot t of a sequence is its token t's place: page table[b][t / page], row
+ * t % page of it. */
+
+/* The cache: d 64 or 128, `page` a power of two from 16 to 256,
+ *   k, v   [n_pages][n_head_kv][page][d] of `type`, pages `page_stride` elements apart (a multiple
+ *          of 8, at least n_head_kv * page * d; k and v may share a buffer that way), 16-byte aligned
+ *   table  int32 [n_batch][max_pages], rows table_stride apart; an entry outside [0, n_pages) is
+ *          no page (-1, say, behind a sequence's last one)
+ * ZWG_TYPE_F16 caches take f32 rows, rounded to the nearest f16 (infinite from 65520 on), ZWG_TYPE_BF16
+ * ones bf16 rows. Where a call needs a slot whose entry is no page, the device error word is set
+ * (reported by zwg_sync) and the slot is left out: not written, or not seen. Pages that two
+ * sequences share may be read by both; if two tokens of a call are written to the same row, either may stay. */
+typedef struct zwg_paged {
+    void* k;
+    void* v;
+    int32_t type;
+    const int32_t* table;
+    size_t table_stride;
+    size_t n_batch, n_head_kv, d, page, n_pages, max_pages, page_stride;
+} zwg_paged;
+
+/* The tokens of a call as a tree: token i of sequence b (at most ZWG_MAX_TREE of them) comes after
+ * token parent[b * batch_stride + i] < i of the call, or, where that is -1, after the sequence's
+ * past tokens (device int32; batch_stride 0: one tree for all sequences). It is held in slot
+ * past + i and stands at position past + the number of tokens above it. A sequence with a parent
+ * of another value is skipped, as one whose past or count is out of range. */
+typedef struct zwg_tree {
+    const int32_t* parent;
+    size_t batch_stride;
+} zwg_tree;
+#define ZWG_MAX_TREE 256
+
+/* Append k and v (n_head_kv heads, `type`: ZWG_TYPE_F32 or _BF16, as the cache takes) of the call's
+ * tokens. With rope, k is rotated to its position on the way in (as zwg_rope, then one rounding),
+ * and q [n_head heads], where given (NULL: none), into q_out (NULL: in place; q_out may be q, but
+ * may not overlap it in another way); past + count may be no more than the tables' n_ctx then.
+ * tree may be NULL: each token comes after the one before. One call at a time on a cache. */
+ZWG_API int zwg_paged_append(const zwg_paged* c, const zwg_seqs* s, const zwg_tree* tree, int type, const zwg_rows* k,
+                             const zwg_rows* v, const zwg_rope_tables* rope, size_t n_head, const zwg_rows* q,
+                             const zwg_rows* q_out, void* stream);
+
+/* Bytes of workspace (0: none, or arguments that zwg_paged_attn refuses) that zwg_paged_attn may need
+ * for this call and for calls of the same sizes that are shorter (a smaller n_past). */
+ZWG_API size_t zwg_paged_attn_workspace(const zwg_paged* c, const zwg_seqs* s, size_t n_head);
+
+/* Attention of the call's queries (n_head a multiple of n_head_kv; query head h reads kv head
+ * h / (n_head / n_head_kv)) over the pages, which hold the call's tokens already. Query i of sequence b
+ * sees slots first[b] .. past + i, or with a tree first[b] .. past - 1, past + i and those of the tokens above
+ * it. Softmax of q . k / sqrt(d) in f32, sums in f32; a query that sees no key gives zeros; what lies in
+ * slots that a query does not see (infinities and NaN too) leaves its output alone. The context's math
+ * mode applies to f32 queries: ZWG_MATH_F32 holds each query and probability in two f16 pieces (22 bits) against
+ * the f16 keys and values, ZWG_MATH_TF32 in one (11 bits); a query's element is held to 2^-25 of its
+ * largest, a probability to 2^-35 of the largest (probabilities are f16 pieces of 2^11 p or more). bf16
+ * queries are taken as they are, their probabilities rounded to bf16 before they weigh values and are
+ * summed. out may be q, but may not overlap it in another way. The workspace belongs to one call
+ * at a time: calls that may overlap (other streams, graphs replayed side by side) need their own. */
+ZWG_API int zwg_paged_attn(const zwg_paged* c, const zwg_seqs* s, const zwg_tree* tree, int type, size_t n_head,
+                           const zwg_rows* q, const zwg_rows* out, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Which drafted tokens the model agrees with: from token 0, which was chosen before, to the child
+ * (of the lowest index) whose token is what the model says after its parent, as long as there is
+ * one. tokens and ids [n_batch][n] (device int32): the drafted tokens, and the model's token after each
+ * (zwg_llm_logits on the rows of their logits). path [n_batch][n]: the agreed tokens' indices, -1
+ * behind them; n_path [n_batch]: how many; next [n_batch]: the model's token after the last of them, which
+ * goes on. Of s only n_batch, n (at most ZWG_MAX_TREE) and count count. A sequence without tokens, or one that
+ * is skipped, has n_path 0 and next -1. */
+ZWG_API int zwg_tree_accept(const zwg_seqs* s, const zwg_tree* tree, const int32_t* tokens, const int32_t* ids,
+                            int32_t* path, int32_t* n_path, int32_t* next, void* stream);
+
+/* Move the rows of token path[b][j] to slot past + j, j < n_path[b] (as zwg_tree_accept gives them; past and
+ * n as in the calls before it), in n_caches caches (a HOST array: a model's layers, one launch for every
+ * 64) that differ in k and v only. Rows behind them stay. A path that does not rise, or leaves the call's n
+ * tokens, is skipped with its sequence. */
+ZWG_API int zwg_paged_keep(const zwg_paged* caches, size_t n_caches, const zwg_seqs* s, const int32_t* path,
+                           const int32_t* n_path, void* stream);
 
 /* The rules on a step's logits. For each row, in this order and in f32:
  *   1. a token that is c > 0 times among the row's last `window` (at most 524287) recent tokens:

@@ -19,7 +19,9 @@ ZWG_MATH_F32 = 0
 ZWG_MATH_BF16 = 1
 ZWG_MATH_TF32 = 2
 ZWG_TYPE_F32 = 0
+ZWG_TYPE_F16 = 1
 ZWG_TYPE_BF16 = 2
+ZWG_MAX_TREE = 256
 
 c_size = ctypes.c_size_t
 c_ptr = ctypes.c_void_p
@@ -158,6 +160,20 @@ class Kv8C(ctypes.Structure):
                 ("n_ctx", c_size)]
 
 
+class PagedC(ctypes.Structure):
+    """zwg_paged: a cache in pages."""
+
+    _fields_ = [("k", c_ptr), ("v", c_ptr), ("type", ctypes.c_int32), ("table", c_ptr), ("table_stride", c_size),
+                ("n_batch", c_size), ("n_head_kv", c_size), ("d", c_size), ("page", c_size), ("n_pages", c_size),
+                ("max_pages", c_size), ("page_stride", c_size)]
+
+
+class TreeC(ctypes.Structure):
+    """zwg_tree: parents of a call's tokens."""
+
+    _fields_ = [("parent", c_ptr), ("batch_stride", c_size)]
+
+
 class LogitRulesC(ctypes.Structure):
     """zwg_logit_rules: penalties, biases and mask of a step's logits."""
 
@@ -255,6 +271,15 @@ SIGNATURES = {
                                     ctypes.POINTER(RowsC), ctypes.POINTER(RowsC), c_ptr, c_size, c_ptr]),
     "zwg_llm_logits": (ctypes.c_int, [c_ptr, c_size, c_size, c_size, ctypes.POINTER(LogitRulesC), c_ptr, c_size,
                                       c_ptr]),
+    "zwg_paged_append": (ctypes.c_int, [ctypes.POINTER(PagedC), ctypes.POINTER(SeqsC), ctypes.POINTER(TreeC), ctypes.c_int,
+                                        ctypes.POINTER(RowsC), ctypes.POINTER(RowsC), ctypes.POINTER(RopeTablesC), c_size,
+                                        ctypes.POINTER(RowsC), ctypes.POINTER(RowsC), c_ptr]),
+    "zwg_paged_attn_workspace": (c_size, [ctypes.POINTER(PagedC), ctypes.POINTER(SeqsC), c_size]),
+    "zwg_paged_attn": (ctypes.c_int, [ctypes.POINTER(PagedC), ctypes.POINTER(SeqsC), ctypes.POINTER(TreeC), ctypes.c_int,
+                                      c_size, ctypes.POINTER(RowsC), ctypes.POINTER(RowsC), c_ptr, c_size, c_ptr]),
+    "zwg_tree_accept": (ctypes.c_int, [ctypes.POINTER(SeqsC), ctypes.POINTER(TreeC), c_ptr, c_ptr, c_ptr, c_ptr, c_ptr,
+                                       c_ptr]),
+    "zwg_paged_keep": (ctypes.c_int, [ctypes.POINTER(PagedC), c_size, ctypes.POINTER(SeqsC), c_ptr, c_ptr, c_ptr]),
     "zwg_llm_state_create_kv8": (ctypes.c_int, [c_size] * 7 + [ctypes.c_double, ctypes.POINTER(c_ptr)]),
     "zwg_llm_state_kv8": (ctypes.c_int, [c_ptr, c_size, ctypes.POINTER(Kv8C)]),
     "zwg_llm_state_set_rope": (ctypes.c_int, [c_ptr, c_ptr, c_ptr, c_ptr]),

@@ -277,6 +277,68 @@ int kv8_attn_launch(const Kv8Attn& p, int type, int pieces, int sm_count, cudaSt
 constexpr int KV8_PREFILL_ROWS = 256, KV8_PREFILL_KEYS = 128;  // of a tile
 int kv8_prefill_launch(const Kv8Attn& p, int type, int pieces, int splits, cudaStream_t st);
 
+// ---- caches in pages ------------------------------------------------------------------------
+constexpr int TYPE_F16 = 1;         // beside TYPE_F32 and TYPE_BF16: ZWG_TYPE_F16
+constexpr int MOST_TREE = 256;      // tokens of a tree (ZWG_MAX_TREE)
+constexpr int MOST_KEPT = 64;       // caches of one launch of paged_keep_launch
+// A cache in pages (zwg_paged, include/zwgpu.h).
+struct Paged {
+    void* k;               // [n_pages][n_head_kv][page][d], f16 or bf16
+    void* v;
+    const int32_t* table;  // [n_batch][ts]
+    size_t ts, ps;         // table row; page, in elements
+    int n_head_kv, d, log_page, n_pages;
+    int room;              // slots a sequence's table has
+};
+// Parents of a call's tokens (zwg_tree); parent null: each token's is the one before it.
+struct Tree {
+    const int32_t* parent;
+    size_t bs;
+};
+// New rows for the cache, k rotated on the way, and q rotated beside them (paged.cu). q.data null: none.
+struct PagedAppend {
+    Paged c;
+    Seqs s;
+    Tree tree;
+    int n_head;
+    Rows q, q_out, k, v;
+    RopeTables rope;
+    int* err;
+};
+int paged_append_launch(const PagedAppend& p, int type, cudaStream_t st);
+// The drafted tokens that the model agrees with (paged.cu).
+struct TreeAccept {
+    Seqs s;
+    Tree tree;
+    const int32_t *tokens, *ids;     // [n_batch][n]
+    int32_t *path, *n_path, *next;   // [n_batch][n], [n_batch], [n_batch]
+    int* err;
+};
+int tree_accept_launch(const TreeAccept& p, cudaStream_t st);
+// Their rows to where the sequence goes on, in `n` caches of the same sizes and table.
+struct PagedKeep {
+    Paged c;  // k and v unused
+    Seqs s;
+    const int32_t *path, *n_path;
+    int n;
+    void *k[MOST_KEPT], *v[MOST_KEPT];
+    int* err;
+};
+int paged_keep_launch(const PagedKeep& p, cudaStream_t st);
+// Attention over the pages (paged_attn.cu).
+struct PagedAttn {
+    Paged c;
+    Seqs s;
+    Tree tree;
+    int n_head;
+    Rows q, out;
+    float* ws;
+    int* err;
+};
+size_t paged_attn_workspace_bytes(const Paged& c, const Seqs& s, int n_head, int sm_count);
+// type: of the rows; pieces: f16 pieces of an f32 query and its probabilities, 1 or 2.
+int paged_attn_launch(const PagedAttn& p, int type, int pieces, int sm_count, cudaStream_t st);
+
 // Penalties, biases, mask and argmax on rows of logits (logits.cu).
 struct LogitRules {
     const int32_t* recent;

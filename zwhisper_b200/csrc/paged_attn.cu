@@ -1,0 +1,630 @@
+// Attention over a cache in pages (zwg_paged_attn): softmax(q . K / sqrt(d)) V, K and V 16-bit floats in pages
+// that a table names, for steps of a token, chunks of a prompt and trees of drafted tokens.
+//
+// paged_split_kernel. The keys are the M side of mma.sync m16n8k16: S^T = K Q^T and O^T = V^T P^T, so that the
+// 8-wide N side is the rows (query * group + head) of a kv head's group, and S^T turns into the operand P^T by two
+// 8x8 register transposes. A warp takes 16 keys at a time, which lie in one page. The order of the d elements
+// in a dot product is free, so lane (g, t) loads 16 consecutive bytes of the rows of keys g and g + 8; the order of
+// the rows of O^T is free, so it loads 16 consecutive bytes of the values of keys 2t, 2t + 1, 2t + 8 and 2t + 9 and
+// pairs them up by byte permutes. So nothing but registers stands between memory and the tensor cores: a warp's next
+// keys are on their way while this group's softmax runs, its next values from the end of this group's products.
+// f32 rows: a query is one or two f16 pieces of q / 2^e (e the exponent of its largest element), a probability one or
+// two of 2^15 p against f16 keys and values; two pieces hold 22 bits, so the result has the accuracy of f32 sums.
+// bf16 rows: queries as they are, probabilities rounded to bf16, and the sum that divides takes the rounded ones, so
+// that what a probability is off by weighs only how far its value is from the result.
+// The splits of a (sequence, kv head, tile of rows) that fit a cluster meet in each other's shared memory; more of them
+// write partials (m, l, O) for paged_combine_kernel.
+#include <algorithm>
+#include <cmath>
+
+#include <cooperative_groups.h>
+
+#include "chain.cuh"
+#include "common.cuh"
+#include "kernels.h"
+#include "kv8_attn.cuh"
+#include "paged.cuh"
+#include "seqs.cuh"
+
+namespace zwg {
+namespace {
+
+namespace cg = cooperative_groups;
+using kv8::kLog2e;
+using kv8::load16;
+using kv8::pieces_of;
+using kv8::power_of;
+using kv8::store4;
+using kv8::wide;
+using paged::Held;
+using paged::page_of;
+using paged::read_tree;
+using paged::row_at;
+
+constexpr int WARPS = 4;         // of a CTA
+constexpr int KEYS = 16;         // of a warp at a time
+constexpr int MAX_CLUSTER = 16;
+
+ZWG_DEV void mma(__half, float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+ZWG_DEV void mma(__nv_bfloat16, float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+ZWG_DEV uint32_t transpose8x8(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+ZWG_DEV uint4 load_cached(const uint16_t* p) { return __ldcg(reinterpret_cast<const uint4*>(p)); }
+ZWG_DEV uint32_t word(const uint4& w, int i) { return i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w; }
+
+// A word's two 16-bit elements, those that are infinite or NaN as zero.
+ZWG_DEV uint32_t finite(uint32_t w, uint32_t exponent) {
+    if ((w & exponent) == exponent) w &= 0xffff0000u;
+    if ((w & exponent << 16) == exponent << 16) w &= 0xffffu;
+    return w;
+}
+
+// What each of n softmax states (m, l) weighs in their sum: f[i] = 2^(m_i - max), and the sum of l f.
+struct Sum {
+    float m, l;
+};
+template <typename M>
+ZWG_DEV Sum weigh(int n, M state, float* f, int step) {
+    Sum x{-INFINITY, 0.f};
+    for (int i = 0; i < n; i++) x.m = fmaxf(x.m, state(i).x);
+    const float base = x.m == -INFINITY ? 0.f : x.m;
+    for (int i = 0; i < n; i++) {
+        const float2 ml = state(i);
+        f[i * step] = exp2_approx(ml.x - base);
+        x.l += ml.y * f[i * step];
+    }
+    return x;
+}
+
+ZWG_DEV void add4(float4& a, float f, float4 x) {
+    a.x += f * x.x;
+    a.y += f * x.y;
+    a.z += f * x.z;
+    a.w += f * x.w;
+}
+
+// The groups of 16 keys [from, to) of a split: the tile's keys first .. past + (the last row's token).
+struct Range {
+    int rows, row0, seen_by_all, end, from, to;
+};
+template <int R>
+ZWG_DEV Range range_of(Place at, int first, int group, int tile, int split, int splits, bool tree) {
+    Range r;
+    r.rows = at.count * group;
+    r.row0 = tile * R;
+    const int q0 = r.row0 / group, q1 = (min(r.rows, r.row0 + R) - 1) / group;
+    r.seen_by_all = tree ? at.past : at.past + q0 + 1;  // slots below it: by every row of the tile
+    r.end = at.past + q1 + 1;                           // slots from it on: by none
+    const int lo = first / KEYS, n = max(0, (r.end + KEYS - 1) / KEYS - lo);
+    const int each = n / splits, more = n - each * splits;
+    r.from = lo + split * each + min(split, more);
+    r.to = r.from + each + (split < more ? 1 : 0);
+    return r;
+}
+
+template <typename T, int D, int NT, int P>
+__global__ void __launch_bounds__(32 * WARPS, NT == 1 ? 3 : 2)
+    paged_split_kernel(PagedAttn p, int splits, int clustered, int vec, float scale) {
+    chain_release();
+    using H = typename Held<T>::type;
+    constexpr int R = 8 * NT, LDO = D + 4, KC = D / 32, VC = D / 64;
+    constexpr bool RAW = sizeof(T) == 2;        // queries as they are
+    constexpr float SHIFT = RAW ? 0.f : 15.f;   // probabilities in units of 2^-15: their f16 pieces stay normal
+    constexpr uint32_t EXP = Held<T>::exponent;
+    __shared__ __align__(16) float sm_o[WARPS][R][LDO];
+    __shared__ float2 state[WARPS][R], merged[R];
+    __shared__ float weight[MAX_CLUSTER][R], inv_l[R];
+    __shared__ int parent[MOST_TREE];
+    __shared__ uint32_t above[R][MOST_TREE / 32];  // a row's token and its ancestors
+    const int tile = blockIdx.x / splits, split = blockIdx.x - tile * splits;
+    const int bh = blockIdx.y, b = bh / p.c.n_head_kv, h = bh - b * p.c.n_head_kv;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int group = p.n_head / p.c.n_head_kv;
+    const bool lead = threadIdx.x == 0 && blockIdx.x == 0 && h == 0, tree = p.tree.parent != nullptr;
+    const int z = chain_wait();
+    const Place at = place_of(p.s, b, p.c.room, lead ? p.err : nullptr);
+    const int first = p.s.first ? __ldcg(p.s.first + b + z) : 0;
+    const Range rg = range_of<R>(at, max(first, 0), group, tile, split, splits, tree);
+    const int rows = rg.rows, row0 = rg.row0, to = rg.to;
+    if (row0 >= rows) return;  // the same for every CTA of a cluster, as the next two
+    if (first < 0) {
+        if (threadIdx.x == 0) set_error(p.err, kErrBounds);
+        return;
+    }
+    if (tree) {
+        if (!read_tree(p.tree, b, at.count, z, parent)) {
+            if (threadIdx.x == 0) set_error(p.err, kErrBounds);
+            return;
+        }
+        if (threadIdx.x < R) {
+            const int r = threadIdx.x;
+            for (int w = 0; w < MOST_TREE / 32; w++) above[r][w] = 0;
+            if (row0 + r < rows)
+                for (int a = (row0 + r) / group; a >= 0; a = parent[a]) above[r][a >> 5] |= 1u << (a & 31);
+        }
+        __syncthreads();
+    }
+
+    // the pages of the warp's next 32 groups, one in each lane
+    int grp = rg.from + warp, pages = 0, it = 0;
+    const auto look = [&](int from) {
+        const int mine = from + lane * WARPS;
+        pages = mine < to ? page_of(p.c, b, mine * KEYS + z) : 0;
+        if (pages < 0) set_error(p.err, kErrBounds);  // its keys are not seen
+    };
+    uint4 kr[2][KC], vr[VC][4];
+    const uint16_t* const kd = static_cast<const uint16_t*>(p.c.k) + z;
+    const uint16_t* const vd = static_cast<const uint16_t*>(p.c.v) + z;
+    const auto load_k = [&](int page, int slot) {
+        const uint16_t* src = kd + row_at(p.c, max(page, 0), h, slot) + g * D + t * 8;
+#pragma unroll
+        for (int m = 0; m < KC; m++) {
+            kr[0][m] = load_cached(src + m * 32);
+            kr[1][m] = load_cached(src + 8 * D + m * 32);
+        }
+    };
+    const auto load_v = [&](int page, int slot) {
+        const uint16_t* src = vd + row_at(p.c, max(page, 0), h, slot) + 2 * t * D + g * 8;
+#pragma unroll
+        for (int c = 0; c < VC; c++)
+#pragma unroll
+            for (int u = 0; u < 4; u++) vr[c][u] = load_cached(src + ((u & 1) + (u >> 1) * 8) * D + c * 64);
+    };
+    look(grp);
+    int page = __shfl_sync(0xffffffffu, pages, 0);
+    if (grp < to) {
+        load_k(page, grp * KEYS);
+        load_v(page, grp * KEYS);
+    }
+
+    // queries: the B operand, lane (g, t) holds row g's elements 8 t .. 8 t + 7 of each 32
+    uint32_t qf[NT][KC][2][P][2];
+    float unit[NT][2];  // of the columns 2t, 2t + 1: 2^e * log2(e) / sqrt(d)
+    int lim[NT][2];     // slots below it may be seen
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        const int row = row0 + nt * 8 + g, i = min(row, rows - 1) / group;
+        const T* q = static_cast<const T*>(p.q.data) + z + b * p.q.bs + i * p.q.ts + (size_t)(h * group + min(row, rows - 1) - i * group) * D + t * 8;
+        if constexpr (RAW) {
+            unit[nt][0] = unit[nt][1] = scale;
+#pragma unroll
+            for (int m = 0; m < KC; m++) {
+                uint32_t w[4];
+                if (vec & 1) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(q + m * 32);
+                    w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+                } else {
+                    const uint16_t* u = reinterpret_cast<const uint16_t*>(q + m * 32);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) w[e] = u[2 * e] | (uint32_t)u[2 * e + 1] << 16;
+                }
+#pragma unroll
+                for (int e = 0; e < 4; e++) qf[nt][m][e >> 1][0][e & 1] = w[e];
+            }
+        } else {
+            float x[KC][8];
+            uint32_t top = 0;
+#pragma unroll
+            for (int m = 0; m < KC; m++) {
+                if (vec & 1) {
+                    *reinterpret_cast<float4*>(&x[m][0]) = *reinterpret_cast<const float4*>(q + m * 32);
+                    *reinterpret_cast<float4*>(&x[m][4]) = *reinterpret_cast<const float4*>(q + m * 32 + 4);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) x[m][e] = q[m * 32 + e];
+                }
+#pragma unroll
+                for (int e = 0; e < 8; e++) top = max(top, __float_as_uint(fabsf(x[m][e])));
+            }
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            float p2, inv;
+            power_of(__uint_as_float(top), p2, inv);
+#pragma unroll
+            for (int e = 0; e < 2; e++) unit[nt][e] = __shfl_sync(0xffffffffu, p2 * scale, (2 * t + e) * 4);
+#pragma unroll
+            for (int m = 0; m < KC; m++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    uint32_t w[P];
+                    pieces_of<P>(x[m][2 * e] * inv, x[m][2 * e + 1] * inv, w);
+#pragma unroll
+                    for (int c = 0; c < P; c++) qf[nt][m][e >> 1][c][e & 1] = w[c];
+                }
+        }
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const int r = row0 + nt * 8 + 2 * t + e;
+            lim[nt][e] = r < rows ? at.past + r / group + 1 : 0;
+        }
+    }
+    // whether the row of column e sees a slot of the tile's range
+    const auto sees = [&](int nt, int e, int slot) {
+        const int j = slot - at.past;
+        bool ok = slot >= first && slot < lim[nt][e];
+        if (tree && ok && j >= 0) ok = above[nt * 8 + 2 * t + e][j >> 5] >> (j & 31) & 1;
+        return ok;
+    };
+
+    float o[VC][4][NT][4] = {}, m[NT][2], l[NT][2] = {};
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) m[nt][0] = m[nt][1] = -INFINITY;
+    for (; grp < to; grp += WARPS) {
+        const int slot = grp * KEYS, here = page;
+        float s[NT][4] = {};
+#pragma unroll
+        for (int c = P - 1; c >= 0; c--)  // (the small pieces first)
+#pragma unroll
+            for (int k = 0; k < KC; k++)
+#pragma unroll
+                for (int hf = 0; hf < 2; hf++)
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+                        mma(H(), s[nt], word(kr[0][k], 2 * hf), word(kr[1][k], 2 * hf), word(kr[0][k], 2 * hf + 1),
+                            word(kr[1][k], 2 * hf + 1), qf[nt][k][hf][c][0], qf[nt][k][hf][c][1]);
+        const int next = grp + WARPS;
+        if (++it == 32) {
+            it = 0;
+            look(next);
+        }
+        page = __shfl_sync(0xffffffffu, pages, it);
+        if (next < to) load_k(page, next * KEYS);
+
+        const bool edge = slot < first || slot + KEYS > rg.seen_by_all || here < 0;
+        bool dirty = false;
+        if (edge) {
+            // values that no row sees count for nothing, whatever they are; of those that some see, what is infinite
+            // or NaN comes in by itself below
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const int key = slot + 2 * t + (u & 1) + (u >> 1) * 8;
+                const bool none = key < first || key >= rg.end || here < 0;
+#pragma unroll
+                for (int c = 0; c < VC; c++) {
+                    uint4& w = vr[c][u];
+                    if (none) w = make_uint4(0, 0, 0, 0);
+                    const uint4 f = make_uint4(finite(w.x, EXP), finite(w.y, EXP), finite(w.z, EXP), finite(w.w, EXP));
+                    dirty |= f.x != w.x || f.y != w.y || f.z != w.z || f.w != w.w;
+                    w = f;
+                }
+            }
+            dirty = __any_sync(0xffffffffu, dirty);
+        }
+        uint32_t pt[NT][2][P];
+        float keep[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                s[nt][e] *= unit[nt][e & 1];
+                if (edge && (here < 0 || !sees(nt, e & 1, slot + g + (e >> 1) * 8))) s[nt][e] = -INFINITY;
+            }
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                float top = fmaxf(s[nt][e], s[nt][2 + e]);
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                top = fmaxf(top, m[nt][e]);
+                const float base = top == -INFINITY ? 0.f : top;
+                keep[nt][e] = exp2_approx(m[nt][e] - base);
+                m[nt][e] = top;
+                s[nt][e] = exp2_approx(s[nt][e] - base + SHIFT);
+                s[nt][2 + e] = exp2_approx(s[nt][2 + e] - base + SHIFT);
+            }
+#pragma unroll
+            for (int hf = 0; hf < 2; hf++) {
+                uint32_t w[P];
+                if constexpr (RAW) {
+                    __nv_bfloat162 x = __floats2bfloat162_rn(s[nt][hf * 2], s[nt][hf * 2 + 1]);
+                    w[0] = *reinterpret_cast<uint32_t*>(&x);
+                    s[nt][hf * 2] = __uint_as_float(w[0] << 16);
+                    s[nt][hf * 2 + 1] = __uint_as_float(w[0] & 0xffff0000u);
+                } else {
+                    pieces_of<P>(s[nt][hf * 2], s[nt][hf * 2 + 1], w);
+                }
+#pragma unroll
+                for (int c = 0; c < P; c++) pt[nt][hf][c] = transpose8x8(w[c]);
+            }
+#pragma unroll
+            for (int e = 0; e < 2; e++) l[nt][e] = l[nt][e] * keep[nt][e] + (s[nt][e] + s[nt][2 + e]);
+        }
+#pragma unroll
+        for (int c = 0; c < VC; c++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const uint32_t w0 = word(vr[c][0], r), w1 = word(vr[c][1], r), w2 = word(vr[c][2], r), w3 = word(vr[c][3], r);
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    // a group's sums start from zero and are added rounded: the tensor cores truncate theirs
+                    float sum[4] = {};
+#pragma unroll
+                    for (int k = P - 1; k >= 0; k--)
+                        mma(H(), sum, __byte_perm(w0, w1, 0x5410), __byte_perm(w0, w1, 0x7632), __byte_perm(w2, w3, 0x5410),
+                            __byte_perm(w2, w3, 0x7632), pt[nt][0][k], pt[nt][1][k]);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) o[c][r][nt][e] = o[c][r][nt][e] * keep[nt][e & 1] + sum[e];
+                }
+            }
+        if (next < to) load_v(page, next * KEYS);
+        if (dirty) {
+            // an infinity stays one in the sum of all that see it, a NaN too
+            for (int key = max(slot, first); key < min(slot + KEYS, rg.end); key++) {
+                const uint16_t* src = vd + row_at(p.c, here, h, key) + g * 8;
+#pragma unroll
+                for (int c = 0; c < VC; c++) {
+                    const uint4 w = load_cached(src + c * 64);
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const uint32_t x = word(w, r);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const uint16_t bits = e >> 1 ? x >> 16 : x & 0xffffu;
+                            if ((bits & EXP) != EXP) continue;
+#pragma unroll
+                            for (int nt = 0; nt < NT; nt++)
+                                if (sees(nt, e & 1, key)) o[c][r][nt][e] += paged::up(*reinterpret_cast<const H*>(&bits));
+                        }
+                    }
+                }
+            }
+        }
+    }
+
+    // the warp's state: sums over the lanes; O in units of 2^-SHIFT, as l
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            float sum = l[nt][e];
+            sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+            const int r = nt * 8 + 2 * t + e;
+            if (g == 0) state[warp][r] = make_float2(m[nt][e], sum);
+#pragma unroll
+            for (int c = 0; c < VC; c++)
+#pragma unroll
+                for (int k = 0; k < 4; k += 2)
+                    *reinterpret_cast<float4*>(&sm_o[warp][r][c * 64 + g * 8 + k * 2]) =
+                        make_float4(o[c][k][nt][e], o[c][k][nt][2 + e], o[c][k + 1][nt][e], o[c][k + 1][nt][2 + e]);
+        }
+    __syncthreads();
+    if (threadIdx.x < R) {
+        const int r = threadIdx.x;
+        const Sum x = weigh(WARPS, [&](int w) { return state[w][r]; }, &weight[0][r], R);
+        merged[r] = make_float2(x.m, x.l);
+        inv_l[r] = x.l == 0.f ? 0.f : 1.f / x.l;
+    }
+    __syncthreads();
+    // a thread has the same four columns of every row it takes
+    constexpr int ROWS_AT_ONCE = 32 * WARPS / (D / 4);
+    const int live = min(R, rows - row0), c4 = threadIdx.x % (D / 4) * 4, r0 = threadIdx.x / (D / 4);
+    T* out = static_cast<T*>(const_cast<void*>(p.out.data)) + z + b * p.out.bs + (size_t)h * group * D + c4;
+    for (int r = r0; r < live; r += ROWS_AT_ONCE) {
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < WARPS; w++) add4(acc, weight[w][r], *reinterpret_cast<const float4*>(&sm_o[w][r][c4]));
+        if (splits == 1) {
+            const int row = row0 + r, i = row / group;
+            store4(out + i * p.out.ts + (size_t)(row - i * group) * D, acc, inv_l[r], vec & 2);
+        } else if (clustered) {
+            *reinterpret_cast<float4*>(&sm_o[0][r][c4]) = acc;  // warp 0's, which no other thread reads
+        } else {
+            float* ws = p.ws + z + (((size_t)bh * gridDim.x + blockIdx.x) * R + r) * (D + 4);
+            *reinterpret_cast<float4*>(ws + 4 + c4) = acc;
+            if (c4 == 0) *reinterpret_cast<float2*>(ws) = merged[r];
+        }
+    }
+    if (splits == 1 || !clustered) return;
+    // the cluster's CTAs: row r's outputs are the CTA's of rank r modulo their number
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    if (threadIdx.x < R) {
+        const int r = threadIdx.x;
+        const Sum x = weigh(splits, [&](int s) { return *cluster.map_shared_rank(&merged[r], s); }, &weight[0][r], R);
+        inv_l[r] = x.l == 0.f ? 0.f : 1.f / x.l;
+    }
+    __syncthreads();
+    for (int r = split + splits * r0; r < live; r += splits * ROWS_AT_ONCE) {
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int s = 0; s < splits; s++)
+            add4(acc, weight[s][r], *reinterpret_cast<const float4*>(cluster.map_shared_rank(&sm_o[0][r][c4], s)));
+        const int row = row0 + r, i = row / group;
+        store4(out + i * p.out.ts + (size_t)(row - i * group) * D, acc, inv_l[r], vec & 2);
+    }
+    cluster.sync();  // the others have read this CTA's shared memory
+}
+
+// The splits' partials to the output, G * D / 4 threads to a row: each of the G groups sums every G-th split, and the
+// groups' sums meet in shared memory.
+template <typename T, int D, int G>
+__global__ void __launch_bounds__(256) paged_combine_kernel(PagedAttn p, int splits, int R, int vec) {
+    chain_release();
+    const int z = chain_wait();
+    constexpr int TO_ROW = G * D / 4, ROWS = 256 / TO_ROW;
+    static_assert(ROWS >= 1 && (G == 1 || ROWS == 1), "whole rows, or one to the CTA");
+    __shared__ int parent[MOST_TREE];
+    __shared__ float top_of[G];
+    __shared__ float sum_of[G];
+    __shared__ float4 sums[G][D / 4];
+    const int bh = blockIdx.y, b = bh / p.c.n_head_kv, h = bh - b * p.c.n_head_kv, group = p.n_head / p.c.n_head_kv;
+    const int row = blockIdx.x * ROWS + threadIdx.x / TO_ROW, sub = threadIdx.x % TO_ROW / (D / 4), c = threadIdx.x % (D / 4);
+    const Place at = place_of(p.s, b, p.c.room, nullptr);
+    if (p.s.first && __ldcg(p.s.first + b + z) < 0) return;
+    if (p.tree.parent && !read_tree(p.tree, b, at.count, z, parent)) return;
+    const bool live = row < at.count * group;
+    if (G > 1 ? !live : blockIdx.x * ROWS >= at.count * group) return;
+    const int tiles = (p.s.n * group + R - 1) / R;
+    const size_t step = (size_t)R * (D + 4);
+    const float* ws = p.ws + z + ((size_t)bh * tiles + row / R) * splits * step + (row % R) * (D + 4);
+    float mx = -INFINITY;
+    if (live)
+#pragma unroll 8
+        for (int s = sub; s < splits; s += G) mx = fmaxf(mx, __ldcg(ws + s * step));
+    if (G > 1) {
+        if (c == 0) top_of[sub] = mx;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < G; w++) mx = fmaxf(mx, top_of[w]);
+    }
+    const float base = mx == -INFINITY ? 0.f : mx;
+    float sum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (live)
+#pragma unroll 8
+        for (int s = sub; s < splits; s += G) {
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(ws + s * step));
+            const float f = exp2_approx(ml.x - base);
+            sum += ml.y * f;
+            add4(acc, f, __ldcg(reinterpret_cast<const float4*>(ws + s * step + 4) + c));
+        }
+    if (G > 1) {
+        if (c == 0) sum_of[sub] = sum;
+        sums[sub][c] = acc;
+        __syncthreads();
+        if (sub > 0) return;
+#pragma unroll
+        for (int w = 1; w < G; w++) {
+            sum += sum_of[w];
+            add4(acc, 1.f, sums[w][c]);
+        }
+    }
+    if (!live) return;
+    const int i = row / group;
+    T* out = static_cast<T*>(const_cast<void*>(p.out.data)) + z + b * p.out.bs + i * p.out.ts +
+             (size_t)(h * group + row - i * group) * D + c * 4;
+    store4(out, acc, sum == 0.f ? 0.f : 1.f / sum, vec & 2);
+}
+
+struct Plan {
+    int tile_rows, tiles;  // query rows of a tile, tiles of a (sequence, kv head)
+    int splits;            // cuts of the keys
+    size_t ws;             // floats of workspace, for this and shorter caches
+};
+
+// Clusters of n CTAs that run at once on the current device: a cluster lives in one GPC, and the GPCs have different
+// numbers of SMs. Asked once for each device.
+template <int NT>
+int ask_clusters(int n) {
+    const auto kern = paged_split_kernel<float, 128, NT, 2>;  // the others need no more than it
+    static std::atomic<uint64_t> done{0};
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)n);
+    cfg.blockDim = dim3(32 * WARPS);
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)n;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int count = 0;
+    if (allow_smem(done, (const void*)kern, 0, true) != cudaSuccess || cudaOccupancyMaxActiveClusters(&count, kern, &cfg) != cudaSuccess)
+        (void)cudaGetLastError();
+    return count;
+}
+int clusters_at_once(int tile_rows, int n) {
+    static std::atomic<int> known[64][2][MAX_CLUSTER + 1];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 1;
+    std::atomic<int>& at = known[dev & 63][tile_rows == 8][n];
+    int count = at.load(std::memory_order_relaxed);
+    if (count == 0) at.store(count = std::max(1, tile_rows == 8 ? ask_clusters<1>(n) : ask_clusters<2>(n)), std::memory_order_relaxed);
+    return count;
+}
+
+// Slots that the longest sequence can have at the call's end.
+int keys_of(const Paged& c, const Seqs& s) { return (int)std::min<long long>((long long)s.n_past + s.n, c.room); }
+
+Plan plan_for(const Paged& c, const Seqs& s, int n_head, int sm_count) {
+    const int rows = s.n * (n_head / c.n_head_kv);
+    Plan p{};
+    p.tile_rows = rows <= 8 ? 8 : 16;
+    p.tiles = (rows + p.tile_rows - 1) / p.tile_rows;
+    const long long ctas = (long long)s.n_batch * c.n_head_kv * p.tiles, places = (long long)sm_count * (p.tile_rows == 8 ? 3 : 2);
+    const int groups = (keys_of(c, s) + KEYS - 1) / KEYS, useful = (groups + WARPS - 1) / WARPS;
+    const int most = (int)std::min<long long>(useful, std::max<long long>(1, places / ctas));
+    int in_cluster = std::min(MAX_CLUSTER, most);
+    while (in_cluster > 1 && ctas > clusters_at_once(p.tile_rows, in_cluster)) in_cluster--;
+    p.splits = in_cluster;
+    const auto rounds = [&](int n) { return (useful + n - 1) / n; };
+    if (most > MAX_CLUSTER && rounds(most) + 6 < rounds(in_cluster)) p.splits = most;
+    if (places / ctas > MAX_CLUSTER) p.ws = (size_t)ctas * most * p.tile_rows * (c.d + 4);
+    return p;
+}
+
+template <typename T, int D, int NT, int P>
+int split_launch(const PagedAttn& p, const Plan& plan, int vec, cudaStream_t st) {
+    const float scale = (float)(1.0 / sqrt((double)D)) * kLog2e;
+    const int clustered = plan.splits <= MAX_CLUSTER;
+    const auto kern = paged_split_kernel<T, D, NT, P>;
+    static std::atomic<uint64_t> done{0};
+    if (allow_smem(done, (const void*)kern, 0, true) != cudaSuccess) return -1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(plan.tiles * plan.splits), (unsigned)(p.s.n_batch * p.c.n_head_kv));
+    cfg.blockDim = dim3(32 * WARPS);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = clustered ? (unsigned)plan.splits : 1;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, kern, p, plan.splits, clustered, vec, scale) == cudaSuccess ? 0 : -1;
+}
+
+template <typename T, int D>
+int combine(const PagedAttn& p, const Plan& plan, int vec, int sm_count, cudaStream_t st) {
+    const int rows = p.s.n * (p.n_head / p.c.n_head_kv);
+    const unsigned segs = (unsigned)(p.s.n_batch * p.c.n_head_kv);
+    constexpr int G = 1024 / D;
+    cudaError_t e;
+    if ((long long)rows * segs > 8 * sm_count)  // more than a CTA to a row fits at once
+        e = launch_chained(paged_combine_kernel<T, D, 1>, dim3((unsigned)(rows + G - 1) / G, segs), dim3(256), st, p, plan.splits, plan.tile_rows, vec);
+    else
+        e = launch_chained(paged_combine_kernel<T, D, G>, dim3((unsigned)rows, segs), dim3(256), st, p, plan.splits, plan.tile_rows, vec);
+    return e == cudaSuccess ? 0 : -1;
+}
+
+template <typename T, int D, int P>
+int attn(const PagedAttn& p, int sm_count, cudaStream_t st) {
+    const Plan plan = plan_for(p.c, p.s, p.n_head, sm_count);
+    const int vec = (wide(p.q, sizeof(T), 16) ? 1 : 0) | (wide(p.out, sizeof(T), 4 * sizeof(T)) ? 2 : 0);
+    int rc = plan.tile_rows == 8 ? split_launch<T, D, 1, P>(p, plan, vec, st) : split_launch<T, D, 2, P>(p, plan, vec, st);
+    if (rc == 0 && plan.splits > MAX_CLUSTER) rc = combine<T, D>(p, plan, vec, sm_count, st);
+    return rc;
+}
+
+}  // namespace
+
+size_t paged_attn_workspace_bytes(const Paged& c, const Seqs& s, int n_head, int sm_count) {
+    if (s.n_batch == 0 || s.n == 0) return 0;
+    return plan_for(c, s, n_head, sm_count).ws * sizeof(float);
+}
+
+int paged_attn_launch(const PagedAttn& p, int type, int pieces, int sm_count, cudaStream_t st) {
+    if (p.s.n_batch == 0 || p.s.n == 0) return 0;
+    if (type == TYPE_BF16) return p.c.d == 64 ? attn<__nv_bfloat16, 64, 1>(p, sm_count, st) : attn<__nv_bfloat16, 128, 1>(p, sm_count, st);
+    if (pieces == 1) return p.c.d == 64 ? attn<float, 64, 1>(p, sm_count, st) : attn<float, 128, 1>(p, sm_count, st);
+    return p.c.d == 64 ? attn<float, 64, 2>(p, sm_count, st) : attn<float, 128, 2>(p, sm_count, st);
+}
+
+}  // namespace zwg

@@ -1070,6 +1070,191 @@ class Kv8Cache:
         return out
 
 
+def _tree(tree, n_batch: int, n: int, device):
+    """A reference to the zwg_tree of parents [n] (of all sequences) or [n_batch][n]; None: none."""
+    if tree is None:
+        return None
+    torch = _torch()
+    if not isinstance(tree, torch.Tensor) or tree.dtype is not torch.int32 or tree.device != device:
+        raise ValueError(f"tree must be an int32 tensor on {device}")
+    shape, strides = tree.shape, tree.stride()
+    if shape != (n,) and shape != (n_batch, n):
+        raise ValueError(f"tree must have shape ({n},) or ({n_batch}, {n}), got {tuple(shape)}")
+    if n > 1 and strides[-1] != 1:
+        raise ValueError("a tree's parents must lie one after another")
+    if n > _lib.ZWG_MAX_TREE:
+        raise ValueError(f"a tree of {n} tokens, at most {_lib.ZWG_MAX_TREE} are taken")
+    return ctypes.byref(_lib.TreeC(tree.data_ptr(), strides[0] if len(shape) == 2 else 0))
+
+
+class PagedCache:
+    """A key/value cache in pages (zwg_paged): K and V [n_pages][n_head_kv][page][d], both float16
+    (for f32 rows) or both bfloat16 (for bf16 rows), d 64 or 128, page a power of two from 16 to 256, and
+    an int32 table [n_batch][max_pages] of each sequence's pages (-1: none yet). CUDA tensors on one
+    device, which the cache keeps; a page's rows lie one after another, pages any distance apart that K and
+    V share, the table's rows too. Who hands out pages writes their numbers into the table before
+    the call that needs them."""
+
+    def __init__(self, k, v, table):
+        torch = _torch()
+        if k.dim() != 4 or not k.is_cuda:
+            raise ValueError("k must be a CUDA tensor [n_pages][n_head_kv][page][d]")
+        if k.dtype is not torch.float16 and k.dtype is not torch.bfloat16:
+            raise ValueError(f"k must be float16 or bfloat16, got {k.dtype}")
+        pages, heads, page, d = shape = k.shape
+        strides = k.stride()
+        if v.shape != shape or v.dtype is not k.dtype or v.device != k.device or (pages > 1 and v.stride(0) != strides[0]):
+            raise ValueError(f"v must be {k.dtype} of shape {tuple(shape)} on {k.device}, its pages as far apart as k's")
+        for name, t in (("k", k), ("v", v)):
+            if not t[0].is_contiguous():
+                raise ValueError(f"a page of {name} must be contiguous")
+        if table.dim() != 2 or table.dtype is not torch.int32 or table.device != k.device:
+            raise ValueError(f"table must be an int32 tensor [n_batch][max_pages] on {k.device}")
+        B, most = table.shape
+        if most > 1 and table.stride(1) != 1:
+            raise ValueError("a sequence's pages must lie one after another")
+        self.k, self.v, self.table, self.device = k, v, table, k.device
+        self.n_batch, self.n_head_kv, self.d, self.page, self.n_ctx = B, heads, d, page, most * page
+        self._row_dtype = torch.float32 if k.dtype is torch.float16 else torch.bfloat16
+        self._c = _lib.PagedC(k.data_ptr(), v.data_ptr(),
+                              _lib.ZWG_TYPE_F16 if k.dtype is torch.float16 else _lib.ZWG_TYPE_BF16, table.data_ptr(),
+                              table.stride(0), B, heads, d, page, pages, most,
+                              strides[0] if pages > 1 else heads * page * d)
+        self._ref = ctypes.byref(self._c)
+
+    @classmethod
+    def empty(cls, n_pages: int, n_batch: int, n_head_kv: int, d: int, page: int, n_ctx: int, dtype=None,
+              device: int = 0) -> "PagedCache":
+        """A cache with a pool of n_pages and a table without pages, for up to n_ctx tokens a sequence.
+        dtype: torch.float16 (None) or torch.bfloat16."""
+        torch = _torch()
+        dev, dtype = torch.device("cuda", device), torch.float16 if dtype is None else dtype
+        k = torch.zeros(n_pages, n_head_kv, page, d, dtype=dtype, device=dev)
+        return cls(k, torch.zeros_like(k), torch.full((n_batch, -(-n_ctx // page)), -1, dtype=torch.int32, device=dev))
+
+    def _call(self, n: int, n_past, count, first, max_past):
+        return _seqs(self.n_batch, n, n_past, count, first, self.n_ctx if max_past is None else max_past, self.device)
+
+    def _check_rows(self, t, name):
+        kind = _row_type(t, name)
+        if t.dim() != 4:
+            raise ValueError(f"{name} must be [n_batch][n][heads][d]")
+        if t.dtype is not self._row_dtype:
+            raise ValueError(f"{name} must be {self._row_dtype} beside a {self.k.dtype} cache, got {t.dtype}")
+        return kind
+
+    def append(self, k, v, n_past, count=None, rope=None, tree=None, q=None, q_out=None, max_past=None):
+        """Append k, v [n_batch][n][n_head_kv][d] (zwg_paged_append) at n_past (an int, or a CUDA int32
+        tensor [n_batch] whose entries are at most max_past; None: the cache's end, or the tables'); count
+        (CUDA int32 [n_batch]): tokens of each sequence. rope: (cos, sin) or (cos, sin, interleaved), the
+        rotation of k on its way in, and of q [n_batch][n][n_head][d], where given, into q_out (None: in
+        place). tree: parents of the call's tokens (CUDA int32 [n] or [n_batch][n], -1 or an earlier token), which
+        then stand at the positions of their depths. Returns the rotated q."""
+        kind = self._check_rows(k, "k")
+        dev, dtype, n = self.device, k.dtype, k.shape[1]
+        shape = (self.n_batch, n, self.n_head_kv, self.d)
+        t = None if rope is None else _tables(rope[0], rope[1], dev, len(rope) > 2 and rope[2])
+        kr, vr = _rows(k, dtype, dev, shape, "k"), _rows(v, dtype, dev, shape, "v")
+        qr = qo = None
+        H = 0
+        if q is not None:
+            if q.dim() != 4:
+                raise ValueError("q must be [n_batch][n][n_head][d]")
+            H = q.shape[2]
+            q_shape = (self.n_batch, n, H, self.d)
+            qr = _rows(q, dtype, dev, q_shape, "q")
+            if q_out is not None:
+                qo = _rows(q_out, dtype, dev, q_shape, "q_out")
+        elif q_out is not None:
+            raise ValueError("q_out without q")
+        if max_past is None and rope is not None:
+            max_past = min(self.n_ctx, rope[0].shape[0])
+        s = self._call(n, n_past, count, None, max_past)
+        _lib.check(_ready(dev).zwg_paged_append(self._ref, s, _tree(tree, self.n_batch, n, dev), kind, kr, vr, t, H, qr, qo,
+                                                _stream_on(dev)))
+        return q if q_out is None else q_out
+
+    def attn_workspace_bytes(self, n: int, n_head: int, n_past=None) -> int:
+        """Workspace of attn for n tokens after n_past (None: the most there can be)."""
+        s = self._call(n, max(self.n_ctx - n, 0) if n_past is None else n_past, None, None, None)
+        return int(_ready(self.device).zwg_paged_attn_workspace(self._ref, s, n_head))
+
+    def attn(self, q, n_past, count=None, first=None, tree=None, max_past=None, out=None, workspace=None):
+        """Attention (zwg_paged_attn) of q [n_batch][n][n_head][d] at n_past (an int, or a CUDA int32 tensor
+        [n_batch] whose entries are at most max_past) over the cache, which holds the call's own tokens already:
+        query i of sequence b sees slots first[b] .. n_past + i, or, with a tree (as in append), the past ones from
+        first[b] on, its own and those of the tokens above it (none: zeros). count, first: CUDA int32 [n_batch]; rows
+        of out behind count[b] stay as they are. workspace: a contiguous CUDA tensor of attn_workspace_bytes
+        (None: one is made). Returns out, of q's shape and type (a new one has zeros there)."""
+        torch = _torch()
+        kind = self._check_rows(q, "q")
+        n, H = q.shape[1], q.shape[2]
+        dev, dtype, shape = self.device, q.dtype, (self.n_batch, n, H, self.d)
+        qr = _rows(q, dtype, dev, shape, "q")
+        if out is not None:
+            o = _rows(out, dtype, dev, shape, "out")
+        else:
+            out, o = _new_rows(q, shape)
+            if count is not None:
+                out.zero_()
+        s, tr = self._call(n, n_past, count, first, max_past), _tree(tree, self.n_batch, n, dev)
+        lib = _ready(dev)
+        ws, size = None, 0
+        if workspace is None:
+            size = lib.zwg_paged_attn_workspace(self._ref, s, H)
+            if size:
+                workspace = torch.empty(size, dtype=torch.uint8, device=dev)
+                ws = workspace.data_ptr()
+        else:
+            if workspace.device != dev or not workspace.is_contiguous():
+                raise ValueError(f"workspace must be a contiguous tensor on {dev}")
+            ws, size = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        _lib.check(lib.zwg_paged_attn(self._ref, s, tr, kind, H, qr, o, ws, size, _stream_on(dev)))
+        return out
+
+
+def tree_accept(tokens, ids, tree, count=None, path=None, n_path=None, following=None):
+    """Which drafted tokens the model agrees with (zwg_tree_accept): tokens [n_batch][n] with their parents
+    `tree` (CUDA int32 [n] or [n_batch][n], -1 or an earlier token), ids [n_batch][n] the model's token after each
+    of them; count (CUDA int32 [n_batch]): tokens of each sequence. Returns (path, n_path, following): the agreed
+    tokens' indices [n_batch][n], token 0 first and -1 behind them, how many there are [n_batch], and
+    the model's token after the last one [n_batch] (CUDA int32, in the tensors given or new ones)."""
+    torch = _torch()
+    if not isinstance(tokens, torch.Tensor) or not tokens.is_cuda or tokens.dim() != 2:
+        raise ValueError("tokens must be a CUDA tensor [n_batch][n]")
+    B, n = shape = tokens.shape
+    dev = tokens.device
+    if tree is None:
+        raise ValueError("tree must be given")
+    args = [_int32_of(tokens, dev, shape, "tokens"), _int32_of(ids, dev, shape, "ids")]
+    path = torch.empty_like(tokens) if path is None else path
+    n_path = tokens.new_empty(B) if n_path is None else n_path
+    following = tokens.new_empty(B) if following is None else following
+    args += [_int32_of(path, dev, shape, "path"), _int32_of(n_path, dev, (B,), "n_path"),
+             _int32_of(following, dev, (B,), "following")]
+    s = _seqs(B, n, 0, count, None, None, dev)
+    _lib.check(_ready(dev).zwg_tree_accept(s, _tree(tree, B, n, dev), *args, _stream_on(dev)))
+    return path, n_path, following
+
+
+def paged_keep(caches, path, n_path, n_past, max_past=None) -> None:
+    """Move the rows of token path[b][j] of the last call at n_past to slot n_past + j, j < n_path[b]
+    (zwg_paged_keep, as tree_accept gives them), in one PagedCache or in several that share a table and sizes
+    (a model's layers)."""
+    torch = _torch()
+    caches = [caches] if isinstance(caches, PagedCache) else list(caches)
+    if not caches:
+        return
+    c = caches[0]
+    if not isinstance(path, torch.Tensor) or path.dim() != 2:
+        raise ValueError("path must be a CUDA int32 tensor [n_batch][n]")
+    n = path.shape[1]
+    args = (_int32_of(path, c.device, (c.n_batch, n), "path"), _int32_of(n_path, c.device, (c.n_batch,), "n_path"))
+    s = c._call(n, n_past, None, None, max_past)
+    all_of = (_lib.PagedC * len(caches))(*(x._c for x in caches))
+    _lib.check(_ready(c.device).zwg_paged_keep(all_of, len(caches), s, *args, _stream_on(c.device)))
+
+
 def llm_logits(logits, recent=None, n_recent=None, window: Optional[int] = None, repeat: float = 1.0,
                presence: float = 0.0, frequency: float = 0.0, bias_ids=None, bias=None, allow=None, out=None):
     """The rules on a step's logits (zwg_llm_logits), in place on CUDA f32 logits [m][n_vocab]:
