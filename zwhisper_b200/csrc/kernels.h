@@ -289,6 +289,7 @@ struct Paged {
     size_t ts, ps;         // table row; page, in elements
     int n_head_kv, d, log_page, n_pages;
     int room;              // slots a sequence's table has
+    int type;              // TYPE_F16 or TYPE_BF16
 };
 // Parents of a call's tokens (zwg_tree); parent null: each token's is the one before it.
 struct Tree {
@@ -338,6 +339,10 @@ struct PagedAttn {
 size_t paged_attn_workspace_bytes(const Paged& c, const Seqs& s, int n_head, int sm_count);
 // type: of the rows; pieces: f16 pieces of an f32 query and its probabilities, 1 or 2.
 int paged_attn_launch(const PagedAttn& p, int type, int pieces, int sm_count, cudaStream_t st);
+
+// Its tcgen05 kernel for many query rows of a kv head (paged_chunk.cu), `splits` cuts of the keys.
+constexpr int PAGED_CHUNK_ROWS = 256, PAGED_CHUNK_KEYS = 128;  // of a tile
+int paged_chunk_launch(const PagedAttn& p, int type, int pieces, int splits, cudaStream_t st);
 
 // Penalties, biases, mask and argmax on rows of logits (logits.cu).
 struct LogitRules {

@@ -32,6 +32,9 @@ ZWG_DEV float up(float x) { return x; }
 ZWG_DEV float up(__half x) { return __half2float(x); }
 ZWG_DEV float up(__nv_bfloat16 x) { return __bfloat162float(x); }
 
+ZWG_DEV void add(float& x, float y) { x += y; }
+ZWG_DEV void add(__nv_bfloat16& x, float y) { x = __float2bfloat16_rn(__bfloat162float(x) + y); }
+
 // The page of sequence b's slot (below c.room), or -1: the table's entry is not one of the pool's.
 ZWG_DEV int page_of(const Paged& c, int b, int slot) {
     const int id = __ldcg(c.table + b * c.ts + (slot >> c.log_page));
@@ -45,12 +48,13 @@ ZWG_DEV size_t row_at(const Paged& c, int page, int h, int slot) {
 
 // The whole CTA: the parents of a sequence's `count` tokens (at most MOST_TREE) into shared memory, and whether
 // each is below its own index. One that is not leaves the sequence out.
-ZWG_DEV bool read_tree(const Tree& t, int b, int count, int z, int* parent) {
+template <typename I>
+ZWG_DEV bool read_tree(const Tree& t, int b, int count, int z, I* parent) {
     int bad = 0;
     const int n = blockDim.x * blockDim.y * blockDim.z;
     for (int i = threadIdx.x + blockDim.x * (threadIdx.y + blockDim.y * threadIdx.z); i < count; i += n) {
         const int a = __ldcg(t.parent + b * t.bs + i + z);
-        parent[i] = a;
+        parent[i] = (I)a;  // (where it is not bad, below MOST_TREE)
         bad |= a < -1 || a >= i;
     }
     return __syncthreads_or(bad) == 0;

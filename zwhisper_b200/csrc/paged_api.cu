@@ -63,7 +63,7 @@ zwg::Paged cache_of(const zwg_paged* c) {
     int log_page = 4;
     while (((size_t)1 << log_page) < c->page) log_page++;
     return zwg::Paged{c->k, c->v, c->table, c->table_stride, c->page_stride, (int)c->n_head_kv, (int)c->d, log_page,
-                      (int)c->n_pages, (int)room_of(c)};
+                      (int)c->n_pages, (int)room_of(c), c->type == ZWG_TYPE_BF16 ? zwg::TYPE_BF16 : zwg::TYPE_F16};
 }
 
 zwg::Tree tree_of(const zwg_tree* t) { return t ? zwg::Tree{t->parent, t->batch_stride} : zwg::Tree{nullptr, 0}; }

@@ -516,7 +516,10 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(PagedAttn p, int spl
 struct Plan {
     int tile_rows, tiles;  // query rows of a tile, tiles of a (sequence, kv head)
     int splits;            // cuts of the keys
+    bool chunk;            // the tcgen05 kernel's
     size_t ws;             // floats of workspace, for this and shorter caches
+    float us;              // about how long it takes, for the choice between the kernels
+    int in_place() const { return chunk ? 1 : MAX_CLUSTER; }  // cuts that need no workspace
 };
 
 // Clusters of n CTAs that run at once on the current device: a cluster lives in one GPC, and the GPCs have different
@@ -552,21 +555,61 @@ int clusters_at_once(int tile_rows, int n) {
 // Slots that the longest sequence can have at the call's end.
 int keys_of(const Paged& c, const Seqs& s) { return (int)std::min<long long>((long long)s.n_past + s.n, c.room); }
 
-Plan plan_for(const Paged& c, const Seqs& s, int n_head, int sm_count) {
-    const int rows = s.n * (n_head / c.n_head_kv);
+// How often SMs are filled: the last time counts half of itself and half of a whole one.
+float waves_of(long long ctas, long long places) {
+    const float w = (float)ctas / places, whole = std::floor(w);
+    return w <= 1.f ? 1.f : whole == w ? w : whole + 0.5f + 0.5f * (w - whole);
+}
+
+Plan plan_split(const Paged& c, const Seqs& s, int rows, bool raw, int sm_count) {
     Plan p{};
-    p.tile_rows = rows <= 8 ? 8 : 16;
+    p.tile_rows = rows <= 8 ? 8 : 16;  // one or two 8-wide N tiles
     p.tiles = (rows + p.tile_rows - 1) / p.tile_rows;
     const long long ctas = (long long)s.n_batch * c.n_head_kv * p.tiles, places = (long long)sm_count * (p.tile_rows == 8 ? 3 : 2);
     const int groups = (keys_of(c, s) + KEYS - 1) / KEYS, useful = (groups + WARPS - 1) / WARPS;
+    const auto turns = [&](int n) { return (useful + n - 1) / n; };  // groups that follow each other in a warp
     const int most = (int)std::min<long long>(useful, std::max<long long>(1, places / ctas));
+    // a cluster that waits for a place doubles the time
     int in_cluster = std::min(MAX_CLUSTER, most);
     while (in_cluster > 1 && ctas > clusters_at_once(p.tile_rows, in_cluster)) in_cluster--;
-    p.splits = in_cluster;
-    const auto rounds = [&](int n) { return (useful + n - 1) / n; };
-    if (most > MAX_CLUSTER && rounds(most) + 6 < rounds(in_cluster)) p.splits = most;
+    // more cuts than that where they save more turns than the second kernel costs
+    p.splits = most > MAX_CLUSTER && turns(most) + 2 < turns(in_cluster) ? most : in_cluster;
     if (places / ctas > MAX_CLUSTER) p.ws = (size_t)ctas * most * p.tile_rows * (c.d + 4);
+    const float turn = c.d == 64 ? raw ? 1.2f : 1.4f : raw ? 1.5f : 2.f;
+    p.us = waves_of(ctas * p.splits, places) * (4.f + turn * turns(p.splits)) + (p.splits > MAX_CLUSTER ? 4.f : p.splits > 1 ? 3.f : 1.f);
     return p;
+}
+
+// The tcgen05 kernel: keys are cut while SMs stay empty, two tiles of keys to a cut at least.
+Plan plan_chunk(const Paged& c, const Seqs& s, int rows, bool raw, int sm_count) {
+    Plan p{};
+    p.chunk = true;
+    p.tile_rows = PAGED_CHUNK_ROWS;
+    p.tiles = (rows + PAGED_CHUNK_ROWS - 1) / PAGED_CHUNK_ROWS;
+    const long long ctas = (long long)s.n_batch * c.n_head_kv * p.tiles;
+    const int key_tiles = (keys_of(c, s) + PAGED_CHUNK_KEYS - 1) / PAGED_CHUNK_KEYS;
+    p.splits = (int)std::min<long long>(std::max<long long>(1, sm_count / ctas), std::max(1, key_tiles / 2));
+    if (p.splits > 1) p.ws = (size_t)ctas * p.splits * p.tile_rows * (c.d + 4);
+    const bool two = rows > PAGED_CHUNK_ROWS / 2;
+    const float start = c.d == 64 ? raw ? 9.f : 11.f : raw ? 11.f : 16.f;
+    const float turn = c.d == 64 ? two ? raw ? 1.9f : 2.5f : raw ? 1.1f : 1.4f : two ? raw ? 2.5f : 5.4f : raw ? 1.9f : 2.5f;
+    p.us = waves_of(ctas * p.splits, sm_count) * (start + turn * ((key_tiles + p.splits - 1) / p.splits)) + (p.splits > 1 ? 2.f : 0.f);
+    return p;
+}
+
+// The tcgen05 kernel has four times the other one's rate and reads the keys once for 256 rows, not 16, but a CTA of it
+// takes 9 to 18 us to start and end. Above 16 rows the shorter estimate runs, its constants read off both kernels'
+// times for 24 to 256 rows a head, 1 to 64 sequences of 200 to 8000 tokens, both d, bf16 and f32: 16 sequences of 2000
+// tokens, d 128, bf16: 24 rows 17 us against the other's 18, 48 rows 27 against 20, 128 rows 45 against 21; one of
+// 2000 tokens: 128 rows 12.5 against 14.6. Up to 16 rows, where the other kernel reads the keys once too, it was never
+// the slower one by more than 5 %.
+Plan plan_for(const Paged& c, const Seqs& s, int n_head, bool raw, int sm_count) {
+    const int rows = s.n * (n_head / c.n_head_kv);
+    Plan split = plan_split(c, s, rows, raw, sm_count);
+    if (rows <= 16) return split;
+    Plan chunk = plan_chunk(c, s, rows, raw, sm_count);
+    split.ws = chunk.ws = std::max(split.ws, chunk.ws);
+    return split.us < chunk.us ? split : chunk;
 }
 
 template <typename T, int D, int NT, int P>
@@ -606,10 +649,12 @@ int combine(const PagedAttn& p, const Plan& plan, int vec, int sm_count, cudaStr
 
 template <typename T, int D, int P>
 int attn(const PagedAttn& p, int sm_count, cudaStream_t st) {
-    const Plan plan = plan_for(p.c, p.s, p.n_head, sm_count);
+    const Plan plan = plan_for(p.c, p.s, p.n_head, sizeof(T) == 2, sm_count);
     const int vec = (wide(p.q, sizeof(T), 16) ? 1 : 0) | (wide(p.out, sizeof(T), 4 * sizeof(T)) ? 2 : 0);
-    int rc = plan.tile_rows == 8 ? split_launch<T, D, 1, P>(p, plan, vec, st) : split_launch<T, D, 2, P>(p, plan, vec, st);
-    if (rc == 0 && plan.splits > MAX_CLUSTER) rc = combine<T, D>(p, plan, vec, sm_count, st);
+    int rc = plan.chunk            ? paged_chunk_launch(p, sizeof(T) == 2 ? TYPE_BF16 : TYPE_F32, P, plan.splits, st)
+             : plan.tile_rows == 8 ? split_launch<T, D, 1, P>(p, plan, vec, st)
+                                   : split_launch<T, D, 2, P>(p, plan, vec, st);
+    if (rc == 0 && plan.splits > plan.in_place()) rc = combine<T, D>(p, plan, vec, sm_count, st);
     return rc;
 }
 
@@ -617,7 +662,7 @@ int attn(const PagedAttn& p, int sm_count, cudaStream_t st) {
 
 size_t paged_attn_workspace_bytes(const Paged& c, const Seqs& s, int n_head, int sm_count) {
     if (s.n_batch == 0 || s.n == 0) return 0;
-    return plan_for(c, s, n_head, sm_count).ws * sizeof(float);
+    return plan_for(c, s, n_head, c.type == TYPE_BF16, sm_count).ws * sizeof(float);
 }
 
 int paged_attn_launch(const PagedAttn& p, int type, int pieces, int sm_count, cudaStream_t st) {
