@@ -25,6 +25,7 @@
 #include "kv8_attn.cuh"
 #include "paged.cuh"
 #include "seqs.cuh"
+#include "sm100.cuh"
 
 namespace zwg {
 namespace {
@@ -41,8 +42,11 @@ using paged::page_of;
 using paged::read_tree;
 using paged::row_at;
 
-constexpr int WARPS = 4;         // of a CTA
-constexpr int KEYS = 16;         // of a warp at a time
+constexpr int SMALL = 4;         // warps of a small CTA; a big one has an SM to itself
+constexpr int big_warps(int tile_rows) { return tile_rows == 8 ? 12 : 8; }  // (two N tiles take twice the registers)
+constexpr int GROUP = 16;        // keys of a product, which lie in one page
+template <int D>
+constexpr int KEYS = GROUP * 128 / D;  // of a warp at a time: 4 KB of them and 4 KB of values
 constexpr int MAX_CLUSTER = 16;
 
 ZWG_DEV void mma(__half, float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -74,23 +78,6 @@ ZWG_DEV uint32_t finite(uint32_t w, uint32_t exponent) {
     return w;
 }
 
-// What each of n softmax states (m, l) weighs in their sum: f[i] = 2^(m_i - max), and the sum of l f.
-struct Sum {
-    float m, l;
-};
-template <typename M>
-ZWG_DEV Sum weigh(int n, M state, float* f, int step) {
-    Sum x{-INFINITY, 0.f};
-    for (int i = 0; i < n; i++) x.m = fmaxf(x.m, state(i).x);
-    const float base = x.m == -INFINITY ? 0.f : x.m;
-    for (int i = 0; i < n; i++) {
-        const float2 ml = state(i);
-        f[i * step] = exp2_approx(ml.x - base);
-        x.l += ml.y * f[i * step];
-    }
-    return x;
-}
-
 ZWG_DEV void add4(float4& a, float f, float4 x) {
     a.x += f * x.x;
     a.y += f * x.y;
@@ -98,11 +85,31 @@ ZWG_DEV void add4(float4& a, float f, float4 x) {
     a.w += f * x.w;
 }
 
-// The groups of 16 keys [from, to) of a split: the tile's keys first .. past + (the last row's token).
+// The sum of n partial results of a row: their states (m, l) and a piece of each one's O, weighed by 2^(m - the largest).
+struct Sum {
+    float m, l;
+    float4 o;
+};
+template <typename M, typename O>
+ZWG_DEV Sum sum_of(int n, M state, O piece) {
+    Sum x{-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+    for (int i = 0; i < n; i++) x.m = fmaxf(x.m, state(i).x);
+    const float base = x.m == -INFINITY ? 0.f : x.m;
+#pragma unroll 4
+    for (int i = 0; i < n; i++) {
+        const float2 ml = state(i);
+        const float f = exp2_approx(ml.x - base);
+        x.l += ml.y * f;
+        add4(x.o, f, piece(i));
+    }
+    return x;
+}
+
+// The turns [from, to) of a split, KEYS slots each: the tile's keys first .. past + (the last row's token).
 struct Range {
     int rows, row0, seen_by_all, end, from, to;
 };
-template <int R>
+template <int R, int KEYS>
 ZWG_DEV Range range_of(Place at, int first, int group, int tile, int split, int splits, bool tree) {
     Range r;
     r.rows = at.count * group;
@@ -117,18 +124,20 @@ ZWG_DEV Range range_of(Place at, int first, int group, int tile, int split, int 
     return r;
 }
 
-template <typename T, int D, int NT, int P>
-__global__ void __launch_bounds__(32 * WARPS, NT == 1 ? 3 : 2)
+// Rows of a cluster's merge: row r's is CTA r % splits, which has a place for every CTA's part of each of its own.
+__host__ __device__ constexpr int rows_of_rank(int R, int splits) { return (R + splits - 1) / splits; }
+
+template <typename T, int D, int NT, int P, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS, big_warps(8 * NT) / WARPS)
     paged_split_kernel(PagedAttn p, int splits, int clustered, int vec, float scale) {
     chain_release();
     using H = typename Held<T>::type;
-    constexpr int R = 8 * NT, LDO = D + 4, KC = D / 32, VC = D / 64;
+    constexpr int R = 8 * NT, LDO = D + 4, KC = D / 32, VC = D / 64, TURN = KEYS<D>, U = TURN / GROUP;
     constexpr bool RAW = sizeof(T) == 2;        // queries as they are
     constexpr float SHIFT = RAW ? 0.f : 15.f;   // probabilities in units of 2^-15: their f16 pieces stay normal
     constexpr uint32_t EXP = Held<T>::exponent;
-    __shared__ __align__(16) float sm_o[WARPS][R][LDO];
-    __shared__ float2 state[WARPS][R], merged[R];
-    __shared__ float weight[MAX_CLUSTER][R], inv_l[R];
+    extern __shared__ __align__(16) float sm_o[];  // [WARPS][R][LDO], then a cluster's inbox [splits][its rows][LDO]
+    __shared__ float2 state[WARPS][R];
     __shared__ int parent[MOST_TREE];
     __shared__ uint32_t above[R][MOST_TREE / 32];  // a row's token and its ancestors
     const int tile = blockIdx.x / splits, split = blockIdx.x - tile * splits;
@@ -136,10 +145,24 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 ? 3 : 2)
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int group = p.n_head / p.c.n_head_kv;
     const bool lead = threadIdx.x == 0 && blockIdx.x == 0 && h == 0, tree = p.tree.parent != nullptr;
+    if (lane < 2 * U) {
+        // before the kernel ahead is through: a hint to L2 for the warp's first two turns, from places that
+        // kernel may still be changing (held within the cache, and read again below)
+        const Place hint{p.s.past ? min(max(__ldcg(p.s.past + b), 0), p.c.room - 1) : p.s.n_past,
+                         p.s.count ? min(max(__ldcg(p.s.count + b), 1), p.s.n) : p.s.n};
+        const Range r = range_of<R, TURN>(hint, p.s.first ? min(max(__ldcg(p.s.first + b), 0), p.c.room - 1) : 0, group, tile, split, splits, tree);
+        const int turn = r.from + warp + lane / U * WARPS, slot = turn * TURN + lane % U * GROUP;
+        const int page = turn < r.to && slot < p.c.room ? page_of(p.c, b, slot) : -1;
+        if (page >= 0) {
+            const size_t at = row_at(p.c, page, h, slot) * 2;
+            sm100::bulk_hint(static_cast<const char*>(p.c.k) + at, GROUP * D * 2);
+            sm100::bulk_hint(static_cast<const char*>(p.c.v) + at, GROUP * D * 2);
+        }
+    }
     const int z = chain_wait();
     const Place at = place_of(p.s, b, p.c.room, lead ? p.err : nullptr);
     const int first = p.s.first ? __ldcg(p.s.first + b + z) : 0;
-    const Range rg = range_of<R>(at, max(first, 0), group, tile, split, splits, tree);
+    const Range rg = range_of<R, TURN>(at, max(first, 0), group, tile, split, splits, tree);
     const int rows = rg.rows, row0 = rg.row0, to = rg.to;
     if (row0 >= rows) return;  // the same for every CTA of a cluster, as the next two
     if (first < 0) {
@@ -159,37 +182,49 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 ? 3 : 2)
         }
         __syncthreads();
     }
+    if (clustered) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // (waited for before the merge)
 
-    // the pages of the warp's next 32 groups, one in each lane
-    int grp = rg.from + warp, pages = 0, it = 0;
+    // the pages of the warp's next 32 groups of keys, one in each lane
+    int turn = rg.from + warp, pages = 0, it = 0;
     const auto look = [&](int from) {
-        const int mine = from + lane * WARPS;
-        pages = mine < to ? page_of(p.c, b, mine * KEYS + z) : 0;
+        const int mine = from + lane / U * WARPS, slot = mine * TURN + lane % U * GROUP;
+        pages = mine < to && slot < rg.end ? page_of(p.c, b, slot + z) : 0;
         if (pages < 0) set_error(p.err, kErrBounds);  // its keys are not seen
     };
-    uint4 kr[2][KC], vr[VC][4];
+    const auto page_in = [&](int (&page)[U]) {
+#pragma unroll
+        for (int u = 0; u < U; u++) page[u] = __shfl_sync(0xffffffffu, pages, it * U + u);
+    };
+    uint4 kr[U][2][KC], vr[U][VC][4];
     const uint16_t* const kd = static_cast<const uint16_t*>(p.c.k) + z;
     const uint16_t* const vd = static_cast<const uint16_t*>(p.c.v) + z;
-    const auto load_k = [&](int page, int slot) {
-        const uint16_t* src = kd + row_at(p.c, max(page, 0), h, slot) + g * D + t * 8;
+    const auto load_k = [&](const int (&page)[U], int slot) {
 #pragma unroll
-        for (int m = 0; m < KC; m++) {
-            kr[0][m] = load_cached(src + m * 32);
-            kr[1][m] = load_cached(src + 8 * D + m * 32);
+        for (int u = 0; u < U; u++) {
+            const uint16_t* src = kd + row_at(p.c, max(page[u], 0), h, slot + u * GROUP) + g * D + t * 8;
+#pragma unroll
+            for (int m = 0; m < KC; m++) {
+                kr[u][0][m] = load_cached(src + m * 32);
+                kr[u][1][m] = load_cached(src + 8 * D + m * 32);
+            }
         }
     };
-    const auto load_v = [&](int page, int slot) {
-        const uint16_t* src = vd + row_at(p.c, max(page, 0), h, slot) + 2 * t * D + g * 8;
+    const auto load_v = [&](const int (&page)[U], int slot) {
 #pragma unroll
-        for (int c = 0; c < VC; c++)
+        for (int u = 0; u < U; u++) {
+            const uint16_t* src = vd + row_at(p.c, max(page[u], 0), h, slot + u * GROUP) + 2 * t * D + g * 8;
 #pragma unroll
-            for (int u = 0; u < 4; u++) vr[c][u] = load_cached(src + ((u & 1) + (u >> 1) * 8) * D + c * 64);
+            for (int c = 0; c < VC; c++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) vr[u][c][k] = load_cached(src + ((k & 1) + (k >> 1) * 8) * D + c * 64);
+        }
     };
-    look(grp);
-    int page = __shfl_sync(0xffffffffu, pages, 0);
-    if (grp < to) {
-        load_k(page, grp * KEYS);
-        load_v(page, grp * KEYS);
+    look(turn);
+    int page[U];
+    page_in(page);
+    if (turn < to) {
+        load_k(page, turn * TURN);
+        load_v(page, turn * TURN);
     }
 
     // queries: the B operand, lane (g, t) holds row g's elements 8 t .. 8 t + 7 of each 32
@@ -264,59 +299,70 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 ? 3 : 2)
     float o[VC][4][NT][4] = {}, m[NT][2], l[NT][2] = {};
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) m[nt][0] = m[nt][1] = -INFINITY;
-    for (; grp < to; grp += WARPS) {
-        const int slot = grp * KEYS, here = page;
-        float s[NT][4] = {};
+    for (; turn < to; turn += WARPS) {
+        const int slot = turn * TURN, next = turn + WARPS;
+        int here[U];
+        float s[U][NT][4] = {};
 #pragma unroll
-        for (int c = P - 1; c >= 0; c--)  // (the small pieces first)
+        for (int u = 0; u < U; u++) {
+            here[u] = page[u];
 #pragma unroll
-            for (int k = 0; k < KC; k++)
+            for (int c = P - 1; c >= 0; c--)  // (the small pieces first)
 #pragma unroll
-                for (int hf = 0; hf < 2; hf++)
+                for (int k = 0; k < KC; k++)
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++)
-                        mma(H(), s[nt], word(kr[0][k], 2 * hf), word(kr[1][k], 2 * hf), word(kr[0][k], 2 * hf + 1),
-                            word(kr[1][k], 2 * hf + 1), qf[nt][k][hf][c][0], qf[nt][k][hf][c][1]);
-        const int next = grp + WARPS;
-        if (++it == 32) {
+                    for (int hf = 0; hf < 2; hf++)
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++)
+                            mma(H(), s[u][nt], word(kr[u][0][k], 2 * hf), word(kr[u][1][k], 2 * hf), word(kr[u][0][k], 2 * hf + 1),
+                                word(kr[u][1][k], 2 * hf + 1), qf[nt][k][hf][c][0], qf[nt][k][hf][c][1]);
+        }
+        if (++it == 32 / U) {
             it = 0;
             look(next);
         }
-        page = __shfl_sync(0xffffffffu, pages, it);
-        if (next < to) load_k(page, next * KEYS);
+        page_in(page);
+        if (next < to) load_k(page, next * TURN);
 
-        const bool edge = slot < first || slot + KEYS > rg.seen_by_all || here < 0;
-        bool dirty = false;
+        bool edge = slot < first || slot + TURN > rg.seen_by_all, dirty = false;
+#pragma unroll
+        for (int u = 0; u < U; u++) edge |= here[u] < 0;
         if (edge) {
             // values that no row sees count for nothing, whatever they are; of those that some see, what is infinite
             // or NaN comes in by itself below
 #pragma unroll
-            for (int u = 0; u < 4; u++) {
-                const int key = slot + 2 * t + (u & 1) + (u >> 1) * 8;
-                const bool none = key < first || key >= rg.end || here < 0;
+            for (int u = 0; u < U; u++)
 #pragma unroll
-                for (int c = 0; c < VC; c++) {
-                    uint4& w = vr[c][u];
-                    if (none) w = make_uint4(0, 0, 0, 0);
-                    const uint4 f = make_uint4(finite(w.x, EXP), finite(w.y, EXP), finite(w.z, EXP), finite(w.w, EXP));
-                    dirty |= f.x != w.x || f.y != w.y || f.z != w.z || f.w != w.w;
-                    w = f;
+                for (int k = 0; k < 4; k++) {
+                    const int key = slot + u * GROUP + 2 * t + (k & 1) + (k >> 1) * 8;
+                    const bool none = key < first || key >= rg.end || here[u] < 0;
+#pragma unroll
+                    for (int c = 0; c < VC; c++) {
+                        uint4& w = vr[u][c][k];
+                        if (none) w = make_uint4(0, 0, 0, 0);
+                        const uint4 f = make_uint4(finite(w.x, EXP), finite(w.y, EXP), finite(w.z, EXP), finite(w.w, EXP));
+                        dirty |= f.x != w.x || f.y != w.y || f.z != w.z || f.w != w.w;
+                        w = f;
+                    }
                 }
-            }
             dirty = __any_sync(0xffffffffu, dirty);
         }
-        uint32_t pt[NT][2][P];
+        uint32_t pt[U][NT][2][P];
         float keep[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                s[nt][e] *= unit[nt][e & 1];
-                if (edge && (here < 0 || !sees(nt, e & 1, slot + g + (e >> 1) * 8))) s[nt][e] = -INFINITY;
-            }
+            for (int u = 0; u < U; u++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    s[u][nt][e] *= unit[nt][e & 1];
+                    if (edge && (here[u] < 0 || !sees(nt, e & 1, slot + u * GROUP + g + (e >> 1) * 8))) s[u][nt][e] = -INFINITY;
+                }
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-                float top = fmaxf(s[nt][e], s[nt][2 + e]);
+                float top = fmaxf(s[0][nt][e], s[0][nt][2 + e]);
+#pragma unroll
+                for (int u = 1; u < U; u++) top = fmax3(top, s[u][nt][e], s[u][nt][2 + e]);
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
@@ -324,48 +370,63 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 ? 3 : 2)
                 const float base = top == -INFINITY ? 0.f : top;
                 keep[nt][e] = exp2_approx(m[nt][e] - base);
                 m[nt][e] = top;
-                s[nt][e] = exp2_approx(s[nt][e] - base + SHIFT);
-                s[nt][2 + e] = exp2_approx(s[nt][2 + e] - base + SHIFT);
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    s[u][nt][e] = exp2_approx(s[u][nt][e] - base + SHIFT);
+                    s[u][nt][2 + e] = exp2_approx(s[u][nt][2 + e] - base + SHIFT);
+                }
             }
 #pragma unroll
-            for (int hf = 0; hf < 2; hf++) {
-                uint32_t w[P];
-                if constexpr (RAW) {
-                    __nv_bfloat162 x = __floats2bfloat162_rn(s[nt][hf * 2], s[nt][hf * 2 + 1]);
-                    w[0] = *reinterpret_cast<uint32_t*>(&x);
-                    s[nt][hf * 2] = __uint_as_float(w[0] << 16);
-                    s[nt][hf * 2 + 1] = __uint_as_float(w[0] & 0xffff0000u);
-                } else {
-                    pieces_of<P>(s[nt][hf * 2], s[nt][hf * 2 + 1], w);
+            for (int u = 0; u < U; u++)
+#pragma unroll
+                for (int hf = 0; hf < 2; hf++) {
+                    uint32_t w[P];
+                    if constexpr (RAW) {
+                        __nv_bfloat162 x = __floats2bfloat162_rn(s[u][nt][hf * 2], s[u][nt][hf * 2 + 1]);
+                        w[0] = *reinterpret_cast<uint32_t*>(&x);
+                        s[u][nt][hf * 2] = __uint_as_float(w[0] << 16);
+                        s[u][nt][hf * 2 + 1] = __uint_as_float(w[0] & 0xffff0000u);
+                    } else {
+                        pieces_of<P>(s[u][nt][hf * 2], s[u][nt][hf * 2 + 1], w);
+                    }
+#pragma unroll
+                    for (int c = 0; c < P; c++) pt[u][nt][hf][c] = transpose8x8(w[c]);
                 }
 #pragma unroll
-                for (int c = 0; c < P; c++) pt[nt][hf][c] = transpose8x8(w[c]);
-            }
+            for (int e = 0; e < 2; e++) {
+                float sum = s[0][nt][e] + s[0][nt][2 + e];
 #pragma unroll
-            for (int e = 0; e < 2; e++) l[nt][e] = l[nt][e] * keep[nt][e] + (s[nt][e] + s[nt][2 + e]);
+                for (int u = 1; u < U; u++) sum += s[u][nt][e] + s[u][nt][2 + e];
+                l[nt][e] = l[nt][e] * keep[nt][e] + sum;
+            }
         }
 #pragma unroll
         for (int c = 0; c < VC; c++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const uint32_t w0 = word(vr[c][0], r), w1 = word(vr[c][1], r), w2 = word(vr[c][2], r), w3 = word(vr[c][3], r);
+            for (int r = 0; r < 4; r++)
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
-                    // a group's sums start from zero and are added rounded: the tensor cores truncate theirs
+                    // a turn's sums start from zero and are added rounded: the tensor cores truncate theirs
                     float sum[4] = {};
 #pragma unroll
-                    for (int k = P - 1; k >= 0; k--)
-                        mma(H(), sum, __byte_perm(w0, w1, 0x5410), __byte_perm(w0, w1, 0x7632), __byte_perm(w2, w3, 0x5410),
-                            __byte_perm(w2, w3, 0x7632), pt[nt][0][k], pt[nt][1][k]);
+                    for (int u = 0; u < U; u++) {
+                        const uint32_t w0 = word(vr[u][c][0], r), w1 = word(vr[u][c][1], r), w2 = word(vr[u][c][2], r), w3 = word(vr[u][c][3], r);
+#pragma unroll
+                        for (int k = P - 1; k >= 0; k--)
+                            mma(H(), sum, __byte_perm(w0, w1, 0x5410), __byte_perm(w0, w1, 0x7632), __byte_perm(w2, w3, 0x5410),
+                                __byte_perm(w2, w3, 0x7632), pt[u][nt][0][k], pt[u][nt][1][k]);
+                    }
 #pragma unroll
                     for (int e = 0; e < 4; e++) o[c][r][nt][e] = o[c][r][nt][e] * keep[nt][e & 1] + sum[e];
                 }
-            }
-        if (next < to) load_v(page, next * KEYS);
+        if (next < to) load_v(page, next * TURN);
         if (dirty) {
             // an infinity stays one in the sum of all that see it, a NaN too
-            for (int key = max(slot, first); key < min(slot + KEYS, rg.end); key++) {
-                const uint16_t* src = vd + row_at(p.c, here, h, key) + g * 8;
+#pragma unroll 1
+            for (int key = max(slot, first); key < min(slot + TURN, rg.end); key++) {
+                const int in = U > 1 && key - slot >= GROUP ? here[U - 1] : here[0];
+                if (in < 0) continue;
+                const uint16_t* src = vd + row_at(p.c, in, h, key) + g * 8;
 #pragma unroll
                 for (int c = 0; c < VC; c++) {
                     const uint4 w = load_cached(src + c * 64);
@@ -401,55 +462,39 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 ? 3 : 2)
             for (int c = 0; c < VC; c++)
 #pragma unroll
                 for (int k = 0; k < 4; k += 2)
-                    *reinterpret_cast<float4*>(&sm_o[warp][r][c * 64 + g * 8 + k * 2]) =
+                    *reinterpret_cast<float4*>(sm_o + (warp * R + r) * LDO + c * 64 + g * 8 + k * 2) =
                         make_float4(o[c][k][nt][e], o[c][k][nt][2 + e], o[c][k + 1][nt][e], o[c][k + 1][nt][2 + e]);
         }
     __syncthreads();
-    if (threadIdx.x < R) {
-        const int r = threadIdx.x;
-        const Sum x = weigh(WARPS, [&](int w) { return state[w][r]; }, &weight[0][r], R);
-        merged[r] = make_float2(x.m, x.l);
-        inv_l[r] = x.l == 0.f ? 0.f : 1.f / x.l;
-    }
-    __syncthreads();
+    if (clustered) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // every CTA of the cluster runs
+    cg::cluster_group cluster = cg::this_cluster();
     // a thread has the same four columns of every row it takes
     constexpr int ROWS_AT_ONCE = 32 * WARPS / (D / 4);
-    const int live = min(R, rows - row0), c4 = threadIdx.x % (D / 4) * 4, r0 = threadIdx.x / (D / 4);
+    const int live = min(R, rows - row0), c4 = threadIdx.x % (D / 4) * 4, r0 = threadIdx.x / (D / 4), per = rows_of_rank(R, splits);
     T* out = static_cast<T*>(const_cast<void*>(p.out.data)) + z + b * p.out.bs + (size_t)h * group * D + c4;
+    float* inbox = sm_o + WARPS * R * LDO;
     for (int r = r0; r < live; r += ROWS_AT_ONCE) {
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int w = 0; w < WARPS; w++) add4(acc, weight[w][r], *reinterpret_cast<const float4*>(&sm_o[w][r][c4]));
+        const Sum x = sum_of(WARPS, [&](int w) { return state[w][r]; },
+                             [&](int w) { return *reinterpret_cast<const float4*>(sm_o + (w * R + r) * LDO + c4); });
         if (splits == 1) {
             const int row = row0 + r, i = row / group;
-            store4(out + i * p.out.ts + (size_t)(row - i * group) * D, acc, inv_l[r], vec & 2);
-        } else if (clustered) {
-            *reinterpret_cast<float4*>(&sm_o[0][r][c4]) = acc;  // warp 0's, which no other thread reads
+            store4(out + i * p.out.ts + (size_t)(row - i * group) * D, x.o, x.l == 0.f ? 0.f : 1.f / x.l, vec & 2);
         } else {
-            float* ws = p.ws + z + (((size_t)bh * gridDim.x + blockIdx.x) * R + r) * (D + 4);
-            *reinterpret_cast<float4*>(ws + 4 + c4) = acc;
-            if (c4 == 0) *reinterpret_cast<float2*>(ws) = merged[r];
+            const int k = r / splits;
+            float* to = clustered ? cluster.map_shared_rank(inbox, r - k * splits) + (split * per + k) * LDO
+                                  : p.ws + z + (((size_t)bh * gridDim.x + blockIdx.x) * R + r) * LDO;
+            *reinterpret_cast<float4*>(to + 4 + c4) = x.o;
+            if (c4 == 0) *reinterpret_cast<float2*>(to) = make_float2(x.m, x.l);
         }
     }
-    if (splits == 1 || !clustered) return;
-    // the cluster's CTAs: row r's outputs are the CTA's of rank r modulo their number
-    cg::cluster_group cluster = cg::this_cluster();
+    if (!clustered) return;
     cluster.sync();
-    if (threadIdx.x < R) {
-        const int r = threadIdx.x;
-        const Sum x = weigh(splits, [&](int s) { return *cluster.map_shared_rank(&merged[r], s); }, &weight[0][r], R);
-        inv_l[r] = x.l == 0.f ? 0.f : 1.f / x.l;
+    for (int k = r0; k * splits + split < live; k += ROWS_AT_ONCE) {
+        const Sum x = sum_of(splits, [&](int s) { return *reinterpret_cast<const float2*>(inbox + (s * per + k) * LDO); },
+                             [&](int s) { return *reinterpret_cast<const float4*>(inbox + (s * per + k) * LDO + 4 + c4); });
+        const int row = row0 + k * splits + split, i = row / group;
+        store4(out + i * p.out.ts + (size_t)(row - i * group) * D, x.o, x.l == 0.f ? 0.f : 1.f / x.l, vec & 2);
     }
-    __syncthreads();
-    for (int r = split + splits * r0; r < live; r += splits * ROWS_AT_ONCE) {
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (int s = 0; s < splits; s++)
-            add4(acc, weight[s][r], *reinterpret_cast<const float4*>(cluster.map_shared_rank(&sm_o[0][r][c4], s)));
-        const int row = row0 + r, i = row / group;
-        store4(out + i * p.out.ts + (size_t)(row - i * group) * D, acc, inv_l[r], vec & 2);
-    }
-    cluster.sync();  // the others have read this CTA's shared memory
 }
 
 // The splits' partials to the output, G * D / 4 threads to a row: each of the G groups sums every G-th split, and the
@@ -462,7 +507,7 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(PagedAttn p, int spl
     static_assert(ROWS >= 1 && (G == 1 || ROWS == 1), "whole rows, or one to the CTA");
     __shared__ int parent[MOST_TREE];
     __shared__ float top_of[G];
-    __shared__ float sum_of[G];
+    __shared__ float sum_of_group[G];
     __shared__ float4 sums[G][D / 4];
     const int bh = blockIdx.y, b = bh / p.c.n_head_kv, h = bh - b * p.c.n_head_kv, group = p.n_head / p.c.n_head_kv;
     const int row = blockIdx.x * ROWS + threadIdx.x / TO_ROW, sub = threadIdx.x % TO_ROW / (D / 4), c = threadIdx.x % (D / 4);
@@ -474,37 +519,48 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(PagedAttn p, int spl
     const int tiles = (p.s.n * group + R - 1) / R;
     const size_t step = (size_t)R * (D + 4);
     const float* ws = p.ws + z + ((size_t)bh * tiles + row / R) * splits * step + (row % R) * (D + 4);
-    float mx = -INFINITY;
-    if (live)
-#pragma unroll 8
-        for (int s = sub; s < splits; s += G) mx = fmaxf(mx, __ldcg(ws + s * step));
-    if (G > 1) {
-        if (c == 0) top_of[sub] = mx;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < G; w++) mx = fmaxf(mx, top_of[w]);
-    }
-    const float base = mx == -INFINITY ? 0.f : mx;
-    float sum = 0.f;
+    // in batches whose loads are all on their way before the first is used
+    constexpr int BATCH = 8;
+    float mx = -INFINITY, sum = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     if (live)
-#pragma unroll 8
-        for (int s = sub; s < splits; s += G) {
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(ws + s * step));
-            const float f = exp2_approx(ml.x - base);
-            sum += ml.y * f;
-            add4(acc, f, __ldcg(reinterpret_cast<const float4*>(ws + s * step + 4) + c));
+#pragma unroll 1
+        for (int s0 = sub; s0 < splits; s0 += BATCH * G) {
+            float2 ml[BATCH];
+            float4 o[BATCH];
+#pragma unroll
+            for (int k = 0; k < BATCH; k++) {
+                const float* at = ws + min(s0 + k * G, splits - 1) * step;
+                ml[k] = __ldcg(reinterpret_cast<const float2*>(at));
+                o[k] = __ldcg(reinterpret_cast<const float4*>(at + 4) + c);
+            }
+            float top = mx;
+#pragma unroll
+            for (int k = 0; k < BATCH; k++)
+                if (s0 + k * G < splits) top = fmaxf(top, ml[k].x);
+            const float base = top == -INFINITY ? 0.f : top, keep = exp2_approx(mx - base);
+            sum *= keep;
+            acc = make_float4(acc.x * keep, acc.y * keep, acc.z * keep, acc.w * keep);
+#pragma unroll
+            for (int k = 0; k < BATCH; k++) {
+                if (s0 + k * G >= splits) continue;
+                const float f = exp2_approx(ml[k].x - base);
+                sum += ml[k].y * f;
+                add4(acc, f, o[k]);
+            }
+            mx = top;
         }
     if (G > 1) {
-        if (c == 0) sum_of[sub] = sum;
+        if (c == 0) {
+            top_of[sub] = mx;
+            sum_of_group[sub] = sum;
+        }
         sums[sub][c] = acc;
         __syncthreads();
         if (sub > 0) return;
-#pragma unroll
-        for (int w = 1; w < G; w++) {
-            sum += sum_of[w];
-            add4(acc, 1.f, sums[w][c]);
-        }
+        const Sum x = sum_of(G, [&](int w) { return make_float2(top_of[w], sum_of_group[w]); }, [&](int w) { return sums[w][c]; });
+        sum = x.l;
+        acc = x.o;
     }
     if (!live) return;
     const int i = row / group;
@@ -516,21 +572,31 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(PagedAttn p, int spl
 struct Plan {
     int tile_rows, tiles;  // query rows of a tile, tiles of a (sequence, kv head)
     int splits;            // cuts of the keys
-    bool chunk;            // the tcgen05 kernel's
+    int warps;             // of a CTA; 0: the tcgen05 kernel's
     size_t ws;             // floats of workspace, for this and shorter caches
     float us;              // about how long it takes, for the choice between the kernels
-    int in_place() const { return chunk ? 1 : MAX_CLUSTER; }  // cuts that need no workspace
+    int in_place() const { return warps ? MAX_CLUSTER : 1; }  // cuts that need no workspace
 };
+
+// Shared memory of a CTA: its warps' O, and a cluster's inbox.
+int smem_of(int d, int tile_rows, int warps, int splits) {
+    const int inbox = splits > 1 && splits <= MAX_CLUSTER ? splits * rows_of_rank(tile_rows, splits) : 0;
+    return (warps * tile_rows + inbox) * (d + 4) * (int)sizeof(float);
+}
+
+// The most of it: splits * rows_of_rank is below R + splits.
+constexpr int most_smem(int d, int tile_rows, int warps) { return (warps * tile_rows + tile_rows + MAX_CLUSTER) * (d + 4) * (int)sizeof(float); }
 
 // Clusters of n CTAs that run at once on the current device: a cluster lives in one GPC, and the GPCs have different
 // numbers of SMs. Asked once for each device.
-template <int NT>
+template <int NT, int WARPS>
 int ask_clusters(int n) {
-    const auto kern = paged_split_kernel<float, 128, NT, 2>;  // the others need no more than it
+    const auto kern = paged_split_kernel<float, 128, NT, 2, WARPS>;  // the others need no more than it
     static std::atomic<uint64_t> done{0};
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)n);
     cfg.blockDim = dim3(32 * WARPS);
+    cfg.dynamicSmemBytes = smem_of(128, 8 * NT, WARPS, n);
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.x = (unsigned)n;
@@ -538,17 +604,22 @@ int ask_clusters(int n) {
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
     int count = 0;
-    if (allow_smem(done, (const void*)kern, 0, true) != cudaSuccess || cudaOccupancyMaxActiveClusters(&count, kern, &cfg) != cudaSuccess)
+    if (allow_smem(done, (const void*)kern, most_smem(128, 8 * NT, WARPS), true) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&count, kern, &cfg) != cudaSuccess)
         (void)cudaGetLastError();
     return count;
 }
-int clusters_at_once(int tile_rows, int n) {
-    static std::atomic<int> known[64][2][MAX_CLUSTER + 1];
+int clusters_at_once(int tile_rows, bool big, int n) {
+    static std::atomic<int> known[64][2][2][MAX_CLUSTER + 1];
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return 1;
-    std::atomic<int>& at = known[dev & 63][tile_rows == 8][n];
+    std::atomic<int>& at = known[dev & 63][tile_rows == 8][big][n];
     int count = at.load(std::memory_order_relaxed);
-    if (count == 0) at.store(count = std::max(1, tile_rows == 8 ? ask_clusters<1>(n) : ask_clusters<2>(n)), std::memory_order_relaxed);
+    if (count == 0) {
+        count = tile_rows == 8 ? big ? ask_clusters<1, big_warps(8)>(n) : ask_clusters<1, SMALL>(n)
+                               : big ? ask_clusters<2, big_warps(16)>(n) : ask_clusters<2, SMALL>(n);
+        at.store(count = std::max(1, count), std::memory_order_relaxed);
+    }
     return count;
 }
 
@@ -565,25 +636,36 @@ Plan plan_split(const Paged& c, const Seqs& s, int rows, bool raw, int sm_count)
     Plan p{};
     p.tile_rows = rows <= 8 ? 8 : 16;  // one or two 8-wide N tiles
     p.tiles = (rows + p.tile_rows - 1) / p.tile_rows;
-    const long long ctas = (long long)s.n_batch * c.n_head_kv * p.tiles, places = (long long)sm_count * (p.tile_rows == 8 ? 3 : 2);
-    const int groups = (keys_of(c, s) + KEYS - 1) / KEYS, useful = (groups + WARPS - 1) / WARPS;
-    const auto turns = [&](int n) { return (useful + n - 1) / n; };  // groups that follow each other in a warp
-    const int most = (int)std::min<long long>(useful, std::max<long long>(1, places / ctas));
-    // a cluster that waits for a place doubles the time
-    int in_cluster = std::min(MAX_CLUSTER, most);
-    while (in_cluster > 1 && ctas > clusters_at_once(p.tile_rows, in_cluster)) in_cluster--;
-    // more cuts than that where they save more turns than the second kernel costs
-    p.splits = most > MAX_CLUSTER && turns(most) + 2 < turns(in_cluster) ? most : in_cluster;
-    if (places / ctas > MAX_CLUSTER) p.ws = (size_t)ctas * most * p.tile_rows * (c.d + 4);
-    const float turn = c.d == 64 ? raw ? 1.2f : 1.4f : raw ? 1.5f : 2.f;
-    p.us = waves_of(ctas * p.splits, places) * (4.f + turn * turns(p.splits)) + (p.splits > MAX_CLUSTER ? 4.f : p.splits > 1 ? 3.f : 1.f);
+    const long long ctas = (long long)s.n_batch * c.n_head_kv * p.tiles;
+    const int key_turns = (keys_of(c, s) + GROUP * 128 / c.d - 1) / (GROUP * 128 / c.d);
+    const float turn = c.d == 64 ? raw ? 1.2f : 1.4f : raw ? 1.5f : 2.f;  // us of a turn, of which a warp has some
+    for (const bool big : {true, false}) {
+        const int warps = big ? big_warps(p.tile_rows) : SMALL;
+        const long long places = (long long)sm_count * (big_warps(p.tile_rows) / warps);
+        const int useful = (key_turns + warps - 1) / warps;
+        const auto turns = [&](int n) { return (useful + n - 1) / n; };  // that follow each other in a warp
+        const int most = (int)std::min<long long>(useful, std::max<long long>(1, places / ctas));
+        // a cluster that waits for a place doubles the time
+        int splits = std::min(MAX_CLUSTER, most);
+        while (splits > 1 && ctas > clusters_at_once(p.tile_rows, big, splits)) splits--;
+        // more cuts than that where they save more turns than the second kernel costs
+        if (most > MAX_CLUSTER && turns(most) + 2 < turns(splits)) splits = most;
+        if (places / ctas > MAX_CLUSTER) p.ws = std::max(p.ws, (size_t)ctas * most * p.tile_rows * (c.d + 4));
+        const float us = waves_of(ctas * splits, places) * (4.f + turn * turns(splits)) + (splits > MAX_CLUSTER ? 4.f : splits > 1 ? 2.f : 0.f) +
+                         (big ? 0.5f : 0.f);
+        if (big || us < p.us) {
+            p.us = us;
+            p.splits = splits;
+            p.warps = warps;
+        }
+    }
     return p;
 }
 
 // The tcgen05 kernel: keys are cut while SMs stay empty, two tiles of keys to a cut at least.
 Plan plan_chunk(const Paged& c, const Seqs& s, int rows, bool raw, int sm_count) {
     Plan p{};
-    p.chunk = true;
+    p.warps = 0;
     p.tile_rows = PAGED_CHUNK_ROWS;
     p.tiles = (rows + PAGED_CHUNK_ROWS - 1) / PAGED_CHUNK_ROWS;
     const long long ctas = (long long)s.n_batch * c.n_head_kv * p.tiles;
@@ -612,16 +694,17 @@ Plan plan_for(const Paged& c, const Seqs& s, int n_head, bool raw, int sm_count)
     return split.us < chunk.us ? split : chunk;
 }
 
-template <typename T, int D, int NT, int P>
+template <typename T, int D, int NT, int P, int WARPS>
 int split_launch(const PagedAttn& p, const Plan& plan, int vec, cudaStream_t st) {
     const float scale = (float)(1.0 / sqrt((double)D)) * kLog2e;
-    const int clustered = plan.splits <= MAX_CLUSTER;
-    const auto kern = paged_split_kernel<T, D, NT, P>;
+    const int clustered = plan.splits > 1 && plan.splits <= MAX_CLUSTER;
+    const auto kern = paged_split_kernel<T, D, NT, P, WARPS>;
     static std::atomic<uint64_t> done{0};
-    if (allow_smem(done, (const void*)kern, 0, true) != cudaSuccess) return -1;
+    if (allow_smem(done, (const void*)kern, most_smem(D, 8 * NT, WARPS), true) != cudaSuccess) return -1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(plan.tiles * plan.splits), (unsigned)(p.s.n_batch * p.c.n_head_kv));
     cfg.blockDim = dim3(32 * WARPS);
+    cfg.dynamicSmemBytes = smem_of(D, 8 * NT, WARPS, plan.splits);
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -632,6 +715,12 @@ int split_launch(const PagedAttn& p, const Plan& plan, int vec, cudaStream_t st)
     cfg.attrs = attr;
     cfg.numAttrs = 2;
     return cudaLaunchKernelEx(&cfg, kern, p, plan.splits, clustered, vec, scale) == cudaSuccess ? 0 : -1;
+}
+
+template <typename T, int D, int NT, int P>
+int split_of(const PagedAttn& p, const Plan& plan, int vec, cudaStream_t st) {
+    return plan.warps == SMALL ? split_launch<T, D, NT, P, SMALL>(p, plan, vec, st)
+                               : split_launch<T, D, NT, P, big_warps(8 * NT)>(p, plan, vec, st);
 }
 
 template <typename T, int D>
@@ -651,9 +740,9 @@ template <typename T, int D, int P>
 int attn(const PagedAttn& p, int sm_count, cudaStream_t st) {
     const Plan plan = plan_for(p.c, p.s, p.n_head, sizeof(T) == 2, sm_count);
     const int vec = (wide(p.q, sizeof(T), 16) ? 1 : 0) | (wide(p.out, sizeof(T), 4 * sizeof(T)) ? 2 : 0);
-    int rc = plan.chunk            ? paged_chunk_launch(p, sizeof(T) == 2 ? TYPE_BF16 : TYPE_F32, P, plan.splits, st)
-             : plan.tile_rows == 8 ? split_launch<T, D, 1, P>(p, plan, vec, st)
-                                   : split_launch<T, D, 2, P>(p, plan, vec, st);
+    int rc = plan.warps == 0       ? paged_chunk_launch(p, sizeof(T) == 2 ? TYPE_BF16 : TYPE_F32, P, plan.splits, st)
+             : plan.tile_rows == 8 ? split_of<T, D, 1, P>(p, plan, vec, st)
+                                   : split_of<T, D, 2, P>(p, plan, vec, st);
     if (rc == 0 && plan.splits > plan.in_place()) rc = combine<T, D>(p, plan, vec, sm_count, st);
     return rc;
 }
