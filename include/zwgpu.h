@@ -733,7 +733,8 @@ ZWG_API size_t zwg_paged_attn_workspace(const zwg_paged* c, const zwg_seqs* s, s
  * h / (n_head / n_head_kv)) over the pages, which hold the call's tokens already. Query i of sequence b
  * sees slots first[b] .. past + i, or with a tree first[b] .. past - 1, past + i and those of the tokens above
  * it. Softmax of q . k / sqrt(d) in f32, sums in f32; a query that sees no key gives zeros; what lies in
- * slots that a query does not see (infinities and NaN too) leaves its output alone. The context's math
+ * slots that a query does not see (infinities and NaN too) leaves its output alone; an infinity or a NaN
+ * among values that it sees gives one of the two in its own column. The context's math
  * mode applies to f32 queries: ZWG_MATH_F32 holds each query and probability in two f16 pieces (22 bits) against
  * the f16 keys and values, ZWG_MATH_TF32 in one (11 bits); a query's element is held to 2^-25 of its
  * largest, a probability to 2^-35 of the largest (probabilities are f16 pieces of 2^11 p or more). bf16

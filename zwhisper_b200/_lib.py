@@ -279,7 +279,7 @@ SIGNATURES = {
                                       c_size, ctypes.POINTER(RowsC), ctypes.POINTER(RowsC), c_ptr, c_size, c_ptr]),
     "zwg_tree_accept": (ctypes.c_int, [ctypes.POINTER(SeqsC), ctypes.POINTER(TreeC), c_ptr, c_ptr, c_ptr, c_ptr, c_ptr,
                                        c_ptr]),
-    "zwg_paged_keep": (ctypes.c_int, [ctypes.POINTER(PagedC), c_size, ctypes.POINTER(SeqsC), c_ptr, c_ptr, c_ptr]),
+    "zwg_paged_keep": (ctypes.c_int, [c_ptr, c_size, ctypes.POINTER(SeqsC), c_ptr, c_ptr, c_ptr]),
     "zwg_llm_state_create_kv8": (ctypes.c_int, [c_size] * 7 + [ctypes.c_double, ctypes.POINTER(c_ptr)]),
     "zwg_llm_state_kv8": (ctypes.c_int, [c_ptr, c_size, ctypes.POINTER(Kv8C)]),
     "zwg_llm_state_set_rope": (ctypes.c_int, [c_ptr, c_ptr, c_ptr, c_ptr]),

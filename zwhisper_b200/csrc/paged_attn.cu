@@ -421,7 +421,7 @@ __global__ void __launch_bounds__(32 * WARPS, big_warps(8 * NT) / WARPS)
                 }
         if (next < to) load_v(page, next * TURN);
         if (dirty) {
-            // an infinity stays one in the sum of all that see it, a NaN too
+            // an infinity or a NaN ends in the sums of all that see it
 #pragma unroll 1
             for (int key = max(slot, first); key < min(slot + TURN, rg.end); key++) {
                 const int in = U > 1 && key - slot >= GROUP ? here[U - 1] : here[0];

@@ -693,7 +693,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             __syncwarp();
         }
         if (splits > 1 && live && ok && half == 0 && (two || t == 0)) *reinterpret_cast<float2*>(ws + lane * (D + 4) - 4) = make_float2(m, l);
-        // what was taken out of the values comes in where a row sees it: an infinity stays one in the row's sum, a NaN too
+        // what was taken out of the values comes in where a row sees it
         bool flagged = false;
 #pragma unroll
         for (int e = 0; e < EDGES * (BN / 32); e++) flagged |= sm.flagged[e / (BN / 32)][e % (BN / 32)] != 0;

@@ -1121,6 +1121,7 @@ class PagedCache:
                               table.stride(0), B, heads, d, page, pages, most,
                               strides[0] if pages > 1 else heads * page * d)
         self._ref = ctypes.byref(self._c)
+        self._raw = bytes(self._c)
 
     @classmethod
     def empty(cls, n_pages: int, n_batch: int, n_head_kv: int, d: int, page: int, n_ctx: int, dtype=None,
@@ -1226,14 +1227,19 @@ def tree_accept(tokens, ids, tree, count=None, path=None, n_path=None, following
     dev = tokens.device
     if tree is None:
         raise ValueError("tree must be given")
-    args = [_int32_of(tokens, dev, shape, "tokens"), _int32_of(ids, dev, shape, "ids")]
-    path = torch.empty_like(tokens) if path is None else path
-    n_path = tokens.new_empty(B) if n_path is None else n_path
-    following = tokens.new_empty(B) if following is None else following
-    args += [_int32_of(path, dev, shape, "path"), _int32_of(n_path, dev, (B,), "n_path"),
-             _int32_of(following, dev, (B,), "following")]
+    given = [_int32_of(tokens, dev, shape, "tokens"), _int32_of(ids, dev, shape, "ids")]
+
+    def out(t, shape, name):
+        if t is not None:
+            return t, _int32_of(t, dev, shape, name)
+        t = torch.empty(shape, dtype=torch.int32, device=dev)
+        return t, t.data_ptr()
+
+    path, p0 = out(path, shape, "path")
+    n_path, p1 = out(n_path, (B,), "n_path")
+    following, p2 = out(following, (B,), "following")
     s = _seqs(B, n, 0, count, None, None, dev)
-    _lib.check(_ready(dev).zwg_tree_accept(s, _tree(tree, B, n, dev), *args, _stream_on(dev)))
+    _lib.check(_ready(dev).zwg_tree_accept(s, _tree(tree, B, n, dev), *given, p0, p1, p2, _stream_on(dev)))
     return path, n_path, following
 
 
@@ -1251,7 +1257,7 @@ def paged_keep(caches, path, n_path, n_past, max_past=None) -> None:
     n = path.shape[1]
     args = (_int32_of(path, c.device, (c.n_batch, n), "path"), _int32_of(n_path, c.device, (c.n_batch,), "n_path"))
     s = c._call(n, n_past, None, None, max_past)
-    all_of = (_lib.PagedC * len(caches))(*(x._c for x in caches))
+    all_of = b"".join([x._raw for x in caches])  # an array of zwg_paged
     _lib.check(_ready(c.device).zwg_paged_keep(all_of, len(caches), s, *args, _stream_on(c.device)))
 
 
