@@ -16,8 +16,27 @@ struct alignas(sizeof(T) * N > 16 ? 16 : sizeof(T) * N) Vec {
     T e[N];
 };
 
-ZWG_DEV void down(float x, float& y) { y = x; }
-ZWG_DEV void down(float x, __nv_bfloat16& y) { y = __float2bfloat16_rn(x); }
+// f32 values rounded to elements of a type, two at a time where it has 16 bits.
+ZWG_DEV uint32_t pair_of(float a, float b, __half) {
+    const __half2 x = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&x);
+}
+ZWG_DEV uint32_t pair_of(float a, float b, __nv_bfloat16) {
+    const __nv_bfloat162 x = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&x);
+}
+template <typename H, int N>
+ZWG_DEV void rounded(const float (&a)[N], Vec<H, N>& o) {
+    if constexpr (sizeof(H) == 4) {
+#pragma unroll
+        for (int j = 0; j < N; j++) o.e[j] = a[j];
+    } else if constexpr (N == 1) {
+        o.e[0] = held(a[0], H());
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; j += 2) reinterpret_cast<uint32_t*>(&o)[j / 2] = pair_of(a[j], a[j + 1], H());
+    }
+}
 
 // ---- append ------------------------------------------------------------------------------
 //
@@ -26,12 +45,12 @@ ZWG_DEV void down(float x, __nv_bfloat16& y) { y = __float2bfloat16_rn(x); }
 // of q and k at position past + i, or past + (token i's ancestors in the call) in a tree; the f32 operations
 // one by one, as rope_kernel, so that both give the same bits. k' and v are rounded once to the cache's type.
 // Bound by memory: every row in once, out once. A thread takes a piece of 8 elements (or, where pairs are
-// halves, both sides' pieces) of up to four of a token's q, k and v heads: they share its table entries, and all
+// halves, both sides' pieces) of up to eight (four) of a token's q, k and v heads: they share its table entries, and all
 // its loads are on their way before the first is used. Rows that are not aligned for that, and rotated parts
-// that do not divide into it, go one element at a time.
-constexpr int HEADS = 4;
+// that do not divide into it, go four elements or one at a time.
+constexpr int heads_of(bool one) { return one ? 8 : 4; }  // of a thread: eight pieces on their way
 
-// N: elements a thread moves at a time (8, or 1). Threads: (piece, group of heads, token).
+// N: elements a thread moves at a time (8, 4, or 1). Threads: (piece, group of heads, token).
 template <typename T, int N, bool INTER>
 __global__ void __launch_bounds__(256) paged_append_kernel(PagedAppend p) {
     chain_release();
@@ -41,6 +60,7 @@ __global__ void __launch_bounds__(256) paged_append_kernel(PagedAppend p) {
     using W = Vec<H, N>;
     constexpr bool ONE = INTER && N > 1;  // a piece holds both sides of its pairs
     constexpr int C = ONE ? N / 2 : N;    // pairs of a piece
+    constexpr int HEADS = heads_of(ONE);
     using F = Vec<float, C>;
     __shared__ int parent[MOST_TREE];
     const bool lead = threadIdx.x == 0 && threadIdx.y == 0 && threadIdx.z == 0 && blockIdx.x == 0 && blockIdx.z == 0;
@@ -87,17 +107,24 @@ __global__ void __launch_bounds__(256) paged_append_kernel(PagedAppend p) {
     const int page = page_of(p.c, b, slot + z);
     if (page < 0 && piece == 0 && threadIdx.y == 0) set_error(p.err, kErrBounds);
     T* qo = static_cast<T*>(const_cast<void*>(p.q_out.data)) + (b * p.q_out.bs + i * p.q_out.ts + z);
+    const size_t in_k = row_at(p.c, max(page, 0), 0, slot) + z;
+    H* const ko = static_cast<H*>(p.c.k) + in_k;
+    H* const vo = static_cast<H*>(p.c.v) + in_k;
+    const size_t hs = (size_t)d << p.c.log_page;  // from head to head in a page
 #pragma unroll
     for (int u = 0; u < HEADS; u++) {
         if (u >= heads) break;
         const int h = h0 + u - p.n_head;
+        const bool turns = turn && h < kv;
         float a[N], c[N];
+        if (turns || sizeof(T) == 4) {
 #pragma unroll
-        for (int j = 0; j < N; j++) a[j] = up(va[u].e[j]);
-        if (!ONE && turn)
-#pragma unroll
-            for (int j = 0; j < N; j++) c[j] = up(vb[u].e[j]);
-        if (turn && h < kv) {
+            for (int j = 0; j < N; j++) {
+                a[j] = up(va[u].e[j]);
+                c[j] = ONE ? 0.f : up(vb[u].e[j]);
+            }
+        }
+        if (turns) {
 #pragma unroll
             for (int j = 0; j < C; j++) {
                 float& x = ONE ? a[(2 * j) % N] : a[j];
@@ -106,34 +133,30 @@ __global__ void __launch_bounds__(256) paged_append_kernel(PagedAppend p) {
                 x = __fsub_rn(__fmul_rn(x0, co.e[j]), __fmul_rn(y0, si.e[j]));
                 y = __fadd_rn(__fmul_rn(x0, si.e[j]), __fmul_rn(y0, co.e[j]));
             }
+            rounded(a, va[u]);
+            if (!ONE) rounded(c, vb[u]);
         }
         if (h < 0) {
             T* y = qo + (h + p.n_head) * d;
-            V o;
-#pragma unroll
-            for (int j = 0; j < N; j++) down(a[j], o.e[j]);
-            *reinterpret_cast<V*>(y + ea) = o;
-            if (!ONE && turn) {
-#pragma unroll
-                for (int j = 0; j < N; j++) down(c[j], o.e[j]);
-                *reinterpret_cast<V*>(y + eb) = o;
-            }
+            *reinterpret_cast<V*>(y + ea) = va[u];
+            if (!ONE && turn) *reinterpret_cast<V*>(y + eb) = vb[u];
         } else if (page >= 0) {
-            H* y = static_cast<H*>(h < kv ? p.c.k : p.c.v) + row_at(p.c, page, h < kv ? h : h - kv, slot) + z;
-            W o;
-#pragma unroll
-            for (int j = 0; j < N; j++) o.e[j] = held(a[j], H());
-            *reinterpret_cast<W*>(y + ea) = o;
-            if (!ONE && turn) {
-#pragma unroll
-                for (int j = 0; j < N; j++) o.e[j] = held(c[j], H());
-                *reinterpret_cast<W*>(y + eb) = o;
+            H* y = h < kv ? ko + h * hs : vo + (h - kv) * hs;
+            W wa, wb;
+            if constexpr (sizeof(T) == 4) {
+                rounded(a, wa);
+                if (!ONE) rounded(c, wb);
+            } else {  // as it is, or as it was rounded
+                wa = *reinterpret_cast<const W*>(&va[u]);
+                if (!ONE) wb = *reinterpret_cast<const W*>(&vb[u]);
             }
+            *reinterpret_cast<W*>(y + ea) = wa;
+            if (!ONE && turn) *reinterpret_cast<W*>(y + eb) = wb;
         }
     }
 }
 
-bool aligned(const Rows& r, size_t elem) { return ((uintptr_t)r.data | (r.bs * elem) | (r.ts * elem)) % 16 == 0; }
+bool aligned(const Rows& r, size_t elem, size_t bytes) { return ((uintptr_t)r.data | (r.bs * elem) | (r.ts * elem)) % bytes == 0; }
 
 template <typename T, int N>
 int append(const PagedAppend& p, cudaStream_t st) {
@@ -141,7 +164,7 @@ int append(const PagedAppend& p, cudaStream_t st) {
     const int rot = p.rope.cos ? p.rope.rot : 0;
     // a head's pieces: a pair of pieces, or a piece that holds its pairs, counts once
     const int pieces = (inter && N > 1 ? rot / N : rot / 2 / N) + (p.c.d - rot) / N;
-    const int groups = (p.n_head + 2 * p.c.n_head_kv + HEADS - 1) / HEADS;
+    const int heads = heads_of(inter && N > 1), groups = (p.n_head + 2 * p.c.n_head_kv + heads - 1) / heads;
     const int y = std::min(groups, std::max(1, 256 / pieces)), tokens = std::min({std::max(1, 256 / (pieces * y)), p.s.n, 64});
     const dim3 grid((p.s.n + tokens - 1) / tokens, p.s.n_batch, (groups + y - 1) / y);
     return launch_chained(inter ? paged_append_kernel<T, N, true> : paged_append_kernel<T, N, false>, grid,
@@ -150,13 +173,18 @@ int append(const PagedAppend& p, cudaStream_t st) {
                : -1;
 }
 
+// Whether rows and rotated parts divide into pieces of n elements that are aligned to their 16 bytes, or to all of them.
+template <typename T>
+bool divides(const PagedAppend& p, int n) {
+    const size_t bytes = std::min<size_t>(16, n * sizeof(T));
+    const int half = p.rope.cos ? p.rope.rot / 2 : 0, pairs = p.rope.interleaved ? n / 2 : n;  // of a piece, and of its table entries
+    return aligned(p.q, sizeof(T), bytes) && aligned(p.q_out, sizeof(T), bytes) && aligned(p.k, sizeof(T), bytes) &&
+           aligned(p.v, sizeof(T), bytes) && half % pairs == 0 && (((uintptr_t)p.rope.cos | (uintptr_t)p.rope.sin) % std::min(16, pairs * 4)) == 0;
+}
+
 template <typename T>
 int append_type(const PagedAppend& p, cudaStream_t st) {
-    constexpr int N = 8;
-    const int half = p.rope.cos ? p.rope.rot / 2 : 0;
-    const bool vec = aligned(p.q, sizeof(T)) && aligned(p.q_out, sizeof(T)) && aligned(p.k, sizeof(T)) && aligned(p.v, sizeof(T)) &&
-                     (p.rope.interleaved ? 2 * half : half) % N == 0 && (((uintptr_t)p.rope.cos | (uintptr_t)p.rope.sin) % 16) == 0;
-    return vec ? append<T, N>(p, st) : append<T, 1>(p, st);
+    return divides<T>(p, 8) ? append<T, 8>(p, st) : divides<T>(p, 4) ? append<T, 4>(p, st) : append<T, 1>(p, st);
 }
 
 // ---- acceptance --------------------------------------------------------------------------
