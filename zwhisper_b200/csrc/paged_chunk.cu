@@ -121,7 +121,7 @@ ZWG_DEV uint32_t finite(uint32_t w, uint32_t exponent) {
     return w;
 }
 
-// vec: bit 0 queries, bit 1 outputs can be moved 16 bytes of f32 at a time.
+// vec: bit 0 queries can be read 4 elements at a time, bit 1 outputs written 16 bytes at a time.
 template <typename T, int D, int P>
 __global__ void __launch_bounds__(THREADS, 1)
     paged_chunk_kernel(PagedAttn p, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
@@ -366,7 +366,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         const uint32_t live_rows = __ballot_sync(0xffffffffu, live);
         {
             // queries: whole rows, a lane four elements; the warps that have a quarter's rows share them out
-            constexpr int LANES = D / 4, AT_ONCE = 32 / LANES, BATCH = 8 / AT_ONCE;  // loads on their way
+            constexpr int LANES = D / 4, AT_ONCE = 32 / LANES, BATCH = (RAW ? 16 : 8) / AT_ONCE;  // loads on their way
             const T* q = static_cast<const T*>(p.q.data) + z + b * p.q.bs + lane % LANES * 4;
             const size_t q_off = i * p.q.ts + in_token;
             const int n_lo = two ? half * 16 : (t * 2 + half) * 8, n_hi = n_lo + (two ? 16 : 8);
@@ -375,7 +375,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 Four<T> xs[BATCH];
                 size_t off[BATCH];
 #pragma unroll
-                for (int c = 0; c < BATCH; c++) off[c] = __shfl_sync(0xffffffffu, q_off, n0 + c * AT_ONCE + lane / LANES);
+                for (int c = 0; c < BATCH; c++) off[c] = __shfl_sync(0xffffffffu, q_off, min(n0 + c * AT_ONCE, n_hi - AT_ONCE) + lane / LANES);
                 if (vec & 1) {  // (a row behind the last one: the first token's)
 #pragma unroll
                     for (int c = 0; c < BATCH; c++) xs[c] = load_four(q + off[c], true);
@@ -385,6 +385,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 }
 #pragma unroll
                 for (int c = 0; c < BATCH; c++) {
+                    if (n0 + c * AT_ONCE >= n_hi) break;
                     const int rr = n0 + c * AT_ONCE + lane / LANES, qr = quarter * 32 + rr, e = lane % LANES * 4;
                     const bool is_live = live_rows >> rr & 1;
                     uint2 w[P];
@@ -653,18 +654,11 @@ __global__ void __launch_bounds__(THREADS, 1)
             m = most;
         }
         const float f = splits > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
-        // the rows' outputs, or their part of the keys' cuts, through the warp's part of the queries' shared memory, 16
-        // columns at a time, so that 4 lanes write 64 consecutive bytes (of f32) of a row
         T* out = static_cast<T*>(const_cast<void*>(p.out.data)) + z + b * p.out.bs + half * COLS;
         const size_t out_off = i * p.out.ts + in_token;
         float* ws = p.ws + z + (((size_t)bh * gridDim.x + blockIdx.x) * 2 * BM + qt * BM + quarter * 32) * (D + 4) + 4 + half * COLS;
-        uint8_t* stage = &sm.q[0][0][0][0] + warp * 2048;
-        size_t offs[4];  // of the rows whose pieces the thread writes
-#pragma unroll
-        for (int n = 0; n < 4; n++) offs[n] = __shfl_sync(0xffffffffu, out_off, n * 8 + lane / 4);
-#pragma unroll 1
-        for (int k = c_lo; k < c_hi; k += 16) {
-            float o[16];
+        // 16 of the thread's columns, ended
+        const auto ended = [&](int k, float (&o)[16]) {
             columns(k, o);
             if (!two) {
 #pragma unroll
@@ -677,17 +671,64 @@ __global__ void __launch_bounds__(THREADS, 1)
                 }
             }
 #pragma unroll
-            for (int u = 0; u < 4; u++)
-                *reinterpret_cast<float4*>(stage + lane * 64 + ((u ^ (lane >> 1 & 3)) << 4)) =
-                    make_float4(o[u * 4] * f, o[u * 4 + 1] * f, o[u * 4 + 2] * f, o[u * 4 + 3] * f);
-            __syncwarp();
+            for (int e = 0; e < 16; e++) o[e] *= f;
+        };
+        if (splits > 1) {
+            // the row's part of the keys' cuts, 16 columns at a time: 4 lanes write 64 consecutive bytes of a row
+            uint8_t* stage = &sm.q[0][0][0][0] + warp * 2048;
+#pragma unroll 1
+            for (int k = c_lo; k < c_hi; k += 16) {
+                float o[16];
+                ended(k, o);
 #pragma unroll
-            for (int n = 0; n < 32; n += 8) {
-                const int rr = n + lane / 4, u = lane & 3, col = k + u * 4;
-                const float4 y = *reinterpret_cast<const float4*>(stage + rr * 64 + ((u ^ (rr >> 1 & 3)) << 4));
-                if (ok && (live_rows >> rr & 1)) {
-                    if (splits > 1) store4(ws + rr * (D + 4) + col, y, 1.f, true);
-                    else store4(out + offs[n / 8] + col, y, 1.f, vec & 2);
+                for (int u = 0; u < 4; u++)
+                    *reinterpret_cast<float4*>(stage + lane * 64 + ((u ^ (lane >> 1 & 3)) << 4)) = make_float4(o[u * 4], o[u * 4 + 1], o[u * 4 + 2], o[u * 4 + 3]);
+                __syncwarp();
+#pragma unroll
+                for (int n = 0; n < 32; n += 8) {
+                    const int rr = n + lane / 4, u = lane & 3;
+                    const float4 y = *reinterpret_cast<const float4*>(stage + rr * 64 + ((u ^ (rr >> 1 & 3)) << 4));
+                    if (ok && (live_rows >> rr & 1)) *reinterpret_cast<float4*>(ws + rr * (D + 4) + k + u * 4) = y;
+                }
+                __syncwarp();
+            }
+        } else {
+            // the row's outputs, all of the thread's columns through the warp's part of the queries' shared memory, so that
+            // neighbouring lanes write a row's consecutive bytes
+            // (f32 rows in one piece reach into the values' buffers, but not where those pass sums on)
+            const int n_u = (c_hi - c_lo) * (int)sizeof(T) / 16;  // 16-byte pieces of a row, a power of two
+            uint8_t* stage = &sm.q[0][0][0][0] + warp * (32 * 16 * n_u);
+            const auto piece = [&](int rr, int u) { return reinterpret_cast<uint4*>(stage + (rr * n_u + (u ^ (rr & (n_u - 1) & 7))) * 16); };
+#pragma unroll 1
+            for (int k = c_lo; k < c_hi; k += 16) {
+                float o[16];
+                ended(k, o);
+#pragma unroll
+                for (int u = 0; u < (int)sizeof(T); u++) {  // 16 columns are that many pieces
+                    uint4 y;
+                    if constexpr (RAW) {
+                        __nv_bfloat162 h2[4];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) h2[e] = __floats2bfloat162_rn(o[(u % 2) * 8 + 2 * e], o[(u % 2) * 8 + 2 * e + 1]);
+                        y = *reinterpret_cast<const uint4*>(h2);
+                    } else {
+                        y = make_uint4(__float_as_uint(o[u * 4]), __float_as_uint(o[u * 4 + 1]), __float_as_uint(o[u * 4 + 2]), __float_as_uint(o[u * 4 + 3]));
+                    }
+                    *piece(lane, (k - c_lo) * (int)sizeof(T) / 16 + u) = y;
+                }
+            }
+            __syncwarp();
+            for (int e = lane; e < 32 * n_u; e += 32) {
+                const int rr = e / n_u, u = e & (n_u - 1);
+                const uint4 y = *piece(rr, u);
+                T* to = out + __shfl_sync(0xffffffffu, out_off, rr) + c_lo + u * (16 / (int)sizeof(T));
+                if (!ok || !(live_rows >> rr & 1)) continue;
+                if (vec & 2) {
+                    *reinterpret_cast<uint4*>(to) = y;
+                } else {
+                    const T* x = reinterpret_cast<const T*>(&y);
+#pragma unroll
+                    for (int c = 0; c < 16 / (int)sizeof(T); c++) to[c] = x[c];
                 }
             }
             __syncwarp();
@@ -752,7 +793,7 @@ int launch(const PagedAttn& p, int splits, cudaStream_t st) {
     if (!map_of(&k, p.c.k, p.c, sizeof(T) == 2) || !map_of(&v, p.c.v, p.c, sizeof(T) == 2)) return -1;
     const int rows = p.s.n * (p.n_head / p.c.n_head_kv), tiles = (rows + PAGED_CHUNK_ROWS - 1) / PAGED_CHUNK_ROWS;
     const float scale = (float)(1.0 / sqrt((double)D)) * kLog2e;
-    const int vec = (wide(p.q, sizeof(T), 4 * sizeof(T)) ? 1 : 0) | (wide(p.out, sizeof(T), 4 * sizeof(T)) ? 2 : 0);
+    const int vec = (wide(p.q, sizeof(T), 4 * sizeof(T)) ? 1 : 0) | (wide(p.out, sizeof(T), 16) ? 2 : 0);
     return launch_chained_smem(kern, dim3((unsigned)(tiles * splits), (unsigned)(p.s.n_batch * p.c.n_head_kv)), dim3(THREADS),
                                smem, st, p, k, v, splits, vec, scale) == cudaSuccess
                ? 0
