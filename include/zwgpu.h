@@ -689,7 +689,8 @@ ZWG_API int zwg_kv8_attn(const zwg_kv8* c, const zwg_seqs* s, int type, size_t n
 
 /* The cache: d 64 or 128, `page` a power of two from 16 to 256,
  *   k, v   [n_pages][n_head_kv][page][d] of `type`, pages `page_stride` elements apart (a multiple
- *          of 8, at least n_head_kv * page * d; k and v may share a buffer that way), 16-byte aligned
+ *          of 8, at least n_head_kv * page * d, below 2^38; k and v may share a buffer that way), 16-byte
+ *          aligned
  *   table  int32 [n_batch][max_pages], rows table_stride apart; an entry outside [0, n_pages) is
  *          no page (-1, say, behind a sequence's last one)
  * ZWG_TYPE_F16 caches take f32 rows, rounded to the nearest f16 (infinite from 65520 on), ZWG_TYPE_BF16

@@ -70,21 +70,26 @@ def attention(q, k, v, seen, pieces, half_step, big):
     n, H, d = q.shape
     group = H // k.shape[0]
     out, tol = np.zeros(q.shape), np.zeros(q.shape)
-    for i in range(n):
-        at = np.flatnonzero(seen[i])
-        if len(at) == 0:
-            continue
-        for h in range(H):
-            kk, vv, qq = k[h // group, at], v[h // group, at], q[i, h].astype(np.float64)
-            s = kk @ qq / np.sqrt(d)
-            e = np.exp(s - s.max())
-            w = e / e.sum()
-            o = w @ vv
-            size = (np.abs(kk) @ np.maximum(np.abs(qq), np.abs(qq).max() * 2.0 ** -11)).max() / np.sqrt(d)
-            piece = {0: 0.0, 1: 2.0 ** -11, 2: 2.0 ** -22}[pieces]
-            ds = size * (piece + (d + 20) * 2.0 ** -23) + 2.0 ** -22 * (1 + np.abs(s).max())
-            mean = w @ np.abs(vv)
-            rel = 2 * ds + {0: 0.0, 1: 2.0 ** -11, 2: 2.0 ** -21}[pieces] + (len(at) + 32) * 2.0 ** -23
-            off = 2.0 ** -8 * (w @ np.abs(vv - o)) if pieces == 0 else len(at) * (2.0 ** -36 if big else 2.0 ** -40) * np.abs(vv).max()
-            out[i, h], tol[i, h] = o, rel * mean + off + half_step * np.abs(o)
+    rows = np.flatnonzero(seen.any(1))
+    used = np.flatnonzero(seen.any(0))
+    if len(rows) == 0:
+        return out, tol + 1e-30
+    mask, number = seen[np.ix_(rows, used)], seen[rows].sum(1)[:, None]
+    for h in range(H):
+        kk, vv, qq = k[h // group, used], v[h // group, used], q[rows, h].astype(np.float64)
+        s = np.where(mask, qq @ kk.T / np.sqrt(d), -np.inf)
+        e = np.exp(s - s.max(1, keepdims=True))
+        w = e / e.sum(1, keepdims=True)
+        o = w @ vv
+        held = np.maximum(np.abs(qq), np.abs(qq).max(1, keepdims=True) * 2.0 ** -11)
+        size = np.where(mask, held @ np.abs(kk).T, 0).max(1, keepdims=True) / np.sqrt(d)
+        piece = {0: 0.0, 1: 2.0 ** -11, 2: 2.0 ** -22}[pieces]
+        ds = size * (piece + (d + 20) * 2.0 ** -23) + 2.0 ** -22 * (1 + np.abs(np.where(mask, s, 0)).max(1, keepdims=True))
+        rel = 2 * ds + {0: 0.0, 1: 2.0 ** -11, 2: 2.0 ** -21}[pieces] + (number + 32) * 2.0 ** -23
+        if pieces == 0:  # the sum of w |v - o|, a column at a time
+            off = 2.0 ** -8 * np.stack([(w * np.abs(vv[:, c][None] - o[:, c][:, None])).sum(1) for c in range(d)], 1)
+        else:
+            most = np.array([np.abs(vv[m]).max() for m in mask])[:, None]
+            off = number * (2.0 ** -36 if big else 2.0 ** -40) * most
+        out[rows, h], tol[rows, h] = o, rel * (w @ np.abs(vv)) + off + half_step * np.abs(o)
     return out, tol * 1.01 + 1e-30

@@ -26,8 +26,8 @@ int check_cache(const zwg_paged* c, const char* what) {
         return fail("%s: max_pages = %zu must be positive, and max_pages * page below 2^30", what, c->max_pages);
     if (c->n_head_kv == 0 || c->n_batch >= kMost || c->n_head_kv >= kMost || c->n_batch * c->n_head_kv > 65535)
         return fail("%s: n_batch * n_head_kv = %zu * %zu must be at most 65535", what, c->n_batch, c->n_head_kv);
-    if (c->page_stride % 8 || c->page_stride < c->n_head_kv * c->page * c->d || c->page_stride > ((size_t)1 << 60) / c->n_pages)
-        return fail("%s: page_stride = %zu must be a multiple of 8 and at least a page's %zu elements", what, c->page_stride,
+    if (c->page_stride % 8 || c->page_stride < c->n_head_kv * c->page * c->d || c->page_stride >= (size_t)1 << 38)
+        return fail("%s: page_stride = %zu must be a multiple of 8, at least a page's %zu elements and below 2^38", what, c->page_stride,
                     c->n_head_kv * c->page * c->d);
     if ((c->n_batch > 1 && c->table_stride < c->max_pages) || c->table_stride > ((size_t)1 << 60) / (c->n_batch + 1))
         return fail("%s: table_stride = %zu below the row's %zu entries, or too large", what, c->table_stride, c->max_pages);
@@ -45,7 +45,7 @@ int check_call(const zwg_paged* c, const zwg_seqs* s, const char* what) {
 
 int check_tree(const zwg_tree* t, const zwg_seqs* s, const char* what) {
     if (!t) return ZWG_OK;
-    if (!t->parent) return fail("%s: null parents", what);
+    if (!t->parent && s->n) return fail("%s: null parents", what);
     if (!al(t->parent, 4)) return fail("%s: parents must be 4-byte aligned", what);
     if (s->n > ZWG_MAX_TREE) return fail("%s: a tree of %zu tokens, at most %d are taken", what, s->n, ZWG_MAX_TREE);
     if (t->batch_stride > ((size_t)1 << 60) / (s->n_batch + 1)) return fail("%s: parents' stride too large", what);
@@ -166,7 +166,7 @@ int zwg_tree_accept(const zwg_seqs* s, const zwg_tree* tree, const int32_t* toke
     int rc = check_seqs(&sq, kMost, what);
     if (!rc) rc = check_tree(tree, &sq, what);
     if (rc || s->n_batch == 0) return rc;
-    if (!tokens || !ids || !path || !n_path || !next) return fail("%s: null buffer", what);
+    if ((s->n && (!tokens || !ids || !path)) || !n_path || !next) return fail("%s: null buffer", what);
     if (!al(tokens, 4) || !al(ids, 4) || !al(path, 4) || !al(n_path, 4) || !al(next, 4)) return fail("%s: 4-byte alignment required", what);
     Ctx* c = cur();
     if (!c) return ZWG_ERROR;
