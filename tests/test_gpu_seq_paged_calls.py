@@ -6,7 +6,7 @@ import pytest
 
 from oracle import paged as O
 from tests.conftest import has_gpu
-from tests.test_gpu_paged import World, check_attn, i32, normal, tree_of, up
+from tests.test_gpu_seq_paged import World, check_attn, i32, normal, tree_of, up
 
 pytestmark = pytest.mark.gpu
 

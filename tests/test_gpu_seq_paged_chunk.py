@@ -1,12 +1,12 @@
 """Attention over pages where the tcgen05 kernel is the one that runs (many rows of many sequences, or a long cache), which
-each test sees to by the kernel's name: against the oracle, in every form it has: both d, f32 in two pieces and one, bf16,
+each test sees to by the kernel's size: against the oracle, in every form it has: both d, f32 in two pieces and one, bf16,
 128 rows and more, cut keys, trees, ragged batches; and what lies where a query does not look."""
 import numpy as np
 import pytest
 
 from oracle import paged as O
 from tests.conftest import has_gpu
-from tests.test_gpu_paged import World, check_attn, i32, normal, tree_of, up
+from tests.test_gpu_seq_paged import World, i32, normal, tree_of, up
 
 pytestmark = pytest.mark.gpu
 
@@ -23,14 +23,47 @@ def env():
 
 
 def attend(torch, cache, q, *args, **kw):
-    """cache.attn, and the names of the kernels it launched."""
-    from torch.profiler import ProfilerActivity, profile
-    with profile(activities=[ProfilerActivity.CUDA, ProfilerActivity.CPU]) as prof:
-        out = cache.attn(q, *args, **kw)
-        torch.cuda.synchronize()
-    names = " ".join(e.key for e in prof.key_averages())
-    assert "paged_chunk" in names, names
+    """cache.attn, which must have launched the kernel of 640 threads: the call is captured as well, into a graph whose
+    nodes tell (a profiler's trace would, too, but one that was first opened a minute ago loses records)."""
+    from cuda.bindings import driver
+    out = cache.attn(q, *args, **kw)
+    graph, side = torch.cuda.CUDAGraph(keep_graph=True), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+        cache.attn(q, *args, **{**kw, "out": torch.empty_like(out)})
+    raw = driver.CUgraph(graph.raw_cuda_graph())
+    err, _, n = driver.cuGraphGetNodes(raw)
+    err, nodes, n = driver.cuGraphGetNodes(raw, n)
+    assert err == driver.CUresult.CUDA_SUCCESS
+    threads = []
+    for node in nodes[:n]:
+        err, kind = driver.cuGraphNodeGetType(node)
+        if kind == driver.CUgraphNodeType.CU_GRAPH_NODE_TYPE_KERNEL:
+            err, params = driver.cuGraphKernelNodeGetParams(node)
+            assert err == driver.CUresult.CUDA_SUCCESS
+            threads.append(params.blockDimX)
+    assert 640 in threads, threads
     return out
+
+
+def contents(w, b):
+    """k and v [n_head_kv][slots][d] of sequence b, in 64 bits."""
+    pages = np.maximum(w.np_table[b, : w.slots // w.page], 0).tolist()
+    return [np.moveaxis(t[pages].double().cpu().numpy(), 1, 0).reshape(w.Hkv, w.slots, w.d) for t in (w.cache.k, w.cache.v)]
+
+
+def check_attn(torch, out, before, w, q, past, count, first, parents, pieces):
+    """Some of the sequences against the oracle; rows behind every sequence's last one as they were."""
+    half = 2.0 ** -8 if q.dtype is torch.bfloat16 else 2.0 ** -24
+    for b in sorted({0, 1, w.B // 3, w.B // 2, w.B - 1}):
+        m = int(count[b])
+        seen = O.seen_slots(past[b], m, int(first[b]), w.slots, None if parents is None else parents[b])
+        want, tol = O.attention(q[b, :m].float().cpu().numpy(), *contents(w, b), seen, pieces, half, True)
+        got = out[b, :m].float().cpu().numpy()
+        bad = ~(np.abs(got - want) <= tol)
+        assert not bad.any(), (b, np.argwhere(bad)[:3], np.abs(got - want)[bad][:3], tol[bad][:3])
+    behind = torch.arange(q.shape[1], device=q.device) >= torch.tensor([int(c) for c in count], device=q.device)[:, None]
+    assert torch.equal(out[behind], before[behind])
 
 
 SHAPES = [  # batch, n, heads, heads_kv, d, page, past, tree
@@ -152,13 +185,13 @@ def test_pages_that_are_none(env, B, n, H, Hkv, d, page, past, tree, bf16):
     out = attend(torch, w.cache, q, past, **args)
     with pytest.raises(ZwgError):
         ops.sync()
-    k, v = w.contents(np.float64)
     for b in {0, 1, B - 1, B // 2}:
+        k, v = contents(w, b)
         seen = O.seen_slots(past, n, 0, w.slots, parents[b] if tree else None)
         for (bb, i) in bad:
             if bb == b:
                 seen[:, i * page:(i + 1) * page] = False
-        want, tol = O.attention(q[b].float().cpu().numpy(), k[b], v[b], seen, 0 if bf16 else 2, 2.0 ** (-8 if bf16 else -24), True)
+        want, tol = O.attention(q[b].float().cpu().numpy(), k, v, seen, 0 if bf16 else 2, 2.0 ** (-8 if bf16 else -24), True)
         assert (np.abs(out[b].float().cpu().numpy() - want) <= tol).all()
 
 
