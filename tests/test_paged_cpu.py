@@ -2,11 +2,16 @@
 (they check their arguments before they ask for a context, so these calls launch nothing), and the oracle's own
 properties."""
 import ctypes
+import os
+import re
+import subprocess
 
 import numpy as np
 import pytest
 
 from oracle import paged as O
+from tests.conftest import ROOT
+from tests.test_integration_examples import NOTES, THERE, blocks, header_members, same_kind
 from zwhisper_b200 import _lib
 
 P = 1 << 20  # an aligned address that is never read: each call is refused before a launch
@@ -161,3 +166,44 @@ def test_the_oracles_attention_is_the_softmax_of_seen_keys():
         s = np.exp(k[h // 2, [0, 2]] @ q[0, h] / np.sqrt(8))
         np.testing.assert_allclose(out[0, h], s @ v[h // 2, [0, 2]] / s.sum(), rtol=1e-12)
     assert not out[1].any() and (tol > 0).all()
+
+
+# ---- the integration notes' examples, as tests/test_integration_examples.py takes the others ----
+
+EXAMPLES = [  # the text it starts with, what is there
+    ("zwg_paged c = {", "size_t n_seq, size_t n_pages, void* k_pool, void* v_pool, const int32_t* table, zwg_seqs s, zwg_rows q, "
+     "zwg_rows k, zwg_rows v, zwg_rows out, zwg_rope_tables tables, void* ws, size_t ws_bytes, void* stream"),
+    ("zwg_tree tree = {", "size_t n, size_t n_seq, size_t n_layer, size_t n_vocab, size_t l, const int32_t* parent, zwg_paged* cache, zwg_seqs s, "
+     "zwg_rows q, zwg_rows k, zwg_rows v, zwg_rows out, zwg_rope_tables tables, zwg_logit_rules rules, float* logits, int32_t* ids, "
+     "const int32_t* tokens, int32_t* path, int32_t* n_path, int32_t* next, void* ws, size_t ws_bytes, void* stream"),
+]
+
+
+@pytest.mark.parametrize("starts,there", EXAMPLES)
+def test_c_example(tmp_path, starts, there):
+    code, = [b for b in blocks("C") if b.startswith(starts)]
+    src = tmp_path / "example.c"
+    src.write_text(f"{THERE}\nvoid example({there});\nvoid example({there})\n{{\n{code}\n}}\n")
+    out = subprocess.run(["gcc", "-std=c11", "-Wall", "-Wextra", "-Werror", "-Wno-missing-field-initializers", "-Wno-unused-function",
+                          "-Wno-unused-parameter", "-fsyntax-only", "-I", os.path.join(ROOT, "include"), str(src)], capture_output=True,
+                         text=True)
+    assert out.returncode == 0, out.stderr
+
+
+def test_every_example_is_here():
+    assert len(blocks("C")) == len(EXAMPLES)
+
+
+@pytest.mark.parametrize("zig,c", [("Paged", "zwg_paged"), ("Tree", "zwg_tree")])
+def test_zig_structs(zig, c):
+    body, = re.findall(r"const " + zig + r" = extern struct \{(.*?)\}", NOTES, flags=re.S)
+    got = [tuple(x.strip() for x in m.split(":", 1)) for m in body.split(",") if m.strip()]
+    want = header_members(c)
+    assert [n for n, _ in got] == [n for n, _ in want]
+    for (n, z), (_, k) in zip(got, want):
+        assert same_kind(z, k), (n, z, k)
+
+
+def test_every_call_is_declared_for_zig():
+    declared = set(re.findall(r'extern "c" fn (zwg_\w+)\(', NOTES))
+    assert {n for n in _lib.SIGNATURES if n.startswith(("zwg_paged", "zwg_tree"))} <= declared

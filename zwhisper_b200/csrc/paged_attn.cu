@@ -182,6 +182,7 @@ __global__ void __launch_bounds__(32 * WARPS, big_warps(8 * NT) / WARPS)
         }
         __syncthreads();
     }
+    __syncwarp();  // (the lanes of the hint: what follows is for whole warps)
     if (clustered) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // (waited for before the merge)
 
     // the pages of the warp's next 32 groups of keys, one in each lane
@@ -444,6 +445,7 @@ __global__ void __launch_bounds__(32 * WARPS, big_warps(8 * NT) / WARPS)
                     }
                 }
             }
+            __syncwarp();
         }
     }
 
@@ -488,6 +490,7 @@ __global__ void __launch_bounds__(32 * WARPS, big_warps(8 * NT) / WARPS)
         }
     }
     if (!clustered) return;
+    __syncwarp();
     cluster.sync();
     for (int k = r0; k * splits + split < live; k += ROWS_AT_ONCE) {
         const Sum x = sum_of(splits, [&](int s) { return *reinterpret_cast<const float2*>(inbox + (s * per + k) * LDO); },
@@ -649,8 +652,10 @@ Plan plan_split(const Paged& c, const Seqs& s, int rows, bool raw, int sm_count)
         int splits = std::min(MAX_CLUSTER, most);
         while (splits > 1 && ctas > clusters_at_once(p.tile_rows, big, splits)) splits--;
         // more cuts than that where they save more turns than the second kernel costs
+        const int in_cluster = splits;
         if (most > MAX_CLUSTER && turns(most) + 2 < turns(splits)) splits = most;
-        if (places / ctas > MAX_CLUSTER) p.ws = std::max(p.ws, (size_t)ctas * most * p.tile_rows * (c.d + 4));
+        // that takes more than 3 turns in the cluster, with these keys or fewer
+        if (most > MAX_CLUSTER && useful > 3 * in_cluster) p.ws = std::max(p.ws, (size_t)ctas * most * p.tile_rows * (c.d + 4));
         const float us = waves_of(ctas * splits, places) * (4.f + turn * turns(splits)) + (splits > MAX_CLUSTER ? 4.f : splits > 1 ? 2.f : 0.f) +
                          (big ? 0.5f : 0.f);
         if (big || us < p.us) {

@@ -191,6 +191,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         mbar_init(&sm.started, 1);
         fence_mbar_init();
     }
+    __syncwarp();
     if (warp == ISSUER) {
         tmem_alloc(&sm.tmem_base, TMEM_COLS);
         tmem_relinquish();
@@ -415,6 +416,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&sm.q_full[qt]);
+            __syncwarp();
         }
         const auto meet = [&] { return two ? all_of(pair, 64, true) : all_of(10, SOFTMAX, true); };
         meet();
@@ -467,6 +469,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             const bool masked = key0 + BN > by_slot || key0 < first || valid != 0xffu;
             uint32_t seen[2];
             if (masked) mask_of(key0 + half * KEYS, valid >> half * 4, seen);
+            __syncwarp();  // (rows have different numbers of ancestors)
             float top = -INFINITY;
             uint32_t s[P == 1 ? KEYS : 16];
             if constexpr (P == 1) {
@@ -512,6 +515,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sm.s_free[t]);
+                __syncwarp();  // what follows is for whole warps (.aligned)
             }
             const bool grow = top > m + STALE;  // from nothing, too
             const float was = m;
@@ -601,6 +605,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&sm.p_full[t]);
+            __syncwarp();
         }
         if (ok && mine > 0) ok = mbar_wait_warp(&sm.pv_done[t], (mine - 1) & 1, err);
         tc_fence_after();

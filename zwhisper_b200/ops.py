@@ -1115,9 +1115,10 @@ class PagedCache:
             raise ValueError("a sequence's pages must lie one after another")
         self.k, self.v, self.table, self.device = k, v, table, k.device
         self.n_batch, self.n_head_kv, self.d, self.page, self.n_ctx = B, heads, d, page, most * page
-        self._row_dtype = torch.float32 if k.dtype is torch.float16 else torch.bfloat16
+        half = k.dtype is torch.float16
+        self._row_dtype, self._row_kind = (torch.float32, _lib.ZWG_TYPE_F32) if half else (torch.bfloat16, _lib.ZWG_TYPE_BF16)
         self._c = _lib.PagedC(k.data_ptr(), v.data_ptr(),
-                              _lib.ZWG_TYPE_F16 if k.dtype is torch.float16 else _lib.ZWG_TYPE_BF16, table.data_ptr(),
+                              _lib.ZWG_TYPE_F16 if half else _lib.ZWG_TYPE_BF16, table.data_ptr(),
                               table.stride(0), B, heads, d, page, pages, most,
                               strides[0] if pages > 1 else heads * page * d)
         self._ref = ctypes.byref(self._c)
@@ -1137,12 +1138,12 @@ class PagedCache:
         return _seqs(self.n_batch, n, n_past, count, first, self.n_ctx if max_past is None else max_past, self.device)
 
     def _check_rows(self, t, name):
-        kind = _row_type(t, name)
+        if isinstance(t, _torch().Tensor) and t.dtype is self._row_dtype and t.dim() == 4:
+            return self._row_kind
+        _row_type(t, name)
         if t.dim() != 4:
             raise ValueError(f"{name} must be [n_batch][n][heads][d]")
-        if t.dtype is not self._row_dtype:
-            raise ValueError(f"{name} must be {self._row_dtype} beside a {self.k.dtype} cache, got {t.dtype}")
-        return kind
+        raise ValueError(f"{name} must be {self._row_dtype} beside a {self.k.dtype} cache, got {t.dtype}")
 
     def append(self, k, v, n_past, count=None, rope=None, tree=None, q=None, q_out=None, max_past=None):
         """Append k, v [n_batch][n][n_head_kv][d] (zwg_paged_append) at n_past (an int, or a CUDA int32
