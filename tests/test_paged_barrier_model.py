@@ -5,7 +5,8 @@ hardware (tests/test_prefill_barrier_model.py).
 
 Roles, as in the kernel: a loader that fills key and value buffers in turn; the warp that goes over values;
 for each of two slots an issuer and a softmax of two halves. `two`: both slots take every key tile, else
-every other one each. `early`: the next S is issued once this one has been read, else behind the PV.
+every other one each. `early`: the next S is issued once this one has been read, else behind the PV. `turns`: the
+slots' exponentials follow each other.
 Products complete in the order each issuer gave them; a commit arrives when everything before it is complete."""
 import os
 import random
@@ -16,8 +17,8 @@ import pytest
 from tests.conftest import ROOT
 from tests.test_prefill_barrier_model import Bar
 
-# early, key buffers, value buffers with two slots of rows; with one both have two
-FORMS = {"d64": (True, 2, 2), "d128": (True, 1, 2), "d64 f32": (False, 2, 2), "d128 f32": (False, 2, 1)}
+# early, key buffers, value buffers with two slots of rows (with one both have two), exponentials in turns
+FORMS = {"d64": (True, 2, 2, True), "d128": (True, 1, 2, True), "d64 f32": (False, 2, 2, False), "d128 f32": (False, 2, 1, True)}
 
 
 class Broken(Exception):
@@ -26,7 +27,7 @@ class Broken(Exception):
 
 def run(form, two, n_tiles, seed, steps=200000):
     """Whether every role ends."""
-    early, ks, vs = FORMS[form]
+    early, ks, vs, turns = FORMS[form]
     if not two:
         ks = vs = 2
     rnd = random.Random(seed)
@@ -34,7 +35,7 @@ def run(form, two, n_tiles, seed, steps=200000):
     k_full, v_full, v_ready = ([Bar(1) for _ in range(2)] for _ in range(3))
     k_empty, v_empty = ([Bar(slots) for _ in range(2)] for _ in range(2))
     s_full, s_free, p_full, pv_done = ([Bar(n) for _ in range(2)] for n in (2, 2, 2, 1))
-    started = Bar(1)
+    started, turn = Bar(1), [Bar(2), Bar(2)]
     pipes = [[], []]
     buffers = {}  # what lies in a buffer, and how many still read it
     met = [[0, 0], [0, 0]]
@@ -127,7 +128,7 @@ def run(form, two, n_tiles, seed, steps=200000):
 
     def softmax(t, half):
         for it in range(count(t)):
-            if t == 1 and it == 0:
+            if not turns and t == 1 and it == 0:
                 yield from wait(started, 0)
             yield from wait(s_full[t], it)
             read(f"s{t}", it, 1)
@@ -140,7 +141,11 @@ def run(form, two, n_tiles, seed, steps=200000):
                 s_free[t].arrive()
                 if it:
                     yield from wait(pv_done[t], it - 1)
+            if turns and (t == 1 or it):
+                yield from wait(turn[t], it - 1 if t == 0 else it)
             yield from pause(10)
+            if turns:
+                turn[t ^ 1].arrive()
             if not early:
                 read(f"s{t}", it, -1)
             have = buffers.get(f"p{t}", (None, 0))
@@ -192,7 +197,7 @@ def test_the_model_would_find_a_buffer_too_few():
     global FORMS
     kept = dict(FORMS)
     try:
-        FORMS["d64"] = (True, 2, 3)  # a third buffer of barriers that there are two of
+        FORMS["d64"] = (True, 2, 3, True)  # a third buffer of barriers that there are two of
         with pytest.raises((Broken, IndexError)):
             for seed in range(20):
                 run("d64", True, 9, seed)

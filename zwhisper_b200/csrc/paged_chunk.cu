@@ -58,6 +58,11 @@ template <int D, int P>
 constexpr bool SHARED = D == 128 && P == 1;
 template <int D, int P>
 constexpr bool EARLY = P == 1;  // the next S is computed as soon as this one has been read
+// The slots' exponentials take turns, so that one's run while the other loads scores, finds maxima and waits: left
+// alone they fall into step, and all wait for the same unit. 32 x 256 tokens after 1744, d 128 bf16 137 -> 130 us, f32
+// 271 -> 261, d 64 bf16 145 -> 134; d 64 in two pieces, whose slots wait for products in between, 200 -> 205: not there.
+template <int D, int P>
+constexpr bool TURNS = P == 1 || D == 128;
 __host__ __device__ constexpr uint32_t s_col(int t) { return t * 128u; }
 template <int D, int P>
 __host__ __device__ constexpr uint32_t p_col(int t) { return BESIDE<D, P> ? 384u + t * 64u : t * 128u; }
@@ -77,7 +82,7 @@ struct Smem {
     uint32_t valid[4];                  // of a tile: a bit for each 16 keys that lie in a page
     uint32_t flagged[EDGES][BN / 32];   // keys whose infinities and NaN were taken out
     uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_ready[2], v_empty[2], s_full[2], s_free[2], p_full[2], pv_done[2], drained[2];
-    uint64_t started;  // slot 0's first P is there
+    uint64_t started, turn[2];  // slot 0's first P is there; a slot may begin its exponentials
     uint32_t tmem_base;
 };
 
@@ -189,6 +194,8 @@ __global__ void __launch_bounds__(THREADS, 1)
             mbar_init(&sm.v_empty[i], two ? 2 : 1);
         }
         mbar_init(&sm.started, 1);
+        mbar_init(&sm.turn[0], 8);
+        mbar_init(&sm.turn[1], 8);
         fence_mbar_init();
     }
     __syncwarp();
@@ -462,7 +469,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int it = 0; ok && it < mine; it++) {
             const int j = two ? it : 2 * it + t, key0 = key_lo + j * BN;
             // slot 1 starts a softmax behind slot 0, so that the one's exponentials run during the other's products
-            if (t == 1 && it == 0) ok = mbar_wait_warp(&sm.started, 0, err);
+            if (!TURNS<D, P> && t == 1 && it == 0) ok = mbar_wait_warp(&sm.started, 0, err);
             ok = ok && mbar_wait_warp(&sm.s_full[t], it & 1, err);
             tc_fence_after();
             const uint32_t valid = sm.valid[j & 3];
@@ -543,6 +550,8 @@ __global__ void __launch_bounds__(THREADS, 1)
                     }
                 }
             }
+            // (a slot's last turn may be one that the other, with a tile less, does not wait for)
+            if (TURNS<D, P> && (t == 1 || it > 0)) ok = mbar_wait_warp(&sm.turn[t], (t == 0 ? it - 1 : it) & 1, err) && ok;
             const float2 u2 = make_float2(unit, unit), nb = make_float2(SHIFT - base, SHIFT - base);
             float2 sum[2] = {};
             if constexpr (P == 1) {
@@ -598,6 +607,11 @@ __global__ void __launch_bounds__(THREADS, 1)
                         tmem_st8(p_addr + c + k * 8, o);
                     }
                 }
+            }
+            if (TURNS<D, P>) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.turn[t ^ 1]);
+                __syncwarp();
             }
             const float2 s2 = __fadd2_rn(sum[0], sum[1]);
             l += s2.x + s2.y;
