@@ -482,6 +482,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(Kv8Attn p, int 
                         tc_fence_before();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&sm.s_free[t]);
+                        __syncwarp();  // the wait for the stores is for whole warps (.aligned)
                     }
                     l = l * alpha + (sum.x + sum.y);
                     tmem_st_wait();
