@@ -641,7 +641,7 @@ Plan plan_split(const Paged& c, const Seqs& s, int rows, bool raw, int sm_count)
     p.tiles = (rows + p.tile_rows - 1) / p.tile_rows;
     const long long ctas = (long long)s.n_batch * c.n_head_kv * p.tiles;
     const int key_turns = (keys_of(c, s) + GROUP * 128 / c.d - 1) / (GROUP * 128 / c.d);
-    const float turn = c.d == 64 ? raw ? 1.2f : 1.4f : raw ? 1.5f : 2.f;  // us of a turn, of which a warp has some
+    const float turn = c.d == 64 ? raw ? 1.5f : 1.8f : raw ? 1.5f : 2.f;  // us of a turn, of which a warp has some
     for (const bool big : {true, false}) {
         const int warps = big ? big_warps(p.tile_rows) : SMALL;
         const long long places = (long long)sm_count * (big_warps(p.tile_rows) / warps);
@@ -656,8 +656,10 @@ Plan plan_split(const Paged& c, const Seqs& s, int rows, bool raw, int sm_count)
         if (most > MAX_CLUSTER && turns(most) + 2 < turns(splits)) splits = most;
         // that takes more than 3 turns in the cluster, with these keys or fewer
         if (most > MAX_CLUSTER && useful > 3 * in_cluster) p.ws = std::max(p.ws, (size_t)ctas * most * p.tile_rows * (c.d + 4));
-        const float us = waves_of(ctas * splits, places) * (4.f + turn * turns(splits)) + (splits > MAX_CLUSTER ? 4.f : splits > 1 ? 2.f : 0.f) +
-                         (big ? 0.5f : 0.f);
+        // merges: of a cluster the longer the more CTAs it has (one sequence of 2256 tokens, 150 rows, in 7 big CTAs 14.1 us,
+        // in 14 small ones 18.6), of a big CTA's warps
+        const float merge = splits > MAX_CLUSTER ? 4.f : splits > 1 ? 2.f + 0.15f * splits : 0.f;
+        const float us = waves_of(ctas * splits, places) * (5.f + turn * turns(splits)) + merge + (big ? 0.5f : 0.f);
         if (big || us < p.us) {
             p.us = us;
             p.splits = splits;
