@@ -517,3 +517,23 @@ def test_a_workspace_serves_shorter_calls(env):
             assert w.cache.attn_workspace_bytes(n, H, past) <= size
             w.cache.attn(q, past, workspace=ws)
     ops.sync()
+
+
+def test_a_workspace_serves_lengths_of_their_own(env):
+    """What attn_workspace_bytes gives for a number of past tokens is enough for lengths on the device, up to it."""
+    torch, ops = env
+    rng = np.random.default_rng(11)
+    for B, n, H, d, bf16, most in ((64, 16, 12, 128, True, 8001), (40, 20, 12, 128, False, 4000), (3, 100, 8, 64, True, 9000)):
+        w = World(torch, ops, rng, B, 2, d, 64, most + n, bf16)
+        size = w.cache.attn_workspace_bytes(n, H, most)
+        ws = torch.empty(max(16, size), dtype=torch.uint8, device="cuda:0")
+        q = up(torch, normal(rng, B, n, H, d), w.row)
+        for top in (most, most // 2, most // 5, 100):
+            past = rng.integers(0, top + 1, B)
+            past[0] = top
+            out = w.cache.attn(q, i32(torch, past), max_past=top, workspace=ws)
+            alone = w.cache.attn(q, top, workspace=ws)
+            # a sequence's output does not depend on the others' lengths but for where its keys are cut
+            half = 2.0 ** (-7 if bf16 else -18)
+            torch.testing.assert_close(out[0].float(), alone[0].float(), rtol=half, atol=half)
+    ops.sync()

@@ -669,9 +669,11 @@ Plan plan_split(const Paged& c, const Seqs& s, int rows, bool raw, int sm_count)
     return p;
 }
 
-// The tcgen05 kernel: keys are cut while SMs stay empty, two tiles of keys to a cut at least. (More cuts where lengths
-// may differ, so that a long sequence holds up less: 32 sequences of up to 4001 tokens, 427 rows, d 64: 70 us, in two
-// cuts 77; the starts and ends of more CTAs and the second kernel take more than it saves.)
+// The tcgen05 kernel: keys are cut while SMs stay empty, two tiles of keys to a cut at least. Where sequences have lengths
+// of their own, one cut more, so that all SMs have work and the longest sequence holds up less, if the cuts still take
+// five times a CTA's start and end: 64 sequences of up to 8001 tokens, 96 rows, d 128, bf16: 141 us in one cut, 105
+// in two where lengths lie between 0 and that, 141 and 135 from half of it on, 144 and 166 if all are alike; of up to
+// 2000 (not cut): 42 and 49, 45 and 58, 46 and 65.
 Plan plan_chunk(const Paged& c, const Seqs& s, int rows, bool raw, int sm_count) {
     Plan p{};
     p.warps = 0;
@@ -679,11 +681,14 @@ Plan plan_chunk(const Paged& c, const Seqs& s, int rows, bool raw, int sm_count)
     p.tiles = (rows + PAGED_CHUNK_ROWS - 1) / PAGED_CHUNK_ROWS;
     const long long ctas = (long long)s.n_batch * c.n_head_kv * p.tiles;
     const int key_tiles = (keys_of(c, s) + PAGED_CHUNK_KEYS - 1) / PAGED_CHUNK_KEYS;
-    p.splits = (int)std::min<long long>(std::max<long long>(1, sm_count / ctas), std::max(1, key_tiles / 2));
-    if (p.splits > 1) p.ws = (size_t)ctas * p.splits * p.tile_rows * (c.d + 4);
     const bool two = rows > PAGED_CHUNK_ROWS / 2;
     const float start = c.d == 64 ? raw ? 9.f : 11.f : raw ? 11.f : 16.f;
     const float turn = c.d == 64 ? two ? raw ? 1.9f : 2.5f : raw ? 1.1f : 1.4f : two ? raw ? 2.5f : 5.4f : raw ? 1.9f : 2.5f;
+    p.splits = (int)std::min<long long>(std::max<long long>(1, sm_count / ctas), std::max(1, key_tiles / 2));
+    const bool more = ctas * p.splits < sm_count && turn * (key_tiles / (p.splits + 1)) >= 5.f * start;
+    const int most = p.splits + (more ? 1 : 0);  // the workspace is asked for with lengths of their own or without
+    if (s.past && more) p.splits++;
+    if (most > 1) p.ws = (size_t)ctas * most * p.tile_rows * (c.d + 4);
     p.us = waves_of(ctas * p.splits, sm_count) * (start + turn * ((key_tiles + p.splits - 1) / p.splits)) + (p.splits > 1 ? 2.f : 0.f);
     return p;
 }
@@ -691,8 +696,8 @@ Plan plan_chunk(const Paged& c, const Seqs& s, int rows, bool raw, int sm_count)
 // The tcgen05 kernel has four times the other one's rate and reads the keys once for 256 rows, not 16, but a CTA of it
 // takes 9 to 18 us to start and end. Above 16 rows the shorter estimate runs, its constants read off both kernels'
 // times for 24 to 256 rows a head, 1 to 64 sequences of 200 to 8000 tokens, both d, bf16 and f32: 16 sequences of 2000
-// tokens, d 128, bf16: 24 rows 17 us against the other's 18, 48 rows 27 against 20, 128 rows 45 against 21; one of
-// 2000 tokens: 128 rows 12.5 against 14.6. Up to 16 rows, where the other kernel reads the keys once too, it was never
+// tokens, d 128, bf16: 24 rows 16.4 us against this one's 20.0, 48 rows 26.4 against 18.4, 128 rows 45.5 against 20.9; one
+// of 2000 tokens: 128 rows 10.4 against 14.9. Up to 16 rows, where the other kernel reads the keys once too, it was never
 // the slower one by more than 5 %.
 Plan plan_for(const Paged& c, const Seqs& s, int n_head, bool raw, int sm_count) {
     const int rows = s.n * (n_head / c.n_head_kv);
