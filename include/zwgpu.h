@@ -757,7 +757,7 @@ ZWG_API int zwg_tree_accept(const zwg_seqs* s, const zwg_tree* tree, const int32
 
 /* Move the rows of token path[b][j] to slot past + j, j < n_path[b] (as zwg_tree_accept gives them; past and
  * n as in the calls before it), in n_caches caches (a HOST array: a model's layers, one launch for every
- * 64) that differ in k and v only. Rows behind them stay. A path that does not rise, or leaves the call's n
+ * 64) that differ in k and v only, no two of these one buffer. Rows behind them stay. A path that does not rise, or leaves the call's n
  * tokens, is skipped with its sequence. */
 ZWG_API int zwg_paged_keep(const zwg_paged* caches, size_t n_caches, const zwg_seqs* s, const int32_t* path,
                            const int32_t* n_path, void* stream);

@@ -137,6 +137,15 @@ def test_refusals():
     assert _lib.load().zwg_tree_accept(None, None, P, P, P, P, P, None) == _lib.ZWG_ERROR
 
 
+def test_one_buffer_twice():
+    """Rows that are moved or written twice in one call would race: refused, wherever the buffer comes again."""
+    one, two, three = cache(k=P, v=P + 16), cache(k=P + 32, v=P + 48), cache(k=P + 64, v=P)
+    refused(keep([one, two, one]), "buffer of cache 2 is given twice")
+    refused(keep([one, two, three]), "buffer of cache 2 is given twice")
+    refused(keep([two, cache(k=P, v=P)]), "buffer of cache 1 is given twice")
+    refused(append(c=cache(k=P, v=P)), "one buffer")
+
+
 def test_a_tree_of_one_line_is_a_chunk():
     for past, n, first in ((0, 1, 0), (5, 7, 2), (3, 4, 9)):
         line = list(range(-1, n - 1))

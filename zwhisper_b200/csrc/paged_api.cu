@@ -98,6 +98,7 @@ int zwg_paged_append(const zwg_paged* cache, const zwg_seqs* s, const zwg_tree* 
     if (!q_out) q_out = q;
     if (!rc && q) rc = check_rows(q, s, n_head * cache->d, type, false, what, "q");
     if (!rc && q) rc = check_rows(q_out, s, n_head * cache->d, type, true, what, "q_out");
+    if (!rc && cache->k == cache->v) rc = fail("%s: k and v of the cache are one buffer", what);
     if (rc) return rc;
     Ctx* c = cur();
     if (!c) return ZWG_ERROR;
@@ -201,6 +202,12 @@ int zwg_paged_keep(const zwg_paged* caches, size_t n_caches, const zwg_seqs* s, 
     if (s->n > ZWG_MAX_TREE) return fail("%s: %zu tokens, at most %d are taken", what, s->n, ZWG_MAX_TREE);
     if (!path || !n_path) return fail("%s: null path", what);
     if (!al(path, 4)) return fail("%s: path must be 4-byte aligned", what);
+    for (size_t i = 0; i < n_caches; i++) {  // rows that were moved may not be moved again
+        const void *k = caches[i].k, *v = caches[i].v;
+        bool twice = k == v;
+        for (size_t j = 0; j < i; j++) twice |= caches[j].k == k || caches[j].v == k || caches[j].k == v || caches[j].v == v;
+        if (twice) return fail("%s: a buffer of cache %zu is given twice", what, i);
+    }
     Ctx* c = cur();
     if (!c) return ZWG_ERROR;
     const OnDevice on(c->device);
