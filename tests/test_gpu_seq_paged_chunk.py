@@ -209,3 +209,32 @@ def test_scores_of_any_size(env, bf16):
         before = torch.zeros_like(q)
         out = attend(torch, w.cache, q, 680, out=before.clone())
         check_attn(torch, out, before, w, q, [680] * 40, [20] * 40, [0] * 40, None, 0 if bf16 else 2)
+
+
+@pytest.mark.parametrize("B", [2, 3, 255, 256, 257, 300])
+@pytest.mark.parametrize("bad", [False, True])
+def test_every_sequence_of_many_lengths_is_taken_once(env, B, bad):
+    """CTAs take up to 256 sequences in the order of their lengths, many of them alike here; an entry out of range is left
+    out, and the others stand."""
+    torch, ops = env
+    rng = np.random.default_rng(B)
+    n, most = (130 if B > 3 else 250), (90 if B > 3 else 3000)
+    w = World(torch, ops, rng, B, 1, 64, 16, most + n, True)
+    past = rng.choice([0, 1, 40, most - 1, most], B)
+    q = up(torch, 1.5 * normal(rng, B, n, 2, 64), w.row)
+    before = up(torch, normal(rng, B, n, 2, 64), w.row)
+    given, count = past.copy(), np.full(B, n)
+    if bad:
+        given[B // 2], count[B // 2] = most + 7, 0  # (count: of what check_attn expects)
+        if B > 3:
+            given[1], count[1] = -(2 ** 31), 0
+    out = attend(torch, w.cache, q, i32(torch, given), max_past=most, out=before.clone())
+    if bad:
+        with pytest.raises(RuntimeError):
+            ops.sync()
+    else:
+        ops.sync()
+    for b in range(B):  # rows that are written differ from those that were there
+        same = (out[b] == before[b]).all(-1).all(-1).sum().item()
+        assert same == n - count[b], (b, same)
+    check_attn(torch, out, before, w, q, past, count, np.zeros(B, int), None, 0)

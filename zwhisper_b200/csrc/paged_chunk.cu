@@ -14,6 +14,7 @@
 // f16 pieces: P's pieces hold 2^11 p with p below 2^4; the tensor cores truncate their sums, so each tile's O starts
 // from zero and is added in f32 to the row's in the thread's registers.
 #include <algorithm>
+#include <climits>
 #include <cmath>
 
 #include "chain.cuh"
@@ -129,21 +130,25 @@ ZWG_DEV uint32_t finite(uint32_t w, uint32_t exponent) {
 // The whole CTA: the sequence that comes n-th by its length, longest first, so that the last CTAs to start are the
 // shortest ones (16 sequences of up to 1750 tokens, 250 new ones, 14 / 2 heads of d 64, f32: 75 -> 61 us; 64 of up to
 // 1000, 128 new ones, d 128, bf16: 85 -> 72). All CTAs see the same lengths; the lower index goes first where they are
-// equal. scratch: n_batch + 1 ints, free behind the call.
-ZWG_DEV int by_length(const Seqs& s, int n, int z, int* scratch) {
-    const int i = threadIdx.x, mine = i < s.n_batch ? __ldcg(s.past + i + z) : 0;
-    if (i < s.n_batch) scratch[1 + i] = mine;
+// equal. Up to MOST_SORTED sequences: a CTA compares each with all, and SMs have several CTAs of more of them in turn, so
+// that one long one holds up less. scratch: MOST_SORTED + 4 ints, free behind the call.
+constexpr int MOST_SORTED = 256;
+ZWG_DEV int by_length(const Seqs& s, int n, int z, int4* scratch) {
+    int* lengths = reinterpret_cast<int*>(scratch);
+    const int i = threadIdx.x, padded = (s.n_batch + 3) & ~3, mine = i < s.n_batch ? __ldcg(s.past + i + z) : INT_MIN;
+    if (i < padded) lengths[i] = mine;  // (behind the last sequence: shorter than any, or as short and after it)
     __syncthreads();
     if (i < s.n_batch) {
         int before = 0;
-        for (int j = 0; j < s.n_batch; j++) {
-            const int other = scratch[1 + j];
-            before += other > mine || (other == mine && j < i);
+        for (int j = 0; j < padded; j += 4) {
+            const int4 w = scratch[j / 4];
+            before += (w.x > mine || (w.x == mine && j < i)) + (w.y > mine || (w.y == mine && j + 1 < i)) +
+                      (w.z > mine || (w.z == mine && j + 2 < i)) + (w.w > mine || (w.w == mine && j + 3 < i));
         }
-        if (before == n) scratch[0] = i;
+        if (before == n) lengths[MOST_SORTED] = i;
     }
     __syncthreads();
-    const int b = scratch[0];
+    const int b = lengths[MOST_SORTED];
     __syncthreads();
     return b;
 }
@@ -172,7 +177,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     const bool tree = p.tree.parent != nullptr;
     int b = blockIdx.y / p.c.n_head_kv;
     const int h = blockIdx.y - b * p.c.n_head_kv;
-    if (p.s.past && p.s.n_batch > 1 && p.s.n_batch <= THREADS) b = by_length(p.s, b, z, reinterpret_cast<int*>(&sm));
+    if (p.s.past && p.s.n_batch > 1 && p.s.n_batch <= MOST_SORTED) b = by_length(p.s, b, z, reinterpret_cast<int4*>(&sm));
     const int bh = b * p.c.n_head_kv + h;
     const Place at = place_of(p.s, b, p.c.room, threadIdx.x == 0 && blockIdx.x == 0 && h == 0 ? p.err : nullptr);
     const int rows = at.count * group, row0 = tile * 2 * BM;
