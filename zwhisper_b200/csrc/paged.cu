@@ -47,7 +47,8 @@ ZWG_DEV void rounded(const float (&a)[N], Vec<H, N>& o) {
 // Bound by memory: every row in once, out once. A thread takes a piece of 8 elements (or, where pairs are
 // halves, both sides' pieces) of up to eight (four) of a token's q, k and v heads: they share its table entries, and all
 // its loads are on their way before the first is used. Rows that are not aligned for that, and rotated parts
-// that do not divide into it, go four elements or one at a time.
+// that do not divide into it, go four elements or one at a time. In a graph: 64 x 256 tokens, 12 + 2 heads of d 128, bf16,
+// interleaved, 24.9 us (134 MB in and out: 5.4 TB/s; issue slots 62 % busy); 64 steps of a token, f32, 2.8 us.
 constexpr int heads_of(bool one) { return one ? 8 : 4; }  // of a thread: eight pieces on their way
 
 // N: elements a thread moves at a time (8, 4, or 1). Threads: (piece, group of heads, token).
@@ -192,7 +193,8 @@ int append_type(const PagedAppend& p, cudaStream_t st) {
 // From node 0, whose token is already chosen: the child with the lowest index whose token is what the model
 // says after its parent, as long as there is one. A warp takes a sequence: a lane holds every 32nd token and
 // its parent, a step is a lane's scan of its own and a minimum over the lanes. Bound by latency: the loads,
-// then about 40 cycles and n / 32 compares a step.
+// then about 40 cycles and n / 32 compares a step. With the kept rows behind it, in a graph: 4.7 us for one tree of 25
+// tokens and 28 caches, 7.1 for 64 trees of 61 and 24 caches.
 constexpr int PER_LANE = MOST_TREE / 32;
 __global__ void __launch_bounds__(32) tree_accept_kernel(TreeAccept p) {
     chain_release();

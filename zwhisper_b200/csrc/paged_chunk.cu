@@ -1,18 +1,26 @@
 // Attention over a cache in pages for many query rows of a kv head (prompt chunks, trees of drafted tokens), on the
 // tcgen05 tensor cores: the formulas of paged_attn.cu with 128 keys and 2 x 128 query rows at a time.
 //
-// paged_chunk_kernel. A CTA of 12 warps takes 256 rows (row = query * group + head) of one (sequence, kv head), or a
-// cut of their keys, in two slots of 128 rows; where it has 128 rows or less, both slots take them and every other
-// tile of keys, so that one's softmax still runs during the other's products, and their sums meet in shared memory at
-// the end. Warps 0-3 and 4-7 are the slots' softmax, a thread a row; warps 8 and 9 issue the products of one slot
-// each: S = Q K^T (from shared memory) into TMEM, then O += P V (P from TMEM, in S's place, or beside it where there is
-// room, so that the next S is computed during this one's softmax); warp 10 brings keys and values by TMA, a box to
-// each page, in the 128-byte swizzle (keys K-major, values MN-major: neither is transposed); warp 11 sees to it that
-// values of slots that no row sees are zero, and takes out infinities and NaN that only some rows see (noted in
-// `flagged`; the rows that do see them take them in at the end, by themselves).
-// bf16 rows: O stays in TMEM and is rescaled there only where a row's maximum grows by more than 2^8. f32 rows in two
-// f16 pieces: P's pieces hold 2^11 p with p below 2^4; the tensor cores truncate their sums, so each tile's O starts
-// from zero and is added in f32 to the row's in the thread's registers.
+// paged_chunk_kernel. A CTA of 20 warps takes 256 rows (row = query * group + head) of one (sequence, kv head), or
+// a cut of their keys, in two slots of 128 rows; where it has 128 rows or less, both slots take them and every
+// other tile of keys, so that one's softmax still runs during the other's products, and their sums meet in shared
+// memory at the end. Warps 0-7 and 8-15 are the slots' softmax, two threads a row that take half of a tile's keys
+// (and later half of O's columns) each, so that these stay in its registers, and tell each other their maxima.
+// Warps 16 and 17 issue the products of one slot each, S = Q K^T (from shared memory) into TMEM and O += P V; warp
+// 18 brings keys and values by TMA, a box to each page, in the 128-byte swizzle (keys K-major, values MN-major:
+// neither is transposed); warp 19 sees to it that values of slots that no row sees are zero, and takes out
+// infinities and NaN that only some rows see (noted in `flagged`; the rows that do see them take them in at the
+// end, by themselves).
+// One piece: P goes beside S (d 64) or into shared memory (d 128), so that the next S is computed during this
+// one's softmax; O stays in TMEM and is rescaled there only where a row's maximum grows by more than 2^8 (bf16
+// rows) or 2^4.
+// Two f16 pieces (f32 rows; P's hold 2^11 p with p below 2^4): P goes over S, and as the tensor cores truncate
+// their sums, each tile's O starts from zero and is added in f32 to the row's in the threads' registers.
+// Bound by the softmax beside the products: 32 sequences of 256 tokens after 1744, 12 / 2 heads of d 128, bf16, in
+// a graph, 130.6 us (57 us of products at the rate of a large bf16 product), the tensor cores are busy 42 % of the
+// time, the exponentials' unit 41 %, issue 52 %, and DRAM reads 93 MB; f32 in two pieces 261 us for twice the
+// products; 16 sequences of up to 1750 tokens with 250 new ones, 14 / 2 heads of d 64, f32, 61 us, of which about
+// 16 are a CTA's start and end.
 #include <algorithm>
 #include <climits>
 #include <cmath>
