@@ -74,6 +74,7 @@ SHAPES = [  # batch, n, heads, heads_kv, d, page, past, tree
     (3, 20, 12, 2, 128, 16, 6000, True),     # cut keys, both slots
     (2, 130, 4, 1, 64, 64, 5000, False),     # cut keys, three CTAs of rows
     (5, 40, 16, 2, 128, 256, 3000, False), (4, 256, 4, 2, 64, 128, 2000, True), (70, 128, 2, 1, 128, 64, 77, False),
+    (60, 30, 6, 1, 64, 32, 3000, True),      # more cuts than fit at once where lengths differ
     (100, 40, 8, 2, 64, 256, 0, False), (90, 100, 8, 2, 128, 16, 0, True),
 ]
 
