@@ -196,7 +196,8 @@ __global__ void __launch_bounds__(32 * WARPS, big_warps(8 * NT) / WARPS)
     int turn = rg.from + warp, pages = 0, it = 0;
     const auto look = [&](int from) {
         const int mine = from + lane / U * WARPS, slot = mine * TURN + lane % U * GROUP;
-        pages = mine < to && slot < rg.end ? page_of(p.c, b, slot + z) : 0;
+        // only where a row sees one of the 16: pages before the first key may have been given back
+        pages = mine < to && max(slot, first) < min(slot + GROUP, rg.end) ? page_of(p.c, b, slot + z) : 0;
         if (pages < 0) set_error(p.err, kErrBounds);  // its keys are not seen
     };
     const auto page_in = [&](int (&page)[U]) {

@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             const int log_box = min(p.c.log_page, 7), box = 1 << log_box, n_box = BN >> log_box;  // a box's rows, a tile's boxes
             const auto look = [&](int j) {  // the page of the lane's box; -1: none of the pool's, -2: not needed
                 const int slot = key_lo + j * BN + lane * box;
-                if (j >= n_tiles || lane >= n_box || slot >= end || slot + box <= first) return -2;
+                if (j >= n_tiles || lane >= n_box || max(slot, first) >= min(slot + box, end)) return -2;
                 return page_of(p.c, b, slot + z);
             };
             int issued = 0, next = look(0);
