@@ -203,3 +203,22 @@ def test_rotary_tables_that_start_anywhere(env, d, rot, inter, bf16):
     ops.sync()
     for other in results[1:]:
         assert all(torch.equal(a, b) for a, b in zip(results[0], other))
+
+
+@pytest.mark.parametrize("B,n,H,d,slots", [(1, 1, 12, 64, 40000), (1, 100, 12, 128, 4000), (3, 300, 4, 64, 256), (1, 140, 12, 128, 96),
+                                           (1, 600, 4, 128, 512)])
+@pytest.mark.parametrize("kv8", [False, True])
+def test_a_workspace_for_lengths_up_to_the_caches_end(env, B, n, H, d, slots, kv8):
+    """Lengths and counts on the device: past tokens up to the cache's end, or more tokens in the call than it holds."""
+    torch, ops = env
+    rng = np.random.default_rng(slots)
+    slots = -(-slots // 32) * 32
+    cache = ops.Kv8Cache.empty(B, 2, d, slots) if kv8 else World(torch, ops, rng, B, 2, d, 16, slots - 32, False).cache
+    n_ctx, count = cache.n_ctx, rng.integers(1, min(n, 9) + 1, B)
+    past = i32(torch, n_ctx - 40 - count if n_ctx > 100 else [0] * B)
+    q = up(torch, normal(rng, B, n, H, d))
+    want = cache.attn(q, past, count=i32(torch, count), max_past=n_ctx)
+    for size in (cache.attn_workspace_bytes(n, H, n_ctx), cache.attn_workspace_bytes(n, H)):
+        ws = torch.empty(max(16, size), dtype=torch.uint8, device="cuda:0")
+        assert torch.equal(cache.attn(q, past, count=i32(torch, count), max_past=n_ctx, workspace=ws, out=torch.zeros_like(q)), want)
+    ops.sync()

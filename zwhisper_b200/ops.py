@@ -897,6 +897,15 @@ def _seqs(n_batch: int, n: int, n_past, count, first, max_past, device):
                                    None if first is None else _int32_of(first, device, (n_batch,), "first")))
 
 
+def _any_seqs(cache, n: int, n_past):
+    """A reference to the zwg_seqs of calls of n tokens whose lengths are at most n_past (None: the cache's end), for a
+    question about their sizes: the address for lengths on the device says that there are some, and is not read."""
+    n_past = cache.n_ctx if n_past is None else operator.index(n_past)
+    if n_past < 0:
+        raise ValueError(f"n_past must not be negative, got {n_past}")
+    return ctypes.byref(_lib.SeqsC(cache.n_batch, n, n_past, 4, None, None))
+
+
 def _stream_on(device):
     """The current stream of a device, as _stream_of, without making a Stream object for it."""
     return _torch()._C._cuda_getCurrentRawStream(device.index)
@@ -1030,8 +1039,9 @@ class Kv8Cache:
         return k, v
 
     def attn_workspace_bytes(self, n: int, n_head: int, n_past=None) -> int:
-        """Workspace of attn for n tokens after n_past (None: the most there can be)."""
-        s = self._call(n, max(self.n_ctx - n, 0) if n_past is None else n_past, None, None, None)
+        """Workspace of attn for n tokens after n_past (None: the most there can be), a number or the most that
+        lengths on the device may be (attn's max_past)."""
+        s = _any_seqs(self, n, n_past)
         return int(_ready(self.device).zwg_kv8_attn_workspace(self._ref, s, n_head))
 
     def attn(self, q, n_past, count=None, first=None, max_past=None, out=None, workspace=None):
@@ -1177,8 +1187,9 @@ class PagedCache:
         return q if q_out is None else q_out
 
     def attn_workspace_bytes(self, n: int, n_head: int, n_past=None) -> int:
-        """Workspace of attn for n tokens after n_past (None: the most there can be)."""
-        s = self._call(n, max(self.n_ctx - n, 0) if n_past is None else n_past, None, None, None)
+        """Workspace of attn for n tokens after n_past (None: the most there can be), a number or the most that
+        lengths on the device may be (attn's max_past)."""
+        s = _any_seqs(self, n, n_past)
         return int(_ready(self.device).zwg_paged_attn_workspace(self._ref, s, n_head))
 
     def attn(self, q, n_past, count=None, first=None, tree=None, max_past=None, out=None, workspace=None):
