@@ -124,7 +124,7 @@ ZWG_DEV Range range_of(Place at, int first, int group, int tile, int split, int 
     const int q0 = r.row0 / group, q1 = (min(r.rows, r.row0 + R) - 1) / group;
     r.seen_by_all = tree ? at.past : at.past + q0 + 1;  // slots below it: by every row of the tile
     r.end = at.past + q1 + 1;                           // slots from it on: by none
-    const int lo = first / KEYS, n = max(0, (r.end + KEYS - 1) / KEYS - lo);
+    const int lo = first / KEYS, n = first < r.end ? (r.end + KEYS - 1) / KEYS - lo : 0;
     const int each = n / splits, more = n - each * splits;
     r.from = lo + split * each + min(split, more);
     r.to = r.from + each + (split < more ? 1 : 0);
@@ -196,8 +196,8 @@ __global__ void __launch_bounds__(32 * WARPS, big_warps(8 * NT) / WARPS)
     int turn = rg.from + warp, pages = 0, it = 0;
     const auto look = [&](int from) {
         const int mine = from + lane / U * WARPS, slot = mine * TURN + lane % U * GROUP;
-        // only where a row sees one of the 16: pages before the first key may have been given back
-        pages = mine < to && max(slot, first) < min(slot + GROUP, rg.end) ? page_of(p.c, b, slot + z) : 0;
+        // (a turn of two pages may begin with one before the first key, which may have been given back)
+        pages = mine < to && slot < rg.end && (U == 1 || slot + GROUP > first) ? page_of(p.c, b, slot + z) : 0;
         if (pages < 0) set_error(p.err, kErrBounds);  // its keys are not seen
     };
     const auto page_in = [&](int (&page)[U]) {

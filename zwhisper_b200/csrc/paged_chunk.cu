@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     const bool two = row0 + BM < rows;                                     // a slot to each 128 rows
     const int end = at.past + (min(rows, row0 + 2 * BM) - 1) / group + 1;  // slots from it on: seen by no row
     const int by_all = tree ? at.past : at.past + row0 / group + 1;        // slots below it: by all
-    const int lo = first / BN, all = max(0, (end + BN - 1) / BN - lo);
+    const int lo = first / BN, all = first < end ? (end + BN - 1) / BN - lo : 0;
     const int from = (int)((long long)all * split / splits), n_tiles = (int)((long long)all * (split + 1) / splits) - from;
     const int key_lo = (lo + from) * BN;
     const int edge0 = max(0, by_all / BN - lo - from);  // the first tile (of this CTA) that not all rows see whole
@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             const int log_box = min(p.c.log_page, 7), box = 1 << log_box, n_box = BN >> log_box;  // a box's rows, a tile's boxes
             const auto look = [&](int j) {  // the page of the lane's box; -1: none of the pool's, -2: not needed
                 const int slot = key_lo + j * BN + lane * box;
-                if (j >= n_tiles || lane >= n_box || max(slot, first) >= min(slot + box, end)) return -2;
+                if (j >= n_tiles || lane >= n_box || slot >= end || slot + box <= first) return -2;
                 return page_of(p.c, b, slot + z);
             };
             int issued = 0, next = look(0);
