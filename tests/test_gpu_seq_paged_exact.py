@@ -67,6 +67,7 @@ CODES = [  # batch, n, heads, heads_kv, d, page, past (most), tree, what runs
     (40, 24, 12, 2, 128, 16, 200, False, "chunk"), (40, 21, 12, 2, 128, 32, 1301, False, "chunk"), (64, 16, 14, 2, 64, 16, 150, True, "chunk"),
     (32, 256, 2, 2, 64, 64, 1744, False, "chunk cuts"), (60, 30, 6, 1, 64, 32, 3000, True, "chunk cuts"),
     (80, 256, 2, 2, 64, 64, 1744, False, "chunk"), (80, 61, 12, 2, 128, 16, 777, True, "chunk"),
+    (1, 2100, 12, 2, 128, 16, 1, False, "any"), (2, 3001, 2, 1, 64, 32, 200, False, "any"), (1, 700, 8, 8, 64, 64, 77, False, "any"),
     (3, 20, 12, 2, 128, 16, 6000, True, "chunk cuts"), (2, 130, 4, 1, 64, 64, 5000, False, "chunk cuts"),
     (4, 256, 4, 2, 64, 128, 2000, True, "chunk cuts"), (2, 100, 12, 2, 128, 256, 30001, False, "chunk cuts"),
 ]
@@ -222,3 +223,47 @@ def test_a_workspace_for_lengths_up_to_the_caches_end(env, B, n, H, d, slots, kv
         ws = torch.empty(max(16, size), dtype=torch.uint8, device="cuda:0")
         assert torch.equal(cache.attn(q, past, count=i32(torch, count), max_past=n_ctx, workspace=ws, out=torch.zeros_like(q)), want)
     ops.sync()
+
+
+SOME = [(2, 1, 12, 2, 128, 16, 700), (1, 1, 14, 2, 64, 16, 30000), (2, 6, 12, 2, 64, 32, 300), (40, 24, 12, 2, 128, 16, 200), (2, 100, 12, 2, 128, 64, 5000)]
+
+
+@pytest.mark.parametrize("B,n,H,Hkv,d,page,past", SOME)
+@pytest.mark.parametrize("bf16", [False, True])
+def test_a_query_that_is_no_number_spoils_its_own_row(env, B, n, H, Hkv, d, page, past, bf16):
+    torch, ops = env
+    rng = np.random.default_rng(n)
+    w = World(torch, ops, rng, B, Hkv, d, page, past + n, bf16)
+    q = up(torch, normal(rng, B, n, H, d), w.row)
+    want = w.cache.attn(q, past)
+    bad = torch.zeros(B, n, H, dtype=torch.bool, device="cuda:0")
+    for i, x in enumerate((float("nan"), float("inf"), -float("inf"))):
+        b, t, h = B - 1, (i * n) // 3, (5 * i + 1) % H
+        q[b, t, h, (7 * i) % d] = x
+        bad[b, t, h] = True
+    got = w.cache.attn(q, past)
+    ops.sync()
+    assert torch.equal(got[~bad], want[~bad]) and not torch.isfinite(got[bad]).any()
+
+
+@pytest.mark.parametrize("B,n,H,Hkv,d,page,past", SOME)
+@pytest.mark.parametrize("bf16", [False, True])
+def test_a_table_that_is_part_of_a_wider_one(env, B, n, H, Hkv, d, page, past, bf16):
+    """Rows of the table further apart than they are long, and not from a 16-byte boundary on."""
+    torch, ops = env
+    rng = np.random.default_rng(n)
+    w = World(torch, ops, rng, B, Hkv, d, page, past + n, bf16)
+    wide = torch.full((B + 2, w.cache.table.shape[1] + 5), 1 << 30, dtype=torch.int32, device="cuda:0")
+    part = wide[1:B + 1, 3:3 + w.cache.table.shape[1]]
+    part.copy_(w.cache.table)
+    pools = [x.clone() for x in (w.cache.k, w.cache.v)]
+    other = ops.PagedCache(*pools, part)
+    q, k, v = (up(torch, normal(rng, B, n, h, d), w.row) for h in (H, Hkv, Hkv))
+    path, kept = i32(torch, [[n - 1] + [-1] * (n - 1)] * B), i32(torch, [1] * B)
+    out = []
+    for c in (w.cache, other):
+        c.append(k, v, past)
+        out.append(c.attn(q, past))
+        ops.paged_keep(c, path, kept, past)
+    ops.sync()
+    assert torch.equal(*out) and torch.equal(other.k, w.cache.k) and torch.equal(other.v, w.cache.v)
