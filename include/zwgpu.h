@@ -582,7 +582,7 @@ ZWG_API int zwg_gemm_f16(const uint16_t* a, size_t lda, size_t a_bs, const uint1
  * where `past` (device int32 [n_batch]) is given; n_past is then the most that past[b] may
  * be. count (device int32 [n_batch], or NULL): sequence b has count[b] <= n tokens in this
  * call, and rows i >= count[b] of every buffer are neither read nor written. first (device
- * int32 [n_batch], or NULL; zwg_kv8_attn only): keys before first[b] are not seen (a batch
+ * int32 [n_batch], or NULL; attention only): keys before first[b] are not seen (a batch
  * padded on the left); first[b] may lie behind them all, so that a query sees none. A sequence
  * whose past[b] or count[b] is out of range (below 0, past[b] > n_past, count[b] > n, beyond the
  * cache or the tables), or whose first[b] is below 0, is skipped: its rows stay as they were, and
@@ -689,10 +689,10 @@ ZWG_API int zwg_kv8_attn(const zwg_kv8* c, const zwg_seqs* s, int type, size_t n
 
 /* The cache: d 64 or 128, `page` a power of two from 16 to 256,
  *   k, v   [n_pages][n_head_kv][page][d] of `type`, pages `page_stride` elements apart (a multiple
- *          of 8, at least n_head_kv * page * d, below 2^38; k and v may share a buffer that way), 16-byte
- *          aligned
+ *          of 8, at least n_head_kv * page * d, below 2^38; k and v may share a buffer that way, but may not
+ *          overlap in another), 16-byte aligned
  *   table  int32 [n_batch][max_pages], rows table_stride apart; an entry outside [0, n_pages) is
- *          no page (-1, say, behind a sequence's last one)
+ *          no page (-1, say, behind a sequence's last one, or before the one of its first[b])
  * ZWG_TYPE_F16 caches take f32 rows, rounded to the nearest f16 (infinite from 65520 on), ZWG_TYPE_BF16
  * ones bf16 rows. Where a call needs a slot whose entry is no page, the device error word is set
  * (reported by zwg_sync) and the slot is left out: not written, or not seen. Pages that two
@@ -733,7 +733,7 @@ ZWG_API size_t zwg_paged_attn_workspace(const zwg_paged* c, const zwg_seqs* s, s
 /* Attention of the call's queries (n_head a multiple of n_head_kv; query head h reads kv head
  * h / (n_head / n_head_kv)) over the pages, which hold the call's tokens already. Query i of sequence b
  * sees slots first[b] .. past + i, or with a tree first[b] .. past - 1, past + i and those of the tokens above
- * it. Softmax of q . k / sqrt(d) in f32, sums in f32; a query that sees no key gives zeros; what lies in
+ * it (none below first[b], where that lies behind past). Softmax of q . k / sqrt(d) in f32, sums in f32; a query that sees no key gives zeros; what lies in
  * slots that a query does not see (infinities and NaN too) leaves its output alone; an infinity or a NaN
  * among values that it sees gives one of the two in its own column. The context's math
  * mode applies to f32 queries: ZWG_MATH_F32 holds each query and probability in two f16 pieces (22 bits) against

@@ -35,6 +35,13 @@ ZWG_DEV float up(__nv_bfloat16 x) { return __bfloat162float(x); }
 ZWG_DEV void add(float& x, float y) { x += y; }
 ZWG_DEV void add(__nv_bfloat16& x, float y) { x = __float2bfloat16_rn(__bfloat162float(x) + y); }
 
+// A word's two 16-bit elements, those that are infinite or NaN as zero.
+ZWG_DEV uint32_t finite(uint32_t w, uint32_t exponent) {
+    if ((w & exponent) == exponent) w &= 0xffff0000u;
+    if ((w & exponent << 16) == exponent << 16) w &= 0xffffu;
+    return w;
+}
+
 // The page of sequence b's slot (below c.room), or -1: the table's entry is not one of the pool's.
 ZWG_DEV int page_of(const Paged& c, int b, int slot) {
     const int id = __ldcg(c.table + b * c.ts + (slot >> c.log_page));

@@ -39,11 +39,11 @@ namespace {
 
 namespace cg = cooperative_groups;
 using kv8::kLog2e;
-using kv8::load16;
 using kv8::pieces_of;
 using kv8::power_of;
 using kv8::store4;
 using kv8::wide;
+using paged::finite;
 using paged::Held;
 using paged::page_of;
 using paged::read_tree;
@@ -77,13 +77,6 @@ ZWG_DEV uint32_t transpose8x8(uint32_t x) {
 
 ZWG_DEV uint4 load_cached(const uint16_t* p) { return __ldcg(reinterpret_cast<const uint4*>(p)); }
 ZWG_DEV uint32_t word(const uint4& w, int i) { return i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w; }
-
-// A word's two 16-bit elements, those that are infinite or NaN as zero.
-ZWG_DEV uint32_t finite(uint32_t w, uint32_t exponent) {
-    if ((w & exponent) == exponent) w &= 0xffff0000u;
-    if ((w & exponent << 16) == exponent << 16) w &= 0xffffu;
-    return w;
-}
 
 ZWG_DEV void add4(float4& a, float f, float4 x) {
     a.x += f * x.x;
@@ -705,8 +698,10 @@ Plan plan_chunk(const Paged& c, const Seqs& s, int rows, bool raw, int sm_count)
 // takes 9 to 18 us to start and end. Above 16 rows the shorter estimate runs, its constants read off both kernels'
 // times for 24 to 256 rows a head, 1 to 64 sequences of 200 to 8000 tokens, both d, bf16 and f32: 16 sequences of 2000
 // tokens, d 128, bf16: 24 rows 16.4 us against this one's 20.0, 48 rows 26.4 against 18.4, 128 rows 45.5 against 20.9; one
-// of 2000 tokens: 128 rows 10.4 against 14.9. Up to 16 rows, where the other kernel reads the keys once too, it was never
-// the slower one by more than 5 %.
+// of 2000 tokens: 128 rows 10.4 against 14.9. Over 288 calls (18 to 258 rows, 1 to 64 sequences of
+// 200 to 8000 tokens, both d and types) the one that runs takes 1.00 of the better one's time in the middle, 1.02 at the
+// 95th of a hundred, 1.33 at the most (4 sequences of 2000 tokens, 96 rows, d 64, bf16: 14.8 us for 11.2). Up to 16
+// rows, where the other kernel reads the keys once too, it was never the slower one by more than 5 %.
 Plan plan_for(const Paged& c, const Seqs& s, int n_head, bool raw, int sm_count) {
     const int rows = s.n * (n_head / c.n_head_kv);
     Plan split = plan_split(c, s, rows, raw, sm_count);

@@ -17,10 +17,12 @@
 // Two f16 pieces (f32 rows; P's hold 2^11 p with p below 2^4): P goes over S, and as the tensor cores truncate
 // their sums, each tile's O starts from zero and is added in f32 to the row's in the threads' registers.
 // Bound by the softmax beside the products: 32 sequences of 256 tokens after 1744, 12 / 2 heads of d 128, bf16, in
-// a graph, 130.6 us (57 us of products at the rate of a large bf16 product), the tensor cores are busy 42 % of the
-// time, the exponentials' unit 41 %, issue 52 %, and DRAM reads 93 MB; f32 in two pieces 261 us for twice the
-// products; 16 sequences of up to 1750 tokens with 250 new ones, 14 / 2 heads of d 64, f32, 61 us, of which about
-// 16 are a CTA's start and end.
+// a graph, 130.6 us (57 us of products at the rate of a large bf16 product). Of the cycles in which an SM has a CTA the
+// tensor cores are busy 42 %, the exponentials' unit 41 %, issue 52 %; of all cycles the tensor cores 32 %, as 384
+// CTAs fill 148 SMs 2.6 times. DRAM reads 93 MB. f32 in two pieces 262 to 276 us, by the scores, for twice the
+// products; 16 sequences of up to 1750 tokens with 250 new ones, 14 / 2 heads of d 64, f32, 61 to 63 us, of which about
+// 16 are a CTA's start and end. A softmax thread's 104 registers are too few in every form: bytes spilled and read back
+// bf16 132 / 328 (d 128), 108 / 316 (d 64); f32 in two pieces 304 / 492, 188 / 240; in one 140 / 336, 108 / 316.
 #include <algorithm>
 #include <climits>
 #include <cmath>
@@ -46,6 +48,7 @@ using kv8::power_of;
 using kv8::store4;
 using kv8::value_of;
 using kv8::wide;
+using paged::finite;
 using paged::Held;
 using paged::page_of;
 using paged::read_tree;
@@ -69,7 +72,7 @@ template <int D, int P>
 constexpr bool EARLY = P == 1;  // the next S is computed as soon as this one has been read
 // The slots' exponentials take turns, so that one's run while the other loads scores, finds maxima and waits: left
 // alone they fall into step, and all wait for the same unit. 32 x 256 tokens after 1744, d 128 bf16 137 -> 130 us, f32
-// 271 -> 261, d 64 bf16 145 -> 134; d 64 in two pieces, whose slots wait for products in between, 200 -> 205: not there.
+// 271 -> 261, d 64 (14 / 2 heads) bf16 145 -> 134; d 64 in two pieces, whose slots wait for products in between, 200 -> 205: not there.
 template <int D, int P>
 constexpr bool TURNS = P == 1 || D == 128;
 __host__ __device__ constexpr uint32_t s_col(int t) { return t * 128u; }
@@ -128,11 +131,6 @@ ZWG_DEV uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u
 ZWG_DEV bool not_finite(uint4 w, uint32_t exponent) {
     const uint32_t k = (0x8000u - exponent) * 0x10001u, m = 0x7fff7fffu;
     return (((w.x & m) + k | (w.y & m) + k | (w.z & m) + k | (w.w & m) + k) & 0x80008000u) != 0;
-}
-ZWG_DEV uint32_t finite(uint32_t w, uint32_t exponent) {
-    if ((w & exponent) == exponent) w &= 0xffff0000u;
-    if ((w & exponent << 16) == exponent << 16) w &= 0xffffu;
-    return w;
 }
 
 // The whole CTA: the sequence that comes n-th by its length, longest first, so that the last CTAs to start are the

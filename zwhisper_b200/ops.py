@@ -1197,8 +1197,10 @@ class PagedCache:
         [n_batch] whose entries are at most max_past) over the cache, which holds the call's own tokens already:
         query i of sequence b sees slots first[b] .. n_past + i, or, with a tree (as in append), the past ones from
         first[b] on, its own and those of the tokens above it (none: zeros). count, first: CUDA int32 [n_batch]; rows
-        of out behind count[b] stay as they are. workspace: a contiguous CUDA tensor of attn_workspace_bytes
-        (None: one is made). Returns out, of q's shape and type (a new one has zeros there)."""
+        of out behind count[b] stay as they are. max_past (None: the cache's end) also sets how many parts the keys
+        are cut into: with one near the lengths that are there, calls take up to half the time. workspace: a contiguous
+        CUDA tensor of attn_workspace_bytes (None: one is made). Returns out, of q's shape and type (a new one has
+        zeros there; the rows of a sequence that is skipped as out of range are undefined in it)."""
         torch = _torch()
         kind = self._check_rows(q, "q")
         n, H = q.shape[1], q.shape[2]
