@@ -1101,9 +1101,9 @@ class PagedCache:
     """A key/value cache in pages (zwg_paged): K and V [n_pages][n_head_kv][page][d], both float16
     (for f32 rows) or both bfloat16 (for bf16 rows), d 64 or 128, page a power of two from 16 to 256, and
     an int32 table [n_batch][max_pages] of each sequence's pages (-1: none yet). CUDA tensors on one
-    device, which the cache keeps; a page's rows lie one after another, pages any distance apart that K and
-    V share, the table's rows too. Who hands out pages writes their numbers into the table before
-    the call that needs them."""
+    device, which the cache keeps and whose places it passes on (write into them, and make another cache for
+    other tensors); a page's rows lie one after another, pages any distance apart that K and V share, the
+    table's rows too. Who hands out pages writes their numbers into the table before the call that needs them."""
 
     def __init__(self, k, v, table):
         torch = _torch()
